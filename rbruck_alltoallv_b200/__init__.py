@@ -28,6 +28,9 @@ def __getattr__(name):
     if name in ("MoEExpertParallel", "grouped_gemm", "grouped_gemm_fp8"):
         from .ops import moe as _m
         return getattr(_m, name)
+    if name == "block_norm":
+        from .ops.norm import block_norm
+        return block_norm
     if name == "PencilTranspose":
         from .ops.fft import PencilTranspose
         return PencilTranspose

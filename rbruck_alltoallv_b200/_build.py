@@ -40,6 +40,7 @@ CUDA_SOURCES = [
     "kernels/grouped_gemm_mxfp8_sm100.cu",
     "kernels/fft_transpose.cu",
     "kernels/reshard.cu",
+    "kernels/block_norm.cu",
     "kernels/noalloc.cu",
     "api/c_api.cu",
     "api/tuner_native.cpp",
