@@ -16,16 +16,6 @@ class Box(C.Structure):
                 ("t2", C.c_longlong)]
 
 
-class BlockNorm(C.Structure):
-    """``rbv_norm_t``: one call of the norms around a block."""
-    _fields_ = ([("T", C.c_longlong)] + [(n, C.c_int) for n in ("H", "z_type", "r_type", "gate_kind", "w1_f32", "w2_f32", "gate_f32")]
-                + [("scale", C.c_float), ("eps", C.c_float)] + [(n, C.c_void_p) for n in ("z", "r", "w1", "gate", "w2")]
-                + [(n, C.c_longlong) for n in ("z_ld", "r_ld", "gate_ld")]
-                + [(n, C.c_void_p) for n in ("rstd1", "rstd2", "r2", "u", "dr2", "du")]
-                + [(n, C.c_longlong) for n in ("dr2_ld", "du_ld")]
-                + [(n, C.c_void_p) for n in ("dz", "dr", "dgate", "dw1", "dw2", "partial")])
-
-
 STATUS_NAMES = {0: "ok", 1: "timeout", 2: "bad_argument", 3: "staging_capacity", 4: "truncate", 5: "aborted"}
 SITE_NAMES = {0: "-", 1: "metadata", 2: "staging_cell", 3: "final_arrival", 4: "bulk_copy"}
 
@@ -91,8 +81,8 @@ def declare_cuda(lib):
     lib.rbv_ctx_set_eager.argtypes = [C.c_void_p, C.c_ulonglong]
     lib.rbv_ctx_set_cooperative.argtypes = [C.c_void_p, C.c_int]
     declare_moe(lib)
-    lib.rbv_block_norm.argtypes = [C.POINTER(BlockNorm), C.c_void_p]
-    lib.rbv_block_norm_backward.argtypes = [C.POINTER(BlockNorm), C.c_void_p]
+    lib.rbv_block_norm.argtypes = [C.c_char_p, C.c_void_p]
+    lib.rbv_block_norm_backward.argtypes = [C.c_char_p, C.c_void_p]
     lib.rbv_block_norm_parts.argtypes = [C.c_longlong, C.c_int, C.c_int]
     lib.rbv_reshard_heads.argtypes = [C.c_void_p, C.POINTER(C.c_void_p), C.POINTER(C.c_void_p), C.c_longlong,
                                       C.c_longlong, C.c_int, C.c_void_p]

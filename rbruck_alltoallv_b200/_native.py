@@ -91,10 +91,3 @@ def current_stream(device: int) -> int:
     raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
     return raw(device) if raw is not None else torch.cuda.current_stream(device).cuda_stream
 
-
-def on_device(device: int):
-    """Context in which launches go to a tensor's device (nothing to do where that is the current one)."""
-    import contextlib
-
-    import torch
-    return contextlib.nullcontext() if torch.cuda.current_device() == device else torch.cuda.device(device)

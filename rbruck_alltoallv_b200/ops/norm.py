@@ -9,27 +9,31 @@ With a block ``f`` between them, a layer of the network is::
 """
 from __future__ import annotations
 
-import ctypes as C
+import struct
 from typing import Optional, Tuple
 
 import torch
 
 from .. import _native
-from .._cuda_decl import BlockNorm
 
 _TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 _GATES = {"none": 0, "channel": 1, "token": 2, "full": 3}
 MAX_HIDDEN = 16384
 
 
-def _ptr(t: Optional[torch.Tensor]):
-    return t.data_ptr() if t is not None else None
+# rbv_norm_t as the C compiler lays it out.  (Packing it in one call takes a fraction of the time of a ctypes.Structure with
+# thirty fields; a call on a few tokens takes no longer on the GPU than its launch on the host.)
+_pack = struct.Struct("@q7i2f5P3q6P2q6P").pack
 
 
-def _rows(t: Optional[torch.Tensor], H: int):
+def _ptr(t: Optional[torch.Tensor]) -> int:
+    return t.data_ptr() if t is not None else 0
+
+
+def _rows(t: torch.Tensor, H: int):
     """``t`` as rows of H packed elements, and the distance between the rows."""
-    if t is None:
-        return None, 0
+    if t.is_contiguous():
+        return t, H
     if t.dim() != 2:
         t = t.reshape(-1, H)
     if t.stride(1) != 1 and H > 1:
@@ -37,40 +41,43 @@ def _rows(t: Optional[torch.Tensor], H: int):
     return t, t.stride(0) if t.shape[0] > 1 else H
 
 
-def _fill(residual, branch, post_weight, gate, kind, scale, pre_weight, eps):
-    """The call's argument block without its outputs, and the tensors that it points into."""
+def _inputs(residual, branch, post_weight, gate, kind, pre_weight):
+    """The argument block's fields up to its scale, and from z to the row distances; the tensors that they point into."""
     H = residual.shape[-1]
+    f32 = torch.float32
     r, r_ld = _rows(residual, H)
-    z, z_ld = _rows(branch, H)
-    g, g_ld = _rows(gate, H) if kind == "full" else (gate.contiguous() if gate is not None else None, 0)
+    z, z_ld = _rows(branch, H) if branch is not None else (None, 0)
+    g, g_ld = (None, 0) if gate is None else _rows(gate, H) if kind == 3 else (gate.contiguous(), 0)
     w1 = post_weight.contiguous() if post_weight is not None else None
     w2 = pre_weight.contiguous() if pre_weight is not None else None
-    ztype = (branch if branch is not None else residual).dtype
-    f32 = torch.float32
-    a = BlockNorm(T=r.shape[0], H=H, z_type=_TYPES[ztype], r_type=_TYPES[residual.dtype], gate_kind=_GATES[kind],
-                  w1_f32=w1 is not None and w1.dtype == f32, w2_f32=w2 is not None and w2.dtype == f32,
-                  gate_f32=g is not None and g.dtype == f32, scale=scale, eps=eps, z=_ptr(z), r=_ptr(r), w1=_ptr(w1),
-                  gate=_ptr(g), w2=_ptr(w2), z_ld=z_ld, r_ld=r_ld, gate_ld=g_ld)
-    return a, (r, z, g, w1, w2)
+    head = (residual.numel() // H, H, _TYPES[residual.dtype if z is None else z.dtype], _TYPES[residual.dtype], kind,
+            w1 is not None and w1.dtype is f32, w2 is not None and w2.dtype is f32, g is not None and g.dtype is f32)
+    return head, (_ptr(z), r.data_ptr(), _ptr(w1), _ptr(g), _ptr(w2), z_ld, r_ld, g_ld), (r, z, g, w1, w2)
+
+
+def _launch(entry, call, device, what):
+    index = device.index
+    if torch.cuda.current_device() == index:
+        rc = entry(call, _native.current_stream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = entry(call, _native.current_stream(index))
+    if rc:
+        raise RuntimeError(f"{what} launch failed (CUDA error {rc})")
 
 
 def _forward(residual, branch, post_weight, gate, kind, scale, pre_weight, eps, stats):
-    a, held = _fill(residual, branch, post_weight, gate, kind, scale, pre_weight, eps)
-    dev = residual.device
-    r2 = torch.empty(residual.shape, dtype=residual.dtype, device=dev) if branch is not None else None
-    u = None
-    if pre_weight is not None:
-        u = torch.empty(residual.shape, dtype=residual.dtype if branch is None else branch.dtype, device=dev)
-    rstd = torch.empty(2, a.T, dtype=torch.float32, device=dev) if stats else None
-    a.r2, a.u = _ptr(r2), _ptr(u)
+    head, body, held = _inputs(residual, branch, post_weight, gate, kind, pre_weight)
+    T = head[0]
+    r2 = residual.new_empty(residual.shape) if branch is not None else None
+    u = (residual if branch is None else branch).new_empty(residual.shape) if pre_weight is not None else None
+    rstd, at = None, 0
     if stats:
-        a.rstd1, a.rstd2 = rstd.data_ptr(), rstd.data_ptr() + 4 * a.T
-    if a.T:
-        lib = _native.cuda_lib()
-        with _native.on_device(dev.index):
-            rc = lib.rbv_block_norm(C.byref(a), _native.current_stream(dev.index))
-        if rc:
-            raise RuntimeError(f"block norm launch failed (CUDA error {rc})")
+        rstd = torch.empty(2 * T, dtype=torch.float32, device=residual.device)
+        at = rstd.data_ptr()
+    if T:
+        call = _pack(*head, scale, eps, *body, at, at + 4 * T if stats else 0, _ptr(r2), _ptr(u), 0, 0, 0, 0, 0, 0, 0, 0, 0, 0)
+        _launch(_native.cuda_lib().rbv_block_norm, call, residual.device, "block norm")
     del held
     return r2, u, rstd
 
@@ -91,29 +98,24 @@ class _BlockNormFunction(torch.autograd.Function):
         kind, scale, eps = ctx.call
         if d_r2 is None and d_u is None:
             return (None,) * 8
-        a, held = _fill(residual, branch, post_weight, gate, kind, scale, pre_weight, eps)
-        T, H, dev = a.T, a.H, residual.device
-        dr2, a.dr2_ld = _rows(d_r2, H)
-        du, a.du_ld = _rows(d_u, H)
-        a.dr2, a.du = _ptr(dr2), _ptr(du)
-        a.rstd1, a.rstd2 = rstd.data_ptr(), rstd.data_ptr() + 4 * T
         need_r, need_z, need_w1, need_gate, need_w2 = ctx.needs_input_grad[:5]
+        head, body, held = _inputs(residual, branch, post_weight, gate, kind, pre_weight)
+        T, H = head[:2]
 
         def grad(t, needed):
-            return (torch.empty if T else torch.zeros)(t.shape, dtype=t.dtype, device=dev) if needed and t is not None else None
-        dr, dz = grad(residual, need_r), grad(branch, need_z)
-        dw1, dgate, dw2 = grad(post_weight, need_w1), grad(gate, need_gate), grad(pre_weight, need_w2 and d_u is not None)
-        a.dr, a.dz, a.dw1, a.dgate, a.dw2 = _ptr(dr), _ptr(dz), _ptr(dw1), _ptr(dgate), _ptr(dw2)
-        if T == 0:
-            return dr, dz, dw1, dgate, dw2, None, None, None
-        lib = _native.cuda_lib()
-        with _native.on_device(dev.index):
-            if dw1 is not None or dw2 is not None or (dgate is not None and kind == "channel"):
-                partial = torch.empty(lib.rbv_block_norm_parts(T, H, a.z_type), 2, H, dtype=torch.float32, device=dev)
-                a.partial = partial.data_ptr()
-            rc = lib.rbv_block_norm_backward(C.byref(a), _native.current_stream(dev.index))
-        if rc:
-            raise RuntimeError(f"block norm backward launch failed (CUDA error {rc})")
+            return (t.new_empty if T else t.new_zeros)(t.shape) if needed else None
+        dr, dz, dw1 = grad(residual, need_r), grad(branch, need_z), grad(post_weight, need_w1)
+        dgate, dw2 = grad(gate, need_gate), grad(pre_weight, need_w2 and d_u is not None)
+        if T:
+            dr2, dr2_ld = _rows(d_r2, H) if d_r2 is not None else (None, 0)
+            du, du_ld = _rows(d_u, H) if d_u is not None else (None, 0)
+            lib, partial = _native.cuda_lib(), None
+            if dw1 is not None or dw2 is not None or (dgate is not None and kind == _GATES["channel"]):
+                partial = rstd.new_empty(2 * H * lib.rbv_block_norm_parts(T, H, head[2]))
+            at = rstd.data_ptr()
+            call = _pack(*head, scale, eps, *body, at, at + 4 * T, 0, 0, _ptr(dr2), _ptr(du), dr2_ld, du_ld, _ptr(dz), _ptr(dr),
+                         _ptr(dgate), _ptr(dw1), _ptr(dw2), _ptr(partial))
+            _launch(lib.rbv_block_norm_backward, call, residual.device, "block norm backward")
         del held
         return dr, dz, dw1, dgate, dw2, None, None, None
 
@@ -148,12 +150,9 @@ def _check(residual, branch, post_weight, gate, scale, pre_weight, eps):
         if t is not None and t.device != residual.device:
             raise ValueError("all tensors must be on one device")
     if gate is not None:
-        try:
-            fits = torch.broadcast_shapes(gate.shape, residual.shape) == residual.shape
-        except RuntimeError:
-            fits = False
-        if not fits:
-            raise ValueError(f"a gate {tuple(gate.shape)} does not broadcast to {tuple(residual.shape)}")
+        g = gate.shape
+        if len(g) > residual.dim() or any(n != 1 and n != m for n, m in zip(reversed(g), reversed(residual.shape))):
+            raise ValueError(f"a gate {tuple(g)} does not broadcast to {tuple(residual.shape)}")
     if not eps >= 0.0:
         raise ValueError("eps must not be negative")
     if not residual.is_cuda:
@@ -176,16 +175,16 @@ def block_norm(residual: torch.Tensor, branch: Optional[torch.Tensor] = None, po
     _check(residual, branch, post_weight, gate, scale, pre_weight, eps)
     kind = "none"
     if gate is not None:
-        shape, lead = gate.shape, residual.shape[:-1]
-        if shape == residual.shape[-1:]:
+        shape, full = gate.shape, residual.shape
+        if shape == full[-1:]:
             kind = "channel"
-        elif shape == lead + (1,):
+        elif shape == full[:-1] + (1,):
             kind = "token"
         else:
             kind = "full"
-            if shape != residual.shape:
-                gate = gate.expand(residual.shape)
-    scale, eps = float(scale), float(eps)
+            if shape != full:
+                gate = gate.expand(full)
+    kind, scale, eps = _GATES[kind], float(scale), float(eps)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (residual, branch, post_weight, gate, pre_weight)):
         r2, u = _BlockNormFunction.apply(residual, branch, post_weight, gate, pre_weight, kind, scale, eps)
     else:
