@@ -32,6 +32,7 @@ CUDA_SOURCES = [
     "kernels/a2av_local.cu",
     "kernels/moe_kernels.cu",
     "kernels/moe_local.cu",
+    "kernels/moe_few.cu",
     "kernels/grouped_gemm_sm100.cu",
     "kernels/grouped_gemm_pair_sm100.cu",
     "kernels/grouped_gemm_fp8_sm100.cu",

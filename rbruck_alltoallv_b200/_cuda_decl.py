@@ -117,6 +117,9 @@ def declare_moe(lib):
     lib.rbv_moe_route_local.argtypes = [vp, vp, i, i, i, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp]
     lib.rbv_moe_dispatch_local.argtypes = [vp, vp, i, i, vp, vp, vp, vp, vp, i, vp, vp, ll, vp, vp]
     lib.rbv_moe_combine_local.argtypes = [vp, vp, i, i, vp, vp, vp, vp]
+    lib.rbv_moe_few_workspace.restype = ll
+    lib.rbv_moe_few_workspace.argtypes = [i] * 5
+    lib.rbv_moe_few_tokens.argtypes = [vp, ll, vp, ll, i, i, i, i, i, vp, vp, vp, vp, vp, vp]
     lib.rbv_moe_route.argtypes = [vp, i, i, vp, vp, vp, vp]
     lib.rbv_moe_layout.argtypes = [vp, i, i, i, vp, vp, vp, vp, vp, vp]
     lib.rbv_moe_layout_aligned.argtypes = [vp, i, i, i, vp, vp, vp, vp, vp, i, vp]

@@ -10,7 +10,7 @@
 #include "rbv/rbruckv.h"
 
 #ifdef __cplusplus
-namespace rbv { constexpr int kMoeMaxGroups = 64; constexpr int kMoeMaxExperts = 256; }
+namespace rbv { constexpr int kMoeMaxGroups = 64; constexpr int kMoeMaxExperts = 256; constexpr int kMoeFewMaxTopK = 8; }
 extern "C" {
 #endif
 
@@ -82,6 +82,19 @@ int rbv_quantize_rows_fp8(const void* x_bf16, long long rows, int K, int ldx, vo
  * case and usually holds half of that. */
 int rbv_quantize_used_rows_fp8(const void* x_bf16, long long rows, const int* used, int K, int ldx, void* out_fp8,
                                float* scale_t, void* cuda_stream);
+
+/* A whole layer for a few tokens (1 <= T <= 64) with every expert on this GPU, in two kernels: choice of the top_k (<= 8)
+ * largest of E (<= 256) logits per token (ties: lower expert; -inf is never chosen, a token without any other logit gets a
+ * row of zeros; a NaN counts as largest and makes the token's row NaN), softmax over the chosen ones, SwiGLU FFN, weighted sum.
+ *   x [T, H] bf16, rows ldx elements apart (a multiple of 8);  logits [T, E] fp32, rows ldl apart;
+ *   w13 [E, 2 I, H] bf16 with gate and up rows interleaved;  w2 [E, H, I] bf16;  out [T, H] bf16.  H % 8 == 0, I % 8 == 0.
+ *   workspace: rbv_moe_few_workspace(...) bytes of this call alone (nothing in it has to be set; -1 for sizes that are not
+ *   taken).  error_flag: device int, may be null; set if a bounded wait ran out.
+ * Both results are for the current device.  Returns 0 or a CUDA error code. */
+long long rbv_moe_few_workspace(int T, int H, int I, int E, int top_k);
+int rbv_moe_few_tokens(const void* x, long long ldx, const float* logits, long long ldl, int T, int H, int I, int E,
+                       int top_k, const void* w13, const void* w2, void* out, void* workspace, int* error_flag,
+                       void* cuda_stream);
 
 /* Router: softmax over E logits per token, top-2, weights renormalised to sum to one.
  *   logits [T, E] fp32;  topk_idx [T, 2] int32;  topk_w [T, 2] fp32;  hist [E] int32 (zeroed by the call). */

@@ -1,0 +1,298 @@
+// Matrix products of a few rows (1 to 64) with large weights, bound by reading the weights once: the parts that the
+// few-token MoE layer (bf16) and the 8-bit integer linear share.
+//
+//   D[row][n] = sum_k A[row][k] W[n][k]
+//
+// A CTA streams pieces of W through a ring in shared memory.  One producer warp fetches, for `nr` weight rows (a multiple
+// of 8, at most 64) and a chunk of 512 bytes along K, four columns of 128 bytes with TMA, all four in one box of 64, 32, 16
+// or 8 rows (K beyond the end reads as zero).  Each of eight consumer warps takes one column, and half of the weight rows or of the
+// rows of A; the sums of the four columns are added when the K range of a piece is done.  A rows come from L2 straight into
+// the registers of the lanes that multiply with them, one chunk ahead (up to 32 rows).
+//
+// The rows of A are the M (16) of mma.sync and the weight rows its N (8): few rows waste multiplications, which are free
+// here, and not memory traffic, and a CTA's share of the weights can be cut at any multiple of 8 rows.  (tcgen05 would take
+// the weights as M, in tiles of 64 or more rows: for one token and two of 64 experts that is 44 tiles of 128 rows for 148
+// SMs.)  The order of K is free as long as A and W agree: lane t of a row has bytes 32 t to 32 t + 31 of its column, in two
+// halves of 16 consecutive bytes, each of which feeds two multiplications, so every operand is one 16-byte load.  Half s of
+// all rows lies in the 16-byte units 2 t + s, which the 128-byte swizzle (unit ^ row % 8) puts into different banks for the
+// two rows that a quarter of a warp reads at a time.
+//
+// One bulk copy per weight row and chunk in place of the boxes reached a quarter of the bandwidth: 401 us against 125 for one
+// token of a layer that reads 704 MB.
+#pragma once
+#include <cstdint>
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+
+#include "kernels/sm100_ptx.cuh"
+
+namespace rbv {
+namespace few {
+
+constexpr int kChunk = 512;               // bytes of a row per stage
+constexpr int kCols = 4;                  // columns of 128 bytes in it
+constexpr int kWarps = 8;                 // consumer warps: kCols x 2
+constexpr int kThreads = (kWarps + 1) * 32;
+constexpr int kMaxRows = 64;              // rows of A
+constexpr int kMaxTile = 64;              // weight rows of a piece
+constexpr int kMaxStages = 32;
+
+// Boxes of 8, 16, 32 and 64 rows: `all` of four columns (the row seen as columns of 128 bytes, as many as it has whole ones),
+// `one` of a single column.
+struct WeightMaps {
+  CUtensorMap all[4], one[4];
+  int whole;                               // chunks that `all` covers; the rest of a row that does not end with a column: `one`
+};
+
+__device__ __forceinline__ uint4 lds16(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ void consumers_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
+
+// bf16 x bf16 -> fp32 (K 16) and s8 x s8 -> s32 (K 32): the same bytes per register.
+__device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+struct Ring {
+  uint64_t full[kMaxStages], empty[kMaxStages];
+  int abort;
+};
+
+struct Cursor {                            // a stage of the ring and its parity
+  int stage = 0;
+  uint32_t phase = 0;
+  __device__ __forceinline__ void next(int stages) {
+    if (++stage == stages) { stage = 0; phase ^= 1u; }
+  }
+};
+
+__device__ __forceinline__ void ring_init(Ring& ring, int stages) {      // one thread
+  for (int s = 0; s < stages; s++) { sm100::mbar_init(&ring.full[s], 1); sm100::mbar_init(&ring.empty[s], kWarps); }
+  ring.abort = 0;
+  sm100::mbar_fence_init();
+}
+
+// Shared memory of a CTA: the buffer in which warps add their sums, then the stages, 1024-byte aligned.
+__host__ __device__ inline uint32_t red_bytes(int tile) { return (uint32_t)tile * kWarps * 64; }
+__host__ __device__ inline uint32_t slot_bytes(int tile) { return (uint32_t)tile * kChunk; }
+
+// Fetches chunk c of `rows` weight rows from `row0` on into a stage: box by box, in a box column by column.  One thread.  A
+// thread gets a box on its way in 150 to 470 cycles, whatever its size, so there is one box per stage for 64 rows: with a box
+// per column the producer set the pace (205 us against 125 for one token of a layer that reads 704 MB).
+template <typename E>                      // element: its size turns bytes along K into coordinates
+__device__ __forceinline__ void fetch_weights(const WeightMaps& maps, uint8_t* slot, int row0, int rows, int c, uint64_t* bar) {
+  sm100::mbar_arrive_expect_tx(bar, (uint32_t)rows * kChunk);
+  int at = 0;
+  #pragma unroll 1
+  for (int b = 3; b >= 0; b--) {
+    if (!(rows & (8 << b))) continue;
+    if (c < maps.whole) sm100::tma_load_3d(slot + at * kChunk, &maps.all[b], 0, row0 + at, c * kCols, bar);
+    else
+      for (int j = 0; j < kCols; j++)
+        sm100::tma_load_2d(slot + at * kChunk + j * (128 * (8 << b)), &maps.one[b], (c * kChunk + j * 128) / (int)sizeof(E), row0 + at, bar);
+    at += 8 << b;
+  }
+}
+
+// Where in a stage of `rows` weight rows the 8 rows of group g are, column j.
+__device__ __forceinline__ uint32_t group_offset(int rows, int g, int j) {
+  int at = 0, n = 0;
+  #pragma unroll
+  for (int b = 3; b >= 0; b--) {
+    if (g * 8 < at + n) break;             // (n: rows of the box that ends at `at + n`)
+    at += n;
+    n = rows & (8 << b);
+  }
+  return (uint32_t)(at * kChunk + j * n * 128 + (g * 8 - at) * 128);
+}
+
+// What the two warps of a column divide between them: the weight rows (at most 16 MT rows of A, in both), or the rows of A
+// (HALVES: 32 of at most 64 each; the accumulators of 64 by 64 would not fit a warp's registers).
+template <int MT_, bool HALVES_>
+struct Spread {
+  static constexpr int MT = MT_;
+  static constexpr bool HALVES = HALVES_;
+  static constexpr int SETS = HALVES ? 2 : 1;
+  static constexpr bool AHEAD = !HALVES;   // rows of A one chunk ahead; with HALVES the registers do not suffice
+  static constexpr int GROUPS = HALVES ? kMaxTile / 8 : kMaxTile / 16;      // groups of 8 weight rows of a warp, at most
+  // row of A of tile m, upper or lower half h of a warp in part q
+  __device__ static __forceinline__ int row(int m, int q, int h, int lane) { return 16 * (m + q * MT) + 8 * h + (lane >> 2); }
+  __device__ static __forceinline__ int set(int part) { return HALVES ? part : 0; }
+  __device__ static __forceinline__ int group0(int part, int groups) { return HALVES ? 0 : part * ((groups + 1) / 2); }
+  __device__ static __forceinline__ int my_groups(int part, int groups) {
+    return HALVES ? groups : part ? groups - (groups + 1) / 2 : (groups + 1) / 2;
+  }
+};
+
+// A lane's part of the rows of A for one chunk: 32 bytes of each of its rows.
+template <typename S>
+struct Rows {
+  uint4 v[S::MT][2][2];                    // tile, half of the tile, half of the 32 bytes
+  // `src`: the rows, null for those that do not exist (they count as zeros); CACHED: through L1 (nobody writes them meanwhile)
+  template <bool CACHED>
+  __device__ __forceinline__ void load(const uint8_t* const (&src)[S::MT][2], long long row_bytes, int c, int col, int lane) {
+    const long long k = (long long)c * kChunk + col * 128 + (lane & 3) * 32;
+    #pragma unroll
+    for (int m = 0; m < S::MT; m++)
+      #pragma unroll
+      for (int h = 0; h < 2; h++)
+        #pragma unroll
+        for (int s = 0; s < 2; s++) {
+          v[m][h][s] = make_uint4(0u, 0u, 0u, 0u);
+          if (src[m][h] && k + 16 * s < row_bytes) {
+            const uint4* p = reinterpret_cast<const uint4*>(src[m][h] + k + 16 * s);
+            v[m][h][s] = CACHED ? __ldg(p) : __ldcg(p);
+          }
+        }
+  }
+};
+
+template <typename S, typename Acc>
+__device__ __forceinline__ void clear(Acc (&acc)[S::MT][S::GROUPS][4]) {
+  #pragma unroll
+  for (int m = 0; m < S::MT; m++)
+    #pragma unroll
+    for (int n = 0; n < S::GROUPS; n++)
+      #pragma unroll
+      for (int k = 0; k < 4; k++) acc[m][n][k] = 0;
+}
+
+// One stage's part of a warp: `groups` groups of 8 weight rows, the n-th at w + off[n].  Groups that do not exist are
+// multiplied as zeros: without branches all loads are on their way before the first multiplication and the chains of different
+// groups overlap.
+template <typename S, typename Acc>
+__device__ __forceinline__ void multiply(Acc (&acc)[S::MT][S::GROUPS][4], uint32_t w, const uint32_t (&off)[S::GROUPS], int groups,
+                                         const Rows<S>& a, int lane) {
+  const uint32_t row = (uint32_t)lane >> 2, t = (uint32_t)lane & 3;
+  const uint32_t wl = w + row * 128u;
+  const uint32_t unit[2] = {((2u * t) ^ row) << 4, ((2u * t + 1u) ^ row) << 4};
+  constexpr int SETS = S::GROUPS / 4;      // four groups at a time
+  #pragma unroll
+  for (int q = 0; q < SETS; q++) {
+    uint4 b[4][2];
+    #pragma unroll
+    for (int n = 0; n < 4; n++)
+      #pragma unroll
+      for (int s = 0; s < 2; s++) {
+        b[n][s] = make_uint4(0u, 0u, 0u, 0u);
+        if (4 * q + n < groups) b[n][s] = lds16(wl + off[4 * q + n] + unit[s]);
+      }
+    #pragma unroll
+    for (int s = 0; s < 2; s++)
+      #pragma unroll
+      for (int half = 0; half < 2; half++)
+        #pragma unroll
+        for (int m = 0; m < S::MT; m++)
+          #pragma unroll
+          for (int n = 0; n < 4; n++) {
+            const uint4 &lo = a.v[m][0][s], &hi = a.v[m][1][s];
+            if (half == 0) mma(acc[m][4 * q + n], lo.x, hi.x, lo.y, hi.y, b[n][s].x, b[n][s].y);
+            else mma(acc[m][4 * q + n], lo.z, hi.z, lo.w, hi.w, b[n][s].z, b[n][s].w);
+          }
+  }
+}
+
+// Adds the columns' sums of a tile of 16 rows of A per set; thread (n = warp, lane) gets those of rows S::row(m, q, 0 and 1,
+// lane) (v[q][0..1], v[q][2..3]) and of weight rows 8 n + 2 (lane % 4) and + 1.  All consumers call it; `red` holds 16 bytes
+// per lane, group and warp.
+template <typename S, typename Acc>
+__device__ __forceinline__ void add_columns(const Acc (&acc)[S::GROUPS][4], uint4* red, int groups, int warp, int lane, Acc (&v)[S::SETS][4]) {
+  const int part = warp >> 2, col = warp & 3, g0 = S::group0(part, groups), mine = S::my_groups(part, groups);
+  #pragma unroll
+  for (int n = 0; n < S::GROUPS; n++)
+    if (n < mine) red[(((g0 + n) * S::SETS + S::set(part)) * kCols + col) * 32 + lane] = *reinterpret_cast<const uint4*>(acc[n]);
+  consumers_sync();
+  #pragma unroll
+  for (int q = 0; q < S::SETS; q++) {
+    #pragma unroll
+    for (int k = 0; k < 4; k++) v[q][k] = 0;
+    if (warp < groups)
+      #pragma unroll
+      for (int j = 0; j < kCols; j++) {
+        const uint4 u = red[((warp * S::SETS + q) * kCols + j) * 32 + lane];
+        const Acc* p = reinterpret_cast<const Acc*>(&u);
+        #pragma unroll
+        for (int k = 0; k < 4; k++) v[q][k] += p[k];
+      }
+  }
+  consumers_sync();
+}
+
+// ---- work split along K over CTAs ------------------------------------------------------------------------------------
+// `total` steps (tile by tile, each of `per_tile` steps along K) are cut into `parts` <= total contiguous ranges of equal
+// length (within one).  A tile whose steps lie in several ranges is finished by the last of their CTAs to arrive, which adds
+// the others' sums in the order of the ranges: the result does not depend on who that is.
+struct Split {
+  long long total;
+  int parts;
+  __device__ __forceinline__ long long begin(int part) const { return (long long)part * total / parts; }
+  __device__ __forceinline__ int owner(long long step) const { return (int)(((step + 1) * parts - 1) / total); }
+};
+
+// Whether this CTA is the one to finish the tile, of `pieces`.  (All consumers call it, after their stores to the workspace.)
+__device__ __forceinline__ bool last_to_arrive(int* counter, int pieces, int* s_flag) {
+  __threadfence();
+  consumers_sync();
+  if (threadIdx.x == 0) *s_flag = atomicAdd(counter, 1) == pieces - 1;
+  consumers_sync();
+  const bool last = *s_flag != 0;
+  if (last) __threadfence();
+  return last;
+}
+
+// ---- host side -------------------------------------------------------------------------------------------------------
+// Weight rows of a piece: an even share of `groups` groups of 8 among `parts`, at most 64 rows.
+inline int tile_rows(long long groups, int parts) {
+  const long long n = (groups + parts - 1) / parts;
+  return (int)(n < 1 ? 8 : n > kMaxTile / 8 ? kMaxTile : n * 8);
+}
+
+// Stages that fit beside `fixed` bytes of static shared memory.
+inline int ring_stages(int tile, size_t fixed) {
+  const size_t room = 227 * 1024 - 1024 /*alignment*/ - fixed - red_bytes(tile), n = room / slot_bytes(tile);
+  return n > (size_t)kMaxStages ? kMaxStages : (int)n;
+}
+inline size_t ring_smem(int tile, int stages) { return 1024 + red_bytes(tile) + (size_t)slot_bytes(tile) * stages; }
+
+// Weights of `rows` rows of row_bytes (a multiple of 16) each, elements of `size` bytes; 128-byte swizzle.
+inline bool weight_maps(WeightMaps* m, const void* base, unsigned long long rows, unsigned long long row_bytes, CUtensorMapDataType type,
+                        int size) {
+  typedef CUresult (*Encode)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                             const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+  static const Encode encode = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    return cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess
+               ? reinterpret_cast<Encode>(p) : nullptr;
+  }();
+  if (!encode) return false;
+  const unsigned per_col = 128u / (unsigned)size;
+  const cuuint64_t cols = row_bytes / 128;                 // whole columns
+  const bool even = row_bytes % 128 == 0;
+  m->whole = (int)(even ? (cols + kCols - 1) / kCols : cols / kCols);      // (columns behind the last one read as zeros)
+  const cuuint64_t dims3[3] = {per_col, rows, cols}, strides3[2] = {row_bytes, 128};
+  const cuuint64_t dims2[2] = {row_bytes / size, rows}, strides2[1] = {row_bytes};
+  const cuuint32_t ones[3] = {1, 1, 1};
+  for (int b = 0; b < 4; b++) {
+    const cuuint32_t box3[3] = {per_col, 8u << b, (cuuint32_t)kCols}, box2[2] = {per_col, 8u << b};
+    if (m->whole > 0 && encode(&m->all[b], type, 3, const_cast<void*>(base), dims3, strides3, box3, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+      return false;
+    if (!even && encode(&m->one[b], type, 2, const_cast<void*>(base), dims2, strides2, box2, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+      return false;
+  }
+  return true;
+}
+
+}  // namespace few
+}  // namespace rbv

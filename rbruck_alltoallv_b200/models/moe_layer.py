@@ -17,12 +17,19 @@ class MoELayer:
         self.ep = MoEExpertParallel(comm, num_experts, hidden, inter, tokens, **kw)
         self.router_weight = router_weight
 
-    def forward(self, x, logits=None):
+    def _logits(self, x, logits):
         if logits is None:
             if self.router_weight is None:
                 raise ValueError("either logits or a router weight is needed")
             logits = (x.float() @ self.router_weight.float().t()).contiguous()
-        return self.ep.forward(x, logits)
+        return logits
+
+    def forward(self, x, logits=None):
+        return self.ep.forward(x, self._logits(x, logits))
+
+    def decode(self, x, logits=None):
+        """The same layer for a few decoded tokens, however many (see :meth:`MoEExpertParallel.decode`)."""
+        return self.ep.decode(x, self._logits(x, logits))
 
     __call__ = forward
 

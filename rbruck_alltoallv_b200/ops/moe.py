@@ -272,6 +272,65 @@ def pack_gate_up(gate: torch.Tensor, up: torch.Tensor) -> torch.Tensor:
     return torch.stack([gate, up], dim=2).reshape(G, 2 * I, H).contiguous()
 
 
+FEW_TOKENS = 64            # tokens that moe_few_tokens takes at most
+FEW_MAX_TOP_K = 8
+
+
+def moe_few_tokens(x: torch.Tensor, logits: torch.Tensor, w13: torch.Tensor, w2: torch.Tensor, top_k: int = 2,
+                   out: Optional[torch.Tensor] = None, error: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """A whole routed SwiGLU layer for a handful of tokens with every expert on this GPU, in two kernels
+    (``csrc/kernels/moe_few.cu``): ``out[t] = sum_j p_tj * W2_e (silu(W1gate_e x_t) * (W1up_e x_t))`` over the ``top_k`` experts
+    ``e`` with the largest logits of token t (ties: the lower expert), ``p`` their softmax.
+
+    ``x`` [T, H] bf16 with 1 to 64 tokens (0: an empty result), ``logits`` [T, E] fp32, ``w13`` [E, 2 I, H] bf16 with gate and up
+    rows interleaved (:func:`pack_gate_up`), ``w2`` [E, H, I] bf16; H and I multiples of 8, E <= 256, ``top_k`` <= 8.  Rows of
+    ``x`` and ``logits`` may be strided.  A logit of -inf masks its expert: it is never taken, a token with fewer others than
+    ``top_k`` is spread over those, and one without any other gets a row of zeros (a padded slot of a batch).  A NaN among a
+    token's logits makes its row NaN.  The number of tokens may change from call to call; weights are read for the experts that
+    some token chooses, once each.  ``error`` (int32 CUDA tensor): set to non-zero if a bounded wait ran out."""
+    if x.dim() != 2 or logits.dim() != 2 or w13.dim() != 3 or w2.dim() != 3:
+        raise ValueError("x [T, H], logits [T, E], w13 [E, 2 I, H] and w2 [E, H, I] are wanted")
+    T, H = x.shape
+    E, _, I = w2.shape
+    if x.dtype != torch.bfloat16 or w13.dtype != torch.bfloat16 or w2.dtype != torch.bfloat16 or logits.dtype != torch.float32:
+        raise ValueError("x and the weights must be bf16, the logits fp32")
+    if logits.shape != (T, E) or w13.shape != (E, 2 * I, H) or w2.shape[1] != H:
+        raise ValueError(f"shapes do not fit: x {tuple(x.shape)}, logits {tuple(logits.shape)}, w13 {tuple(w13.shape)}, "
+                         f"w2 {tuple(w2.shape)}")
+    if T > FEW_TOKENS:
+        raise ValueError(f"{T} tokens: moe_few_tokens takes at most {FEW_TOKENS}; MoEExpertParallel.forward is for more")
+    if H < 8 or I < 8 or H % 8 or I % 8 or not 1 <= E <= 256 or not 1 <= top_k <= min(FEW_MAX_TOP_K, E):
+        raise ValueError(f"hidden {H} and FFN width {I} must be multiples of 8, experts {E} at most 256, top_k {top_k} at most "
+                         f"{FEW_MAX_TOP_K} and the experts")
+    if not (w13.is_contiguous() and w2.is_contiguous()) or (w13.data_ptr() | w2.data_ptr()) % 16:
+        raise ValueError("the weights must be contiguous and 16-byte aligned")
+    if not x.is_cuda or any(t.device != x.device for t in (logits, w13, w2)):
+        raise ValueError("all tensors must be on one GPU")
+    if out is None:
+        out = torch.empty(T, H, dtype=torch.bfloat16, device=x.device)
+    elif out.shape != (T, H) or out.dtype != torch.bfloat16 or not out.is_contiguous() or out.device != x.device or out.data_ptr() % 16:
+        raise ValueError("out must be a contiguous, 16-byte aligned bf16 tensor [T, H] on the same GPU")
+    if T == 0:
+        return out
+    if x.stride(1) != 1 or x.data_ptr() % 16 or (T > 1 and (x.stride(0) % 8 or x.stride(0) < H)):
+        x = x.clone(memory_format=torch.contiguous_format)
+    if (logits.stride(1) != 1 and E > 1) or (T > 1 and logits.stride(0) < E):
+        logits = logits.contiguous()
+    index = x.device.index
+    if torch.cuda.current_device() != index:
+        with torch.cuda.device(index):
+            return moe_few_tokens(x, logits, w13, w2, top_k, out, error)
+    lib = _native.cuda_lib()
+    # the workspace belongs to this call alone: calls on other streams and captured ones have their own
+    ws = torch.empty(lib.rbv_moe_few_workspace(T, H, I, E, top_k), dtype=torch.uint8, device=x.device)
+    rc = lib.rbv_moe_few_tokens(x.data_ptr(), x.stride(0) if T > 1 else H, logits.data_ptr(), logits.stride(0) if T > 1 else E, T, H,
+                                I, E, top_k, w13.data_ptr(), w2.data_ptr(), out.data_ptr(), ws.data_ptr(), _p(error),
+                                _native.current_stream(index))
+    if rc:
+        raise RuntimeError(f"few-token MoE launch failed (CUDA error {rc})")
+    return out
+
+
 class MoEExpertParallel:
     """One MoE FFN layer sharded by experts over the ranks of a communicator (one rank per GPU)."""
 
@@ -450,6 +509,13 @@ class MoEExpertParallel:
             self._check(lib.rbv_moe_combine(ctx, _p(out), T, H, _p(self.topk_idx), _p(self.topk_w), _p(self.slot),
                                             self.y_off, self.E, _p(self.error[3:4]), st), "combine")
         return out
+
+    def decode(self, x: torch.Tensor, logits: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """The layer for a batch of decoded tokens: any number of them up to :data:`FEW_TOKENS`, whatever ``tokens`` the layer
+        was made for, in two kernels (:func:`moe_few_tokens`).  bf16 experts on one rank."""
+        if self.P != 1 or self.fp8:
+            raise ValueError("decode() is for bf16 experts on one rank")
+        return moe_few_tokens(x, logits, self.w13, self.w2, 2, out, self.error[1:2])
 
     def _layout_and_dispatch(self, x, st):
         lib, ctx, T, H = self.lib, self.comm._ctx, self.T, self.H

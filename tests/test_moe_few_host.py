@@ -1,0 +1,35 @@
+"""The few-token MoE layer without a GPU: what is refused."""
+import pytest
+import torch
+
+from rbruck_alltoallv_b200.ops.moe import moe_few_tokens
+
+BF = torch.bfloat16
+
+
+def _args(T=3, H=16, I=24, E=4):
+    return dict(x=torch.zeros(T, H, dtype=BF), logits=torch.zeros(T, E), w13=torch.zeros(E, 2 * I, H, dtype=BF),
+                w2=torch.zeros(E, H, I, dtype=BF))
+
+
+@pytest.mark.parametrize("change,words", [
+    (dict(x=torch.zeros(16, dtype=BF)), "are wanted"),
+    (dict(x=torch.zeros(3, 16)), "must be bf16"),
+    (dict(logits=torch.zeros(3, 4, dtype=BF)), "logits fp32"),
+    (dict(logits=torch.zeros(3, 5)), "do not fit"),
+    (dict(w13=torch.zeros(4, 24, 16, dtype=BF)), "do not fit"),
+    (dict(w2=torch.zeros(4, 8, 24, dtype=BF)), "do not fit"),
+    (_args(T=65), "at most 64"),
+    (_args(H=12), "multiples of 8"),
+    (_args(I=20), "multiples of 8"),
+    (_args(E=257), "at most 256"),
+    (dict(top_k=0), "top_k"),
+    (dict(top_k=5), "top_k"),
+    ({**_args(E=16), "top_k": 9}, "top_k"),
+    (dict(w2=torch.zeros(4, 24, 16, dtype=BF).transpose(1, 2)), "contiguous"),
+    (dict(w13=torch.zeros(4 * 48 * 16 + 1, dtype=BF)[1:].view(4, 48, 16)), "16-byte aligned"),
+    (dict(), "on one GPU"),
+])
+def test_refusals(change, words):
+    with pytest.raises(ValueError, match=words):
+        moe_few_tokens(**{**_args(), **change})
