@@ -6,8 +6,9 @@
 // A CTA streams pieces of W through a ring in shared memory.  One producer warp fetches, for `nr` weight rows (a multiple
 // of 8, at most 64) and a chunk of 512 bytes along K, four columns of 128 bytes with TMA, all four in one box of 64, 32, 16
 // or 8 rows (K beyond the end reads as zero).  Each of eight consumer warps takes one column, and half of the weight rows or of the
-// rows of A; the sums of the four columns are added when the K range of a piece is done.  A rows come from L2 straight into
-// the registers of the lanes that multiply with them, one chunk ahead (up to 32 rows).
+// rows of A; the sums of the four columns are added when the K range of a piece is done.  The rows of A come from L2, either
+// straight into the registers of the lanes that multiply with them, a chunk or two ahead, or, where they lie one behind the
+// other, with TMA through the ring (a second producer): under load L2 takes longer than a stage.
 //
 // The rows of A are the M (16) of mma.sync and the weight rows its N (8): few rows waste multiplications, which are free
 // here, and not memory traffic, and a CTA's share of the weights can be cut at any multiple of 8 rows.  (tcgen05 would take
@@ -33,7 +34,7 @@ namespace few {
 constexpr int kChunk = 512;               // bytes of a row per stage
 constexpr int kCols = 4;                  // columns of 128 bytes in it
 constexpr int kWarps = 8;                 // consumer warps: kCols x 2
-constexpr int kThreads = (kWarps + 1) * 32;
+constexpr int kThreads = (kWarps + 2) * 32;         // and two producers, one for the weights and one for the rows of A
 constexpr int kMaxRows = 64;              // rows of A
 constexpr int kMaxTile = 64;              // weight rows of a piece
 constexpr int kMaxStages = 32;
@@ -75,32 +76,46 @@ struct Cursor {                            // a stage of the ring and its parity
   }
 };
 
-__device__ __forceinline__ void ring_init(Ring& ring, int stages) {      // one thread
-  for (int s = 0; s < stages; s++) { sm100::mbar_init(&ring.full[s], 1); sm100::mbar_init(&ring.empty[s], kWarps); }
+__device__ __forceinline__ void ring_init(Ring& ring, int stages, int producers) {      // one thread
+  for (int s = 0; s < stages; s++) { sm100::mbar_init(&ring.full[s], producers); sm100::mbar_init(&ring.empty[s], kWarps); }
   ring.abort = 0;
   sm100::mbar_fence_init();
 }
 
 // Shared memory of a CTA: the buffer in which warps add their sums, then the stages, 1024-byte aligned.
 __host__ __device__ inline uint32_t red_bytes(int tile) { return (uint32_t)tile * kWarps * 64; }
-__host__ __device__ inline uint32_t slot_bytes(int tile) { return (uint32_t)tile * kChunk; }
+// A stage: `tile` weight rows and, where those of A go through shared memory too, `rows` of them (0 otherwise).
+__host__ __device__ inline uint32_t slot_bytes(int tile, int rows) { return (uint32_t)(tile + rows) * kChunk; }
+// Rows of the box that holds r rows of A.
+__host__ __device__ inline int box_rows(int r) { return r <= 8 ? 8 : r <= 16 ? 16 : r <= 32 ? 32 : 64; }
 
-// Fetches chunk c of `rows` weight rows from `row0` on into a stage: box by box, in a box column by column.  One thread.  A
-// thread gets a box on its way in 150 to 470 cycles, whatever its size, so there is one box per stage for 64 rows: with a box
-// per column the producer set the pace (205 us against 125 for one token of a layer that reads 704 MB).
+// Fetches chunk c of `rows` rows (a multiple of 8) from `row0` on to `dst`: box by box, in a box column by column.  One thread.
+// A thread gets a box on its way in 150 cycles or more, whatever its size, so there is one box per stage for 64 rows: with a
+// box per column the producer set the pace (205 us against 125 for one token of a layer that reads 704 MB).
 template <typename E>                      // element: its size turns bytes along K into coordinates
-__device__ __forceinline__ void fetch_weights(const WeightMaps& maps, uint8_t* slot, int row0, int rows, int c, uint64_t* bar) {
+__device__ __forceinline__ void fetch(const WeightMaps& maps, uint8_t* dst, int row0, int rows, int c, uint64_t* bar) {
   sm100::mbar_arrive_expect_tx(bar, (uint32_t)rows * kChunk);
-  int at = 0;
-  #pragma unroll 1
-  for (int b = 3; b >= 0; b--) {
-    if (!(rows & (8 << b))) continue;
-    if (c < maps.whole) sm100::tma_load_3d(slot + at * kChunk, &maps.all[b], 0, row0 + at, c * kCols, bar);
-    else
-      for (int j = 0; j < kCols; j++)
-        sm100::tma_load_2d(slot + at * kChunk + j * (128 * (8 << b)), &maps.one[b], (c * kChunk + j * 128) / (int)sizeof(E), row0 + at, bar);
-    at += 8 << b;
+  if (c < maps.whole) {
+    #pragma unroll 1
+    do {
+      const int b = 28 - __clz(rows);      // largest box that fits: 8 << b rows
+      sm100::tma_load_3d(dst, &maps.all[b], 0, row0, c * kCols, bar);
+      dst += kChunk << (b + 3);
+      row0 += 8 << b;
+      rows -= 8 << b;
+    } while (rows > 0);
+    return;
   }
+  #pragma unroll 1
+  do {
+    const int b = 28 - __clz(rows);
+    #pragma unroll 1
+    for (int j = 0; j < kCols; j++)
+      sm100::tma_load_2d(dst + j * (128 << (b + 3)), &maps.one[b], (c * kChunk + j * 128) / (int)sizeof(E), row0, bar);
+    dst += kChunk << (b + 3);
+    row0 += 8 << b;
+    rows -= 8 << b;
+  } while (rows > 0);
 }
 
 // Where in a stage of `rows` weight rows the 8 rows of group g are, column j.
@@ -122,7 +137,7 @@ struct Spread {
   static constexpr int MT = MT_;
   static constexpr bool HALVES = HALVES_;
   static constexpr int SETS = HALVES ? 2 : 1;
-  static constexpr bool AHEAD = !HALVES;   // rows of A one chunk ahead; with HALVES the registers do not suffice
+  static constexpr int AHEAD = HALVES ? 0 : MT == 1 ? 2 : 1;      // chunks that rows of A from memory are ahead, as registers allow
   static constexpr int GROUPS = HALVES ? kMaxTile / 8 : kMaxTile / 16;      // groups of 8 weight rows of a warp, at most
   // row of A of tile m, upper or lower half h of a warp in part q
   __device__ static __forceinline__ int row(int m, int q, int h, int lane) { return 16 * (m + q * MT) + 8 * h + (lane >> 2); }
@@ -133,14 +148,13 @@ struct Spread {
   }
 };
 
-// A lane's part of the rows of A for one chunk: 32 bytes of each of its rows.
+// A lane's part of the rows of A for one chunk: 32 bytes of each of its rows, zeros for rows that do not exist.
 template <typename S>
 struct Rows {
   uint4 v[S::MT][2][2];                    // tile, half of the tile, half of the 32 bytes
-  // `src`: the rows, null for those that do not exist (they count as zeros); CACHED: through L1 (nobody writes them meanwhile)
-  template <bool CACHED>
-  __device__ __forceinline__ void load(const uint8_t* const (&src)[S::MT][2], long long row_bytes, int c, int col, int lane) {
-    const long long k = (long long)c * kChunk + col * 128 + (lane & 3) * 32;
+  // from memory (nobody writes there meanwhile); `src`: the rows, null for those that do not exist
+  __device__ __forceinline__ void load(const uint8_t* const (&src)[S::MT][2], int row_bytes, int c, int col, int lane) {
+    const int k = c * kChunk + col * 128 + (lane & 3) * 32;
     #pragma unroll
     for (int m = 0; m < S::MT; m++)
       #pragma unroll
@@ -148,10 +162,20 @@ struct Rows {
         #pragma unroll
         for (int s = 0; s < 2; s++) {
           v[m][h][s] = make_uint4(0u, 0u, 0u, 0u);
-          if (src[m][h] && k + 16 * s < row_bytes) {
-            const uint4* p = reinterpret_cast<const uint4*>(src[m][h] + k + 16 * s);
-            v[m][h][s] = CACHED ? __ldg(p) : __ldcg(p);
-          }
+          if (src[m][h] && k + 16 * s < row_bytes) v[m][h][s] = __ldg(reinterpret_cast<const uint4*>(src[m][h] + k + 16 * s));
+        }
+  }
+  // from a box of a stage; `at`: rows of it, negative for those that do not exist
+  __device__ __forceinline__ void load(const int (&at)[S::MT][2], uint32_t box, int rows, int col, int lane) {
+    const uint32_t base = box + (uint32_t)(col * rows * 128), t = (uint32_t)lane & 3;
+    #pragma unroll
+    for (int m = 0; m < S::MT; m++)
+      #pragma unroll
+      for (int h = 0; h < 2; h++)
+        #pragma unroll
+        for (int s = 0; s < 2; s++) {
+          v[m][h][s] = make_uint4(0u, 0u, 0u, 0u);
+          if (at[m][h] >= 0) v[m][h][s] = lds16(base + (uint32_t)at[m][h] * 128u + (((2u * t + s) ^ ((uint32_t)at[m][h] & 7u)) << 4));
         }
   }
 };
@@ -257,11 +281,11 @@ inline int tile_rows(long long groups, int parts) {
 }
 
 // Stages that fit beside `fixed` bytes of static shared memory.
-inline int ring_stages(int tile, size_t fixed) {
-  const size_t room = 227 * 1024 - 1024 /*alignment*/ - fixed - red_bytes(tile), n = room / slot_bytes(tile);
+inline int ring_stages(int tile, int rows, size_t fixed) {
+  const size_t room = 227 * 1024 - 1024 /*alignment*/ - fixed - red_bytes(tile), n = room / slot_bytes(tile, rows);
   return n > (size_t)kMaxStages ? kMaxStages : (int)n;
 }
-inline size_t ring_smem(int tile, int stages) { return 1024 + red_bytes(tile) + (size_t)slot_bytes(tile) * stages; }
+inline size_t ring_smem(int tile, int rows, int stages) { return 1024 + red_bytes(tile) + (size_t)slot_bytes(tile, rows) * stages; }
 
 // Weights of `rows` rows of row_bytes (a multiple of 16) each, elements of `size` bytes; 128-byte swizzle.
 inline bool weight_maps(WeightMaps* m, const void* base, unsigned long long rows, unsigned long long row_bytes, CUtensorMapDataType type,

@@ -35,12 +35,12 @@ struct FewArgs {
   long long ldl;                          // elements
   int T, H, I, E, top_k;
   const uint8_t *w13, *w2;
-  __nv_bfloat16* h;                       // [T * top_k, I]
+  __nv_bfloat16* h;                       // [T * top_k, I], in the order of the used experts
   float* partial;                         // [2 * CTAs][T][tile]
   int* counters;                          // one per column tile of the down product
   __nv_bfloat16* out;
   int* error;
-  int tile, stages;                       // weight rows of a piece at most, ring stages
+  int tile, box, stages;                  // weight rows of a piece and rows of A in a stage, at most; ring stages
 };
 
 // The choice, as every CTA makes it.
@@ -202,23 +202,20 @@ __device__ __forceinline__ bool up_piece(const FewArgs& a, Shared& s, uint4* red
     }
   float acc[S::MT][S::GROUPS][4];
   clear<S>(acc);
-  const long long row_bytes = 2ll * a.H;
-  const int chunks = (int)((row_bytes + kChunk - 1) / kChunk);
-  Rows<S> rows, next;
-  if (S::AHEAD) next.template load<true>(src, row_bytes, 0, col, lane);
+  const int row_bytes = 2 * a.H, chunks = (row_bytes + kChunk - 1) / kChunk;
+  Rows<S> ahead[S::AHEAD + 1];             // (beyond the last chunk nothing is read)
+  #pragma unroll
+  for (int i = 0; i < S::AHEAD; i++) ahead[i].load(src, row_bytes, i, col, lane);
   for (int c = 0; c < chunks; c++) {
-    if (S::AHEAD) {
-      rows = next;
-      if (c + 1 < chunks) next.template load<true>(src, row_bytes, c + 1, col, lane);
-    } else {
-      rows.template load<true>(src, row_bytes, c, col, lane);
-    }
+    ahead[S::AHEAD].load(src, row_bytes, c + S::AHEAD, col, lane);
     if (ok && !sm100::mbar_wait(&s.ring.full[cur.stage], cur.phase, &s.ring.abort)) { ok = false; s.ring.abort = 1; }
     __syncwarp();
-    multiply<S>(acc, slots + (uint32_t)cur.stage * slot_bytes(a.tile), off, mine, rows, lane);
+    multiply<S>(acc, slots + (uint32_t)cur.stage * slot_bytes(a.tile, 0), off, mine, ahead[0], lane);
     __syncwarp();
     if (lane == 0) sm100::mbar_arrive(&s.ring.empty[cur.stage]);
     cur.next(a.stages);
+    #pragma unroll
+    for (int i = 0; i < S::AHEAD; i++) ahead[i] = ahead[i + 1];
   }
   #pragma unroll
   for (int m = 0; m < S::MT; m++) {
@@ -232,7 +229,7 @@ __device__ __forceinline__ bool up_piece(const FewArgs& a, Shared& s, uint4* red
           const int slot = list[r];
           const float gate = v[q][2 * h], up = v[q][2 * h + 1];
           const float y = s.choice.weight[slot] * (gate / (1.0f + __expf(-gate)) * up);
-          a.h[(long long)slot * a.I + p.row0 / 2 + warp * 4 + (lane & 3)] = __float2bfloat16_rn(y);
+          a.h[(long long)(s.choice.start[p.u] + r) * a.I + p.row0 / 2 + warp * 4 + (lane & 3)] = __float2bfloat16_rn(y);
         }
       }
   }
@@ -248,7 +245,7 @@ __global__ void __launch_bounds__(kThreads, 1) moe_few_up_kernel(const __grid_co
   uint8_t* base = aligned_smem(dyn);
   uint4* red = reinterpret_cast<uint4*>(base);
   uint8_t* slots = base + red_bytes(a.tile);
-  if (threadIdx.x == 0) ring_init(s.ring, a.stages);
+  if (threadIdx.x == 0) ring_init(s.ring, a.stages, 1);
   pdl_wait();
   pdl_trigger();      // after the wait: the down kernel reads the logits before it waits for this one
   if (blockIdx.x == 0)
@@ -257,8 +254,8 @@ __global__ void __launch_bounds__(kThreads, 1) moe_few_up_kernel(const __grid_co
   UpWalk walk(a, s.choice.n_used);
   UpPiece p;
   Cursor cur;
-  if (warp == kWarps) {
-    if (lane != 0) return;
+  if (warp >= kWarps) {
+    if (warp != kWarps || lane != 0) return;
     const int chunks = (2 * a.H + kChunk - 1) / kChunk;
     bool ok = true;
     while (ok && walk.next(p)) {
@@ -266,7 +263,7 @@ __global__ void __launch_bounds__(kThreads, 1) moe_few_up_kernel(const __grid_co
       for (int c = 0; c < chunks; c++) {
         ok = sm100::mbar_wait(&s.ring.empty[cur.stage], cur.phase ^ 1u, &s.ring.abort);
         if (!ok) break;
-        fetch_weights<__nv_bfloat16>(maps, slots + (size_t)cur.stage * slot_bytes(a.tile), row0, p.rows, c, &s.ring.full[cur.stage]);
+        fetch<__nv_bfloat16>(maps, slots + (size_t)cur.stage * slot_bytes(a.tile, 0), row0, p.rows, c, &s.ring.full[cur.stage]);
         cur.next(a.stages);
       }
     }
@@ -288,19 +285,33 @@ __global__ void __launch_bounds__(kThreads, 1) moe_few_up_kernel(const __grid_co
 struct DownWalk {
   Split split;
   long long at, end;
-  int chunks, per_tile;
-  __device__ __forceinline__ DownWalk(const FewArgs& a, int n_used) {
-    chunks = (int)((2ll * a.I + kChunk - 1) / kChunk);
+  int chunks, per_tile, n_used;
+  int tile, u, c;                         // of step `at`
+  __device__ __forceinline__ DownWalk(const FewArgs& a, int n_used_) {
+    n_used = n_used_;
+    chunks = (2 * a.I + kChunk - 1) / kChunk;
     per_tile = n_used * chunks;
     split.total = (long long)((a.H + a.tile - 1) / a.tile) * per_tile;
     split.parts = (int)min((long long)gridDim.x, split.total);
     at = end = 0;
     if ((int)blockIdx.x < split.parts) { at = split.begin(blockIdx.x); end = split.begin(blockIdx.x + 1); }
+    tile = (int)(at / per_tile);
+    const int in_tile = (int)(at - (long long)tile * per_tile);
+    u = in_tile / chunks;
+    c = in_tile - u * chunks;
+  }
+  __device__ __forceinline__ void step() {
+    at++;
+    if (++c == chunks) {
+      c = 0;
+      if (++u == n_used) { u = 0; tile++; }
+    }
   }
 };
 
 template <typename S>       // by the tokens: 16, 32 or 64 at most
-__global__ void __launch_bounds__(kThreads, 1) moe_few_down_kernel(const __grid_constant__ WeightMaps maps, const __grid_constant__ FewArgs a) {
+__global__ void __launch_bounds__(kThreads, 1) moe_few_down_kernel(const __grid_constant__ WeightMaps maps, const __grid_constant__ WeightMaps h_maps,
+                                                                   const __grid_constant__ FewArgs a) {
   extern __shared__ uint8_t dyn[];
   __shared__ Shared s;
   constexpr int MT = S::MT;
@@ -308,7 +319,7 @@ __global__ void __launch_bounds__(kThreads, 1) moe_few_down_kernel(const __grid_
   uint8_t* base = aligned_smem(dyn);
   uint4* red = reinterpret_cast<uint4*>(base);
   uint8_t* slots = base + red_bytes(a.tile);
-  if (tid == 0) ring_init(s.ring, a.stages);
+  if (tid == 0) ring_init(s.ring, a.stages, 2);
   pdl_trigger();
   choose(s.choice, a);
   const int n_used = s.choice.n_used;
@@ -318,19 +329,27 @@ __global__ void __launch_bounds__(kThreads, 1) moe_few_down_kernel(const __grid_
       a.out[i] = __float2bfloat16_rn(0.0f);
     return;
   }
-  const DownWalk walk(a, n_used);
-  const long long row_bytes = 2ll * a.I;
+  DownWalk walk(a, n_used);
   Cursor cur;
-  if (warp == kWarps) {                   // the weights do not wait for the first kernel
+  if (warp >= kWarps) {                   // the weights do not wait for the first kernel, the rows of h do
     if (lane != 0) return;
+    const bool weights = warp == kWarps;
     bool ok = true;
-    for (long long at = walk.at; at < walk.end; at++) {
+    if (!weights) {
+      pdl_wait();
+      asm volatile("fence.proxy.async;" ::: "memory");
+    }
+    for (; walk.at < walk.end; walk.step()) {
       ok = sm100::mbar_wait(&s.ring.empty[cur.stage], cur.phase ^ 1u, &s.ring.abort);
       if (!ok) break;
-      const int tile = (int)(at / walk.per_tile), in_tile = (int)(at - (long long)tile * walk.per_tile);
-      const int u = in_tile / walk.chunks, c = in_tile - u * walk.chunks, col0 = tile * a.tile;
-      fetch_weights<__nv_bfloat16>(maps, slots + (size_t)cur.stage * slot_bytes(a.tile), s.choice.used[u] * a.H + col0,
-                                   min(a.tile, a.H - col0), c, &s.ring.full[cur.stage]);
+      uint8_t* slot = slots + (size_t)cur.stage * slot_bytes(a.tile, a.box);
+      uint64_t* bar = &s.ring.full[cur.stage];
+      if (weights) {
+        const int col0 = walk.tile * a.tile;
+        fetch<__nv_bfloat16>(maps, slot, s.choice.used[walk.u] * a.H + col0, min(a.tile, a.H - col0), walk.c, bar);
+      } else {
+        fetch<__nv_bfloat16>(h_maps, slot + a.tile * kChunk, s.choice.start[walk.u], box_rows(s.choice.rows[walk.u]), walk.c, bar);
+      }
       cur.next(a.stages);
     }
     if (!ok) s.ring.abort = 1;
@@ -340,9 +359,9 @@ __global__ void __launch_bounds__(kThreads, 1) moe_few_down_kernel(const __grid_
   bool ok = true;
   const uint32_t slots_at = sm100::smem_u32(slots);
   const int part = warp >> 2, wcol = warp & 3;
-  for (long long at0 = walk.at; at0 < walk.end;) {
-    const int tile = (int)(at0 / walk.per_tile);
-    const long long first = (long long)tile * walk.per_tile, stop = min(walk.end, first + walk.per_tile);
+  while (walk.at < walk.end) {
+    const int tile = walk.tile;
+    const long long first = (long long)tile * walk.per_tile, at0 = walk.at, stop = min(walk.end, first + walk.per_tile);
     const int col0 = tile * a.tile, nr = min(a.tile, a.H - col0), groups = nr / 8;
     const int g0 = S::group0(part, groups), mine = S::my_groups(part, groups);
     uint32_t off[S::GROUPS];
@@ -350,36 +369,30 @@ __global__ void __launch_bounds__(kThreads, 1) moe_few_down_kernel(const __grid_
     for (int n = 0; n < S::GROUPS; n++) off[n] = group_offset(nr, g0 + n, wcol);
     float acc[MT][S::GROUPS][4];
     clear<S>(acc);
-    // the rows of h for a step, one step ahead: tokens that did not choose the expert count as zeros
-    int u = (int)(at0 - first) / walk.chunks, c = (int)(at0 - first) - u * walk.chunks;
-    const uint8_t* src[MT][2];
-    auto expert_rows = [&]() {
-      const int e = s.choice.used[u];
-      #pragma unroll
-      for (int m = 0; m < MT; m++)
+    // where the tokens' rows of h are in a stage of expert u: tokens that did not choose it count as zeros
+    int u = -1, box = 0, rows_at[MT][2];
+    for (; walk.at < stop; walk.step()) {
+      if (walk.u != u) {
+        u = walk.u;
+        box = box_rows(s.choice.rows[u]);
+        const int e = s.choice.used[u];
         #pragma unroll
-        for (int h = 0; h < 2; h++) {
-          const int t = S::row(m, S::set(part), h, lane);
-          src[m][h] = nullptr;
-          if (t < a.T)
-            for (int j = 0; j < a.top_k; j++)
-              if (s.choice.expert[t * a.top_k + j] == e)
-                src[m][h] = reinterpret_cast<const uint8_t*>(a.h) + (long long)(t * a.top_k + j) * row_bytes;
-        }
-    };
-    expert_rows();
-    Rows<S> rows, next;
-    if (S::AHEAD) next.template load<false>(src, row_bytes, c, wcol, lane);
-    for (long long at = at0; at < stop; at++) {
-      if (S::AHEAD) rows = next;
-      else rows.template load<false>(src, row_bytes, c, wcol, lane);
-      if (at + 1 < stop) {
-        if (++c == walk.chunks) { c = 0; u++; expert_rows(); }
-        if (S::AHEAD) next.template load<false>(src, row_bytes, c, wcol, lane);
+        for (int m = 0; m < MT; m++)
+          #pragma unroll
+          for (int h = 0; h < 2; h++) {
+            const int t = S::row(m, S::set(part), h, lane);
+            rows_at[m][h] = -1;
+            if (t < a.T)
+              for (int j = 0; j < a.top_k; j++)
+                if (s.choice.expert[t * a.top_k + j] == e) rows_at[m][h] = s.choice.at[t * a.top_k + j];
+          }
       }
       if (ok && !sm100::mbar_wait(&s.ring.full[cur.stage], cur.phase, &s.ring.abort)) { ok = false; s.ring.abort = 1; }
       __syncwarp();
-      multiply<S>(acc, slots_at + (uint32_t)cur.stage * slot_bytes(a.tile), off, mine, rows, lane);
+      const uint32_t slot = slots_at + (uint32_t)cur.stage * slot_bytes(a.tile, a.box);
+      Rows<S> rows;
+      rows.load(rows_at, slot + (uint32_t)a.tile * kChunk, box, wcol, lane);
+      multiply<S>(acc, slot, off, mine, rows, lane);
       __syncwarp();
       if (lane == 0) sm100::mbar_arrive(&s.ring.empty[cur.stage]);
       cur.next(a.stages);
@@ -420,7 +433,6 @@ __global__ void __launch_bounds__(kThreads, 1) moe_few_down_kernel(const __grid_
         }
       }
     }
-    at0 = stop;
   }
   if (!ok && a.error) atomicExch(a.error, 2);
 }
@@ -433,13 +445,15 @@ size_t round_up(size_t v, size_t to) { return (v + to - 1) / to * to; }
 bool few_plan(int T, int H, int I, int E, int top_k, FewPlan* p) {
   if (T < 1 || T > kMaxRows || E < 1 || E > kMoeMaxExperts || top_k < 1 || top_k > kMoeFewMaxTopK || top_k > E) return false;
   if (H < 8 || I < 8 || H % 8 || I % 8 || 2ll * E * I > 0x7fffffffll || (long long)E * H > 0x7fffffffll) return false;
-  if (H > (1 << 24) || I > (1 << 24)) return false;
+  if (H > (1 << 24) || I > (1 << 24)) return false;      // (row lengths in bytes, and coordinates a box beyond them, fit an int)
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&p->sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return false;
   const int used = E < T * top_k ? E : T * top_k;   // experts in use, at most
   p->up_tile = tile_rows((long long)used * (2 * I / 8), p->sms);
-  // about two CTAs per column tile at least, so that the ends of the ranges cost little
-  p->down_tile = tile_rows(H / 8, p->sms / 2);
+  // columns of the result in a piece: the most, in one box, that leave a CTA eight steps to share the work out evenly
+  const long long steps = (long long)used * ((2 * I + kChunk - 1) / kChunk);
+  p->down_tile = kMaxTile;
+  while (p->down_tile > 8 && (H + p->down_tile - 1) / p->down_tile * steps < 8ll * p->sms) p->down_tile /= 2;
   p->h_bytes = round_up((size_t)T * top_k * I * 2, 256);
   p->partial_bytes = round_up((size_t)2 * p->sms * T * p->down_tile * 4, 256);
   p->counter_bytes = round_up((size_t)(H / 8) * 4, 256);
@@ -448,17 +462,21 @@ bool few_plan(int T, int H, int I, int E, int top_k, FewPlan* p) {
 
 template <int MAX, typename S>
 cudaError_t few_launch(FewArgs a, const FewPlan& p, cudaStream_t st) {
-  auto launch = [&](auto kernel, int tile, const uint8_t* w, long long rows, long long row_bytes) {
-    WeightMaps maps;
-    if (!weight_maps(&maps, w, (unsigned long long)rows, (unsigned long long)row_bytes, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2)) return cudaErrorUnknown;
+  const CUtensorMapDataType bf16 = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  WeightMaps w13, w2, h;
+  if (!weight_maps(&w13, a.w13, 2ull * a.E * a.I, 2ull * a.H, bf16, 2) || !weight_maps(&w2, a.w2, (unsigned long long)a.E * a.H, 2ull * a.I, bf16, 2) ||
+      !weight_maps(&h, a.h, (unsigned long long)a.T * a.top_k, 2ull * a.I, bf16, 2))
+    return cudaErrorUnknown;
+  auto launch = [&](auto kernel, int tile, int box, const auto&... maps) {
     a.tile = tile;
-    a.stages = ring_stages(tile, sizeof(Shared));
-    const size_t smem = ring_smem(tile, a.stages);
+    a.box = box;
+    a.stages = ring_stages(tile, box, sizeof(Shared));
+    const size_t smem = ring_smem(tile, box, a.stages);
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    return e != cudaSuccess ? e : launch_dependent(kernel, dim3(p.sms), dim3(kThreads), smem, st, maps, a);
+    return e != cudaSuccess ? e : launch_dependent(kernel, dim3(p.sms), dim3(kThreads), smem, st, maps..., a);
   };
-  const cudaError_t e = launch(moe_few_up_kernel<MAX>, p.up_tile, a.w13, 2ll * a.E * a.I, 2ll * a.H);
-  return e != cudaSuccess ? e : launch(moe_few_down_kernel<S>, p.down_tile, a.w2, (long long)a.E * a.H, 2ll * a.I);
+  const cudaError_t e = launch(moe_few_up_kernel<MAX>, p.up_tile, 0, w13);
+  return e != cudaSuccess ? e : launch(moe_few_down_kernel<S>, p.down_tile, box_rows(a.T), w2, h);
 }
 
 }  // namespace
