@@ -52,6 +52,7 @@ __device__ __forceinline__ uint4 lds16(uint32_t addr) {
   return v;
 }
 __device__ __forceinline__ void consumers_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
+__device__ __forceinline__ void part_sync(int part) { asm volatile("bar.sync %0, 128;" ::"r"(2 + part) : "memory"); }
 
 // bf16 x bf16 -> fp32 (K 16) and s8 x s8 -> s32 (K 32): the same bytes per register.
 __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -68,54 +69,115 @@ struct Ring {
   int abort;
 };
 
-struct Cursor {                            // a stage of the ring and its parity
-  int stage = 0;
-  uint32_t phase = 0;
-  __device__ __forceinline__ void next(int stages) {
-    if (++stage == stages) { stage = 0; phase ^= 1u; }
-  }
-};
-
 __device__ __forceinline__ void ring_init(Ring& ring, int stages, int producers) {      // one thread
   for (int s = 0; s < stages; s++) { sm100::mbar_init(&ring.full[s], producers); sm100::mbar_init(&ring.empty[s], kWarps); }
   ring.abort = 0;
   sm100::mbar_fence_init();
 }
 
+// A warp's place in the ring, as addresses in shared memory: a warp that works alone pays for every instruction between two
+// loads or multiplications, a stage of a small piece with as many cycles as its bytes take.
+struct Cursor {
+  uint32_t full, empty, slot;             // barriers and start of the current stage
+  uint32_t phase = 0;
+  int left, stages;                        // stages until the ring begins again
+  uint32_t slot_bytes;
+  Ring* ring;
+  bool ok = true;
+  __device__ __forceinline__ Cursor(Ring& r, uint32_t slots, int n, uint32_t bytes)
+      : full(sm100::smem_u32(r.full)), empty(sm100::smem_u32(r.empty)), slot(slots), left(n), stages(n), slot_bytes(bytes), ring(&r) {}
+  __device__ __forceinline__ void next() {
+    full += 8; empty += 8; slot += slot_bytes;
+    if (--left == 0) {
+      left = stages;
+      full -= 8u * stages; empty -= 8u * stages; slot -= slot_bytes * stages;
+      phase ^= 1u;
+    }
+  }
+  __device__ __forceinline__ static bool try_wait(uint32_t bar, uint32_t parity) {
+    uint32_t done;
+    asm volatile("{\n\t.reg .pred P;\n\tmbarrier.try_wait.parity.shared::cta.b64 P, [%1], %2;\n\tselp.b32 %0, 1, 0, P;\n\t}"
+                 : "=r"(done) : "r"(bar), "r"(parity) : "memory");
+    return done != 0;
+  }
+  // Bounded; once a wait of this CTA has run out, nobody waits any more (results are garbage, and reported).
+  __device__ __forceinline__ void wait(uint32_t bar, uint32_t parity) {
+    if (try_wait(bar, parity) || !ok) return;
+    volatile int* abort = &ring->abort;
+    for (uint32_t i = 0; i < (1u << 24); i++) {
+      if (try_wait(bar, parity)) return;
+      if ((i & 1023u) == 1023u && *abort) break;
+    }
+    ok = false;
+    *abort = 1;
+  }
+  __device__ __forceinline__ void wait_full() { wait(full, phase); }
+  __device__ __forceinline__ void wait_empty() { wait(empty, phase ^ 1u); }
+  __device__ __forceinline__ void release() {          // one lane per consumer warp
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(empty) : "memory");
+  }
+};
+
 // Shared memory of a CTA: the buffer in which warps add their sums, then the stages, 1024-byte aligned.
-__host__ __device__ inline uint32_t red_bytes(int tile) { return (uint32_t)tile * kWarps * 64; }
+constexpr uint32_t kRedBytes = 2 * 2 * kCols * 32 * 16;       // two groups of weight rows at a time per part
 // A stage: `tile` weight rows and, where those of A go through shared memory too, `rows` of them (0 otherwise).
 __host__ __device__ inline uint32_t slot_bytes(int tile, int rows) { return (uint32_t)(tile + rows) * kChunk; }
 // Rows of the box that holds r rows of A.
 __host__ __device__ inline int box_rows(int r) { return r <= 8 ? 8 : r <= 16 ? 16 : r <= 32 ? 32 : 64; }
 
-// Fetches chunk c of `rows` rows (a multiple of 8) from `row0` on to `dst`: box by box, in a box column by column.  One thread.
-// A thread gets a box on its way in 150 cycles or more, whatever its size, so there is one box per stage for 64 rows: with a
-// box per column the producer set the pace (205 us against 125 for one token of a layer that reads 704 MB).
+__device__ __forceinline__ void expect(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* m, int row, int column, uint32_t bar) {
+  asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+               ::"r"(dst), "l"(m), "r"(bar), "r"(0), "r"(row), "r"(column) : "memory");
+}
+__device__ __forceinline__ void load_column(uint32_t dst, const CUtensorMap* m, int x, int row, uint32_t bar) {
+  asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+               ::"r"(dst), "l"(m), "r"(bar), "r"(x), "r"(row) : "memory");
+}
+
+// Fetches chunks c0 to c1 - 1 of `rows` rows (a multiple of 8) from `row0` on, one per stage, `off` bytes into it: box by box, in
+// a box column by column.  One thread, which gets a box on its way in 150 cycles or more whatever its size: there is one box
+// per stage for 64 rows (with a box per column the producer set the pace, 205 us against 119 for one token of a layer that
+// reads 704 MB).  False: a wait ran out, stop.
 template <typename E>                      // element: its size turns bytes along K into coordinates
-__device__ __forceinline__ void fetch(const WeightMaps& maps, uint8_t* dst, int row0, int rows, int c, uint64_t* bar) {
-  sm100::mbar_arrive_expect_tx(bar, (uint32_t)rows * kChunk);
-  if (c < maps.whole) {
+__device__ __forceinline__ bool feed(const WeightMaps& maps, Cursor& cur, uint32_t off, int row0, int rows, int c0, int c1) {
+  const uint32_t bytes = (uint32_t)rows * kChunk;
+  const int big = 28 - __clz(rows);        // the largest box that fits has 8 << big rows
+  int c = c0;
+  if (rows == 8 << big) {
+    const CUtensorMap* m = &maps.all[big];
     #pragma unroll 1
-    do {
-      const int b = 28 - __clz(rows);      // largest box that fits: 8 << b rows
-      sm100::tma_load_3d(dst, &maps.all[b], 0, row0, c * kCols, bar);
-      dst += kChunk << (b + 3);
-      row0 += 8 << b;
-      rows -= 8 << b;
-    } while (rows > 0);
-    return;
+    for (; c < c1 && c < maps.whole; c++) {
+      cur.wait_empty();
+      if (!cur.ok) return false;
+      expect(cur.full, bytes);
+      load_box(cur.slot + off, m, row0, c * kCols, cur.full);
+      cur.next();
+    }
   }
   #pragma unroll 1
-  do {
-    const int b = 28 - __clz(rows);
+  for (; c < c1; c++) {
+    cur.wait_empty();
+    if (!cur.ok) return false;
+    expect(cur.full, bytes);
+    uint32_t dst = cur.slot + off;
+    int at = 0;
     #pragma unroll 1
-    for (int j = 0; j < kCols; j++)
-      sm100::tma_load_2d(dst + j * (128 << (b + 3)), &maps.one[b], (c * kChunk + j * 128) / (int)sizeof(E), row0, bar);
-    dst += kChunk << (b + 3);
-    row0 += 8 << b;
-    rows -= 8 << b;
-  } while (rows > 0);
+    for (int b = big; b >= 0; b--) {
+      if (!(rows & (8 << b))) continue;
+      if (c < maps.whole) load_box(dst, &maps.all[b], row0 + at, c * kCols, cur.full);
+      else
+        #pragma unroll 1
+        for (int j = 0; j < kCols; j++)
+          load_column(dst + (uint32_t)(j * (1024 << b)), &maps.one[b], (c * kChunk + j * 128) / (int)sizeof(E), row0 + at, cur.full);
+      dst += (uint32_t)kChunk << (b + 3);
+      at += 8 << b;
+    }
+    cur.next();
+  }
+  return true;
 }
 
 // Where in a stage of `rows` weight rows the 8 rows of group g are, column j.
@@ -190,88 +252,74 @@ __device__ __forceinline__ void clear(Acc (&acc)[S::MT][S::GROUPS][4]) {
       for (int k = 0; k < 4; k++) acc[m][n][k] = 0;
 }
 
-// One stage's part of a warp: `groups` groups of 8 weight rows, the n-th at w + off[n].  Groups that do not exist are
-// multiplied as zeros: without branches all loads are on their way before the first multiplication and the chains of different
-// groups overlap.
-template <typename S, typename Acc>
+// One stage's part of a warp: G groups of 8 weight rows, the n-th at w + off[n].  Groups from `groups` on do not exist and are
+// multiplied as zeros: without branches all loads are on their way before the first multiplication and the chains of
+// different groups overlap.
+template <typename S, int G, typename Acc>
 __device__ __forceinline__ void multiply(Acc (&acc)[S::MT][S::GROUPS][4], uint32_t w, const uint32_t (&off)[S::GROUPS], int groups,
                                          const Rows<S>& a, int lane) {
   const uint32_t row = (uint32_t)lane >> 2, t = (uint32_t)lane & 3;
   const uint32_t wl = w + row * 128u;
-  const uint32_t unit[2] = {((2u * t) ^ row) << 4, ((2u * t + 1u) ^ row) << 4};
-  constexpr int SETS = S::GROUPS / 4;      // four groups at a time
+  constexpr int AT_ONCE = G < 4 ? G : 4;
   #pragma unroll
-  for (int q = 0; q < SETS; q++) {
-    uint4 b[4][2];
+  for (int q = 0; q < G; q += AT_ONCE)
     #pragma unroll
-    for (int n = 0; n < 4; n++)
+    for (int s = 0; s < 2; s++) {
+      uint4 b[AT_ONCE];
       #pragma unroll
-      for (int s = 0; s < 2; s++) {
-        b[n][s] = make_uint4(0u, 0u, 0u, 0u);
-        if (4 * q + n < groups) b[n][s] = lds16(wl + off[4 * q + n] + unit[s]);
+      for (int n = 0; n < AT_ONCE; n++) {
+        b[n] = make_uint4(0u, 0u, 0u, 0u);
+        if (q + n < groups) b[n] = lds16(wl + off[q + n] + (((2u * t + s) ^ row) << 4));
       }
-    #pragma unroll
-    for (int s = 0; s < 2; s++)
       #pragma unroll
       for (int half = 0; half < 2; half++)
         #pragma unroll
         for (int m = 0; m < S::MT; m++)
           #pragma unroll
-          for (int n = 0; n < 4; n++) {
+          for (int n = 0; n < AT_ONCE; n++) {
             const uint4 &lo = a.v[m][0][s], &hi = a.v[m][1][s];
-            if (half == 0) mma(acc[m][4 * q + n], lo.x, hi.x, lo.y, hi.y, b[n][s].x, b[n][s].y);
-            else mma(acc[m][4 * q + n], lo.z, hi.z, lo.w, hi.w, b[n][s].z, b[n][s].w);
+            if (half == 0) mma(acc[m][q + n], lo.x, hi.x, lo.y, hi.y, b[n].x, b[n].y);
+            else mma(acc[m][q + n], lo.z, hi.z, lo.w, hi.w, b[n].z, b[n].w);
           }
-  }
+    }
 }
 
-// Adds the columns' sums of a tile of 16 rows of A per set; thread (n = warp, lane) gets those of rows S::row(m, q, 0 and 1,
-// lane) (v[q][0..1], v[q][2..3]) and of weight rows 8 n + 2 (lane % 4) and + 1.  All consumers call it; `red` holds 16 bytes
-// per lane, group and warp.
-template <typename S, typename Acc>
-__device__ __forceinline__ void add_columns(const Acc (&acc)[S::GROUPS][4], uint4* red, int groups, int warp, int lane, Acc (&v)[S::SETS][4]) {
-  const int part = warp >> 2, col = warp & 3, g0 = S::group0(part, groups), mine = S::my_groups(part, groups);
+// Adds the sums of a part's four columns and hands them out: put(row of A, weight row of the piece, sums of that weight row and
+// the next one).  The parts do not wait for one another.
+template <typename S, typename Acc, typename Put>
+__device__ __forceinline__ void add_columns(const Acc (&acc)[S::MT][S::GROUPS][4], uint4* red, int g0, int groups, int part, int col,
+                                            int lane, Put&& put) {
+  uint4* mine = red + part * (2 * kCols * 32);
+  const int sub = col >> 1, h = col & 1;   // which of two groups, and which half of a tile's rows, this warp adds
   #pragma unroll
-  for (int n = 0; n < S::GROUPS; n++)
-    if (n < mine) red[(((g0 + n) * S::SETS + S::set(part)) * kCols + col) * 32 + lane] = *reinterpret_cast<const uint4*>(acc[n]);
-  consumers_sync();
-  #pragma unroll
-  for (int q = 0; q < S::SETS; q++) {
+  for (int m = 0; m < S::MT; m++)
     #pragma unroll
-    for (int k = 0; k < 4; k++) v[q][k] = 0;
-    if (warp < groups)
+    for (int n = 0; n < S::GROUPS; n += 2) {
+      if (n >= groups) break;
+      mine[col * 32 + lane] = *reinterpret_cast<const uint4*>(acc[m][n]);
+      mine[(kCols + col) * 32 + lane] = *reinterpret_cast<const uint4*>(acc[m][n + 1]);
+      part_sync(part);
+      Acc v0 = 0, v1 = 0;
       #pragma unroll
       for (int j = 0; j < kCols; j++) {
-        const uint4 u = red[((warp * S::SETS + q) * kCols + j) * 32 + lane];
-        const Acc* p = reinterpret_cast<const Acc*>(&u);
-        #pragma unroll
-        for (int k = 0; k < 4; k++) v[q][k] += p[k];
+        const uint2 u = reinterpret_cast<const uint2*>(mine + (sub * kCols + j) * 32 + lane)[h];
+        v0 += *reinterpret_cast<const Acc*>(&u.x);
+        v1 += *reinterpret_cast<const Acc*>(&u.y);
       }
-  }
-  consumers_sync();
+      if (n + sub < groups) put(S::row(m, S::set(part), h, lane), (g0 + n + sub) * 8 + (lane & 3) * 2, v0, v1);
+      part_sync(part);
+    }
 }
 
 // ---- work split along K over CTAs ------------------------------------------------------------------------------------
 // `total` steps (tile by tile, each of `per_tile` steps along K) are cut into `parts` <= total contiguous ranges of equal
 // length (within one).  A tile whose steps lie in several ranges is finished by the last of their CTAs to arrive, which adds
-// the others' sums in the order of the ranges: the result does not depend on who that is.
+// the others' sums in the order of the ranges: the result does not depend on who that is.  (total * parts fits 32 bits.)
 struct Split {
-  long long total;
-  int parts;
-  __device__ __forceinline__ long long begin(int part) const { return (long long)part * total / parts; }
-  __device__ __forceinline__ int owner(long long step) const { return (int)(((step + 1) * parts - 1) / total); }
+  unsigned total, parts;
+  __device__ __forceinline__ unsigned begin(unsigned part) const { return part * total / parts; }
+  __device__ __forceinline__ unsigned owner(unsigned step) const { return ((step + 1) * parts - 1) / total; }
 };
-
-// Whether this CTA is the one to finish the tile, of `pieces`.  (All consumers call it, after their stores to the workspace.)
-__device__ __forceinline__ bool last_to_arrive(int* counter, int pieces, int* s_flag) {
-  __threadfence();
-  consumers_sync();
-  if (threadIdx.x == 0) *s_flag = atomicAdd(counter, 1) == pieces - 1;
-  consumers_sync();
-  const bool last = *s_flag != 0;
-  if (last) __threadfence();
-  return last;
-}
 
 // ---- host side -------------------------------------------------------------------------------------------------------
 // Weight rows of a piece: an even share of `groups` groups of 8 among `parts`, at most 64 rows.
@@ -282,10 +330,10 @@ inline int tile_rows(long long groups, int parts) {
 
 // Stages that fit beside `fixed` bytes of static shared memory.
 inline int ring_stages(int tile, int rows, size_t fixed) {
-  const size_t room = 227 * 1024 - 1024 /*alignment*/ - fixed - red_bytes(tile), n = room / slot_bytes(tile, rows);
+  const size_t room = 227 * 1024 - 1024 /*alignment*/ - fixed - kRedBytes, n = room / slot_bytes(tile, rows);
   return n > (size_t)kMaxStages ? kMaxStages : (int)n;
 }
-inline size_t ring_smem(int tile, int rows, int stages) { return 1024 + red_bytes(tile) + (size_t)slot_bytes(tile, rows) * stages; }
+inline size_t ring_smem(int tile, int rows, int stages) { return 1024 + kRedBytes + (size_t)slot_bytes(tile, rows) * stages; }
 
 // Weights of `rows` rows of row_bytes (a multiple of 16) each, elements of `size` bytes; 128-byte swizzle.
 inline bool weight_maps(WeightMaps* m, const void* base, unsigned long long rows, unsigned long long row_bytes, CUtensorMapDataType type,

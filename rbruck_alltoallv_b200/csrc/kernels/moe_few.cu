@@ -16,6 +16,7 @@
 #include <cuda_runtime.h>
 
 #include <cstdint>
+#include <type_traits>
 
 #include "kernels/few_rows.cuh"
 #include "kernels/pdl.cuh"
@@ -25,8 +26,6 @@ namespace rbv {
 namespace {
 
 using namespace few;
-
-constexpr int kMaxSlots = kMaxRows * kMoeFewMaxTopK;
 
 struct FewArgs {
   const uint8_t* x;
@@ -44,7 +43,9 @@ struct FewArgs {
 };
 
 // The choice, as every CTA makes it.
+template <int TOKENS>
 struct Choice {
+  static constexpr int kMaxSlots = TOKENS * kMoeFewMaxTopK;
   short expert[kMaxSlots];                // of slot t * top_k + j; negative: none
   float weight[kMaxSlots];
   short at[kMaxSlots];                    // row of the slot among its expert's rows
@@ -65,49 +66,58 @@ __device__ __forceinline__ unsigned logit_key(float v) {
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 
-__device__ __forceinline__ void choose(Choice& c, const FewArgs& a) {   // all threads of the CTA
+// The choice of one token by one warp, for E <= 32 * WORDS; lane j gets the j-th expert (negative: none) and its weight.
+template <int WORDS>
+__device__ __forceinline__ void choose_token(const float* row, int E, int top_k, int lane, int& expert, float& weight) {
+  unsigned key[WORDS];
+  float val[WORDS];
+  #pragma unroll
+  for (int j = 0; j < WORDS; j++) val[j] = j * 32 + lane < E ? __ldcg(row + j * 32 + lane) : 0.0f;
+  #pragma unroll
+  for (int j = 0; j < WORDS; j++) key[j] = j * 32 + lane < E ? logit_key(val[j]) : 0u;
+  float first = 0.0f, sum = 0.0f;
+  expert = -1;
+  weight = 0.0f;
+  for (int k = 0; k < top_k; k++) {
+    unsigned best = 0u;
+    #pragma unroll
+    for (int j = 0; j < WORDS; j++) best = max(best, key[j]);
+    best = __reduce_max_sync(0xffffffffu, best);
+    if (best <= kMasked) break;
+    int e = 0x7fffffff;
+    #pragma unroll
+    for (int j = WORDS - 1; j >= 0; j--)
+      if (key[j] == best) e = j * 32 + lane;
+    e = __reduce_min_sync(0xffffffffu, e);
+    float v = 0.0f;
+    #pragma unroll
+    for (int j = 0; j < WORDS; j++)
+      if (j == (e >> 5)) {
+        v = val[j];
+        if (lane == (e & 31)) key[j] = 0u;
+      }
+    v = __shfl_sync(0xffffffffu, v, e & 31);
+    if (k == 0) first = v;
+    const float p = __expf(v - first);
+    sum += p;
+    if (lane == k) { expert = e; weight = p; }
+  }
+  if (expert >= 0) weight /= sum;
+}
+
+template <int TOKENS>
+__device__ __forceinline__ void choose(Choice<TOKENS>& c, const FewArgs& a) {   // all threads of the CTA
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, warps = blockDim.x >> 5;
   const int slots = a.T * a.top_k;
   for (int t = warp; t < a.T; t += warps) {
-    unsigned key[kMoeMaxExperts / 32];
-    float val[kMoeMaxExperts / 32];
     const float* row = a.logits + (long long)t * a.ldl;
-    #pragma unroll
-    for (int j = 0; j < kMoeMaxExperts / 32; j++) {
-      const int e = j * 32 + lane;
-      val[j] = e < a.E ? __ldcg(row + e) : 0.0f;
-    }
-    #pragma unroll
-    for (int j = 0; j < kMoeMaxExperts / 32; j++) key[j] = j * 32 + lane < a.E ? logit_key(val[j]) : 0u;
-    float first = 0.0f, sum = 0.0f, mine = 0.0f;
-    int chosen = -1;
-    for (int k = 0; k < a.top_k; k++) {
-      unsigned best = 0u;
-      #pragma unroll
-      for (int j = 0; j < kMoeMaxExperts / 32; j++) best = max(best, key[j]);
-      best = __reduce_max_sync(0xffffffffu, best);
-      if (best <= kMasked) break;
-      int e = 0x7fffffff;
-      #pragma unroll
-      for (int j = kMoeMaxExperts / 32 - 1; j >= 0; j--)
-        if (key[j] == best) e = j * 32 + lane;
-      e = __reduce_min_sync(0xffffffffu, e);
-      float v = 0.0f;
-      #pragma unroll
-      for (int j = 0; j < kMoeMaxExperts / 32; j++)
-        if (j == (e >> 5)) {
-          v = val[j];
-          if (lane == (e & 31)) key[j] = 0u;
-        }
-      v = __shfl_sync(0xffffffffu, v, e & 31);
-      if (k == 0) first = v;
-      const float p = __expf(v - first);
-      sum += p;
-      if (lane == k) { chosen = e; mine = p; }
-    }
+    int expert;
+    float weight;
+    if (a.E <= 64) choose_token<2>(row, a.E, a.top_k, lane, expert, weight);
+    else choose_token<kMoeMaxExperts / 32>(row, a.E, a.top_k, lane, expert, weight);
     if (lane < a.top_k) {
-      c.expert[t * a.top_k + lane] = (short)chosen;
-      c.weight[t * a.top_k + lane] = chosen >= 0 ? mine / sum : 0.0f;
+      c.expert[t * a.top_k + lane] = (short)expert;
+      c.weight[t * a.top_k + lane] = weight;
     }
   }
   __syncthreads();
@@ -127,7 +137,7 @@ __device__ __forceinline__ void choose(Choice& c, const FewArgs& a) {   // all t
       if (lane >= o) before += v;
     }
     if (lane == 31) { c.warp_used[warp] = __popc(has); c.warp_rows[warp] = before; }
-    asm volatile("bar.sync 2, 256;" ::: "memory");
+    consumers_sync();
     int u = __popc(has & ((1u << lane) - 1u)), r = before - n, all_used = 0, all_rows = 0;
     for (int w = 0; w < 8; w++) {
       if (w < warp) { u += c.warp_used[w]; r += c.warp_rows[w]; }
@@ -148,12 +158,12 @@ __device__ __forceinline__ void choose(Choice& c, const FewArgs& a) {   // all t
   __syncthreads();
 }
 
+template <int TOKENS>
 struct Shared {
   Ring ring;
-  Choice choice;
-  int flag;
+  Choice<TOKENS> choice;
+  int flag[2];
 };
-
 __device__ __forceinline__ uint8_t* aligned_smem(uint8_t* p) {
   return reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(p) + 1023) & ~uintptr_t(1023));
 }
@@ -162,30 +172,32 @@ __device__ __forceinline__ uint8_t* aligned_smem(uint8_t* p) {
 struct UpPiece { int u, row0, rows; };    // used expert, first weight row, weight rows
 
 struct UpWalk {
-  long long at, end;
-  int per_expert, tile;                   // in groups of 8 rows
+  unsigned at, end, per_expert, tile;     // in groups of 8 rows
+  unsigned u, g;                          // used expert and group of `at`
   __device__ __forceinline__ UpWalk(const FewArgs& a, int n_used) {
     per_expert = 2 * a.I / 8;
     tile = a.tile / 8;
-    const long long total = (long long)n_used * per_expert;
-    at = total * blockIdx.x / gridDim.x;
-    end = total * (blockIdx.x + 1) / gridDim.x;
+    const Split split{n_used * per_expert, gridDim.x};
+    at = split.begin(blockIdx.x);
+    end = split.begin(blockIdx.x + 1);
+    u = at / per_expert;
+    g = at - u * per_expert;
   }
   __device__ __forceinline__ bool next(UpPiece& p) {
     if (at >= end) return false;
-    p.u = (int)(at / per_expert);
-    const int g = (int)(at - (long long)p.u * per_expert);
-    const int n = (int)min((long long)min(tile, per_expert - g), end - at);
+    if (g == per_expert) { g = 0; u++; }
+    const unsigned n = min(min(tile, per_expert - g), end - at);
+    p.u = u;
     p.row0 = g * 8;
     p.rows = n * 8;
     at += n;
+    g += n;
     return true;
   }
 };
 
-template <typename S>
-__device__ __forceinline__ bool up_piece(const FewArgs& a, Shared& s, uint4* red, uint32_t slots, Cursor& cur, const UpPiece& p, int warp,
-                                         int lane, bool ok) {
+template <typename S, int TOKENS>
+__device__ __forceinline__ void up_piece(const FewArgs& a, Shared<TOKENS>& s, uint4* red, Cursor& cur, const UpPiece& p, int warp, int lane) {
   const int R = s.choice.rows[p.u], groups = p.rows / 8, part = warp >> 2, col = warp & 3;
   const int g0 = S::group0(part, groups), mine = S::my_groups(part, groups);
   uint32_t off[S::GROUPS];
@@ -203,49 +215,44 @@ __device__ __forceinline__ bool up_piece(const FewArgs& a, Shared& s, uint4* red
   float acc[S::MT][S::GROUPS][4];
   clear<S>(acc);
   const int row_bytes = 2 * a.H, chunks = (row_bytes + kChunk - 1) / kChunk;
-  Rows<S> ahead[S::AHEAD + 1];             // (beyond the last chunk nothing is read)
-  #pragma unroll
-  for (int i = 0; i < S::AHEAD; i++) ahead[i].load(src, row_bytes, i, col, lane);
-  for (int c = 0; c < chunks; c++) {
-    ahead[S::AHEAD].load(src, row_bytes, c + S::AHEAD, col, lane);
-    if (ok && !sm100::mbar_wait(&s.ring.full[cur.stage], cur.phase, &s.ring.abort)) { ok = false; s.ring.abort = 1; }
-    __syncwarp();
-    multiply<S>(acc, slots + (uint32_t)cur.stage * slot_bytes(a.tile, 0), off, mine, ahead[0], lane);
-    __syncwarp();
-    if (lane == 0) sm100::mbar_arrive(&s.ring.empty[cur.stage]);
-    cur.next(a.stages);
+  auto run = [&](auto tag) {
+    constexpr int G = decltype(tag)::value;
+    Rows<S> ahead[S::AHEAD + 1];             // (beyond the last chunk nothing is read)
     #pragma unroll
-    for (int i = 0; i < S::AHEAD; i++) ahead[i] = ahead[i + 1];
-  }
-  #pragma unroll
-  for (int m = 0; m < S::MT; m++) {
-    float v[S::SETS][4];
-    add_columns<S>(acc[m], red, groups, warp, lane, v);
-    if (warp < groups)
+    for (int i = 0; i < S::AHEAD; i++) ahead[i].load(src, row_bytes, i, col, lane);
+    #pragma unroll 1
+    for (int c = 0; c < chunks; c++) {
+      ahead[S::AHEAD].load(src, row_bytes, c + S::AHEAD, col, lane);
+      cur.wait_full();
+      __syncwarp();
+      multiply<S, G>(acc, cur.slot, off, mine, ahead[0], lane);
+      __syncwarp();
+      if (lane == 0) cur.release();
+      cur.next();
       #pragma unroll
-      for (int i = 0; i < 2 * S::SETS; i++) {
-        const int q = i >> 1, h = i & 1, r = S::row(m, q, h, lane);
-        if (r < R) {
-          const int slot = list[r];
-          const float gate = v[q][2 * h], up = v[q][2 * h + 1];
-          const float y = s.choice.weight[slot] * (gate / (1.0f + __expf(-gate)) * up);
-          a.h[(long long)(s.choice.start[p.u] + r) * a.I + p.row0 / 2 + warp * 4 + (lane & 3)] = __float2bfloat16_rn(y);
-        }
-      }
-  }
-  return ok;
+      for (int i = 0; i < S::AHEAD; i++) ahead[i] = ahead[i + 1];
+    }
+  };
+  if (S::GROUPS == 4 && S::MT == 1 && groups <= 4) run(std::integral_constant<int, 2>());
+  else run(std::integral_constant<int, S::GROUPS>());
+  add_columns<S>(acc, red, g0, mine, part, col, lane, [&](int r, int row, float gate, float up) {
+    if (r >= R) return;
+    const int i = s.choice.start[p.u] + r;
+    const float y = s.choice.weight[s.choice.list[i]] * (gate / (1.0f + __expf(-gate)) * up);
+    a.h[(long long)i * a.I + (p.row0 + row) / 2] = __float2bfloat16_rn(y);
+  });
 }
 
-// MAX: rows of an expert at most, 16, 32 or 64.
+// MAX: tokens, and with them rows of an expert, at most: 16, 32 or 64.
 template <int MAX>
 __global__ void __launch_bounds__(kThreads, 1) moe_few_up_kernel(const __grid_constant__ WeightMaps maps, const __grid_constant__ FewArgs a) {
   extern __shared__ uint8_t dyn[];
-  __shared__ Shared s;
+  __shared__ Shared<MAX> s;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   uint8_t* base = aligned_smem(dyn);
   uint4* red = reinterpret_cast<uint4*>(base);
-  uint8_t* slots = base + red_bytes(a.tile);
   if (threadIdx.x == 0) ring_init(s.ring, a.stages, 1);
+  if (warp == kWarps && lane < 4 && maps.whole) sm100::tma_prefetch_desc(&maps.all[lane]);
   pdl_wait();
   pdl_trigger();      // after the wait: the down kernel reads the logits before it waits for this one
   if (blockIdx.x == 0)
@@ -253,73 +260,68 @@ __global__ void __launch_bounds__(kThreads, 1) moe_few_up_kernel(const __grid_co
   choose(s.choice, a);
   UpWalk walk(a, s.choice.n_used);
   UpPiece p;
-  Cursor cur;
+  Cursor cur(s.ring, sm100::smem_u32(base + kRedBytes), a.stages, slot_bytes(a.tile, 0));
   if (warp >= kWarps) {
     if (warp != kWarps || lane != 0) return;
     const int chunks = (2 * a.H + kChunk - 1) / kChunk;
-    bool ok = true;
-    while (ok && walk.next(p)) {
-      const int row0 = s.choice.used[p.u] * 2 * a.I + p.row0;
-      for (int c = 0; c < chunks; c++) {
-        ok = sm100::mbar_wait(&s.ring.empty[cur.stage], cur.phase ^ 1u, &s.ring.abort);
-        if (!ok) break;
-        fetch<__nv_bfloat16>(maps, slots + (size_t)cur.stage * slot_bytes(a.tile, 0), row0, p.rows, c, &s.ring.full[cur.stage]);
-        cur.next(a.stages);
-      }
-    }
-    if (!ok) s.ring.abort = 1;
+    while (walk.next(p) && feed<__nv_bfloat16>(maps, cur, 0, s.choice.used[p.u] * 2 * a.I + p.row0, p.rows, 0, chunks)) {}
     return;
   }
-  bool ok = true;
-  const uint32_t at = sm100::smem_u32(slots);
   while (walk.next(p)) {
     const int R = s.choice.rows[p.u];
-    if (MAX == 16 || R <= 16) ok = up_piece<Spread<1, false>>(a, s, red, at, cur, p, warp, lane, ok);
-    else if (MAX == 32 || R <= 32) ok = up_piece<Spread<2, false>>(a, s, red, at, cur, p, warp, lane, ok);
-    else ok = up_piece<Spread<2, true>>(a, s, red, at, cur, p, warp, lane, ok);
+    if (MAX == 16 || R <= 16) up_piece<Spread<1, false>>(a, s, red, cur, p, warp, lane);
+    else if (MAX == 32 || R <= 32) up_piece<Spread<2, false>>(a, s, red, cur, p, warp, lane);
+    else up_piece<Spread<2, true>>(a, s, red, cur, p, warp, lane);
   }
-  if (!ok && a.error) atomicExch(a.error, 1);
+  if (!cur.ok && a.error) atomicExch(a.error, 1);
 }
 
 // ---- down: column tiles of the result x used experts x chunks of K, split evenly among the CTAs -------------------------
+struct DownPiece { int tile, u, c0, c1; };       // column tile, used expert, chunks of K
+
 struct DownWalk {
   Split split;
-  long long at, end;
-  int chunks, per_tile, n_used;
+  unsigned at, end, per_tile;             // in steps
+  int chunks, n_used;
   int tile, u, c;                         // of step `at`
   __device__ __forceinline__ DownWalk(const FewArgs& a, int n_used_) {
     n_used = n_used_;
     chunks = (2 * a.I + kChunk - 1) / kChunk;
     per_tile = n_used * chunks;
-    split.total = (long long)((a.H + a.tile - 1) / a.tile) * per_tile;
-    split.parts = (int)min((long long)gridDim.x, split.total);
+    split.total = (unsigned)((a.H + a.tile - 1) / a.tile) * per_tile;
+    split.parts = min(gridDim.x, split.total);
     at = end = 0;
-    if ((int)blockIdx.x < split.parts) { at = split.begin(blockIdx.x); end = split.begin(blockIdx.x + 1); }
-    tile = (int)(at / per_tile);
-    const int in_tile = (int)(at - (long long)tile * per_tile);
+    if (blockIdx.x < split.parts) { at = split.begin(blockIdx.x); end = split.begin(blockIdx.x + 1); }
+    tile = at / per_tile;
+    const unsigned in_tile = at - tile * per_tile;
     u = in_tile / chunks;
     c = in_tile - u * chunks;
   }
-  __device__ __forceinline__ void step() {
-    at++;
-    if (++c == chunks) {
-      c = 0;
-      if (++u == n_used) { u = 0; tile++; }
-    }
+  __device__ __forceinline__ bool next(DownPiece& p) {
+    if (at >= end) return false;
+    p.tile = tile;
+    p.u = u;
+    p.c0 = c;
+    p.c1 = (int)min((unsigned)chunks, c + (end - at));
+    at += p.c1 - p.c0;
+    c = 0;                                // (the next one begins an expert, or there is none)
+    if (++u == n_used) { u = 0; tile++; }
+    return true;
   }
 };
 
-template <typename S>       // by the tokens: 16, 32 or 64 at most
+template <int MAX>
 __global__ void __launch_bounds__(kThreads, 1) moe_few_down_kernel(const __grid_constant__ WeightMaps maps, const __grid_constant__ WeightMaps h_maps,
                                                                    const __grid_constant__ FewArgs a) {
   extern __shared__ uint8_t dyn[];
-  __shared__ Shared s;
+  __shared__ Shared<MAX> s;
+  using S = Spread<(MAX > 16 ? 2 : 1), (MAX > 32)>;
   constexpr int MT = S::MT;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   uint8_t* base = aligned_smem(dyn);
   uint4* red = reinterpret_cast<uint4*>(base);
-  uint8_t* slots = base + red_bytes(a.tile);
   if (tid == 0) ring_init(s.ring, a.stages, 2);
+  if (warp >= kWarps && lane < 4 && maps.whole) sm100::tma_prefetch_desc(warp == kWarps ? &maps.all[lane] : &h_maps.all[lane]);
   pdl_trigger();
   choose(s.choice, a);
   const int n_used = s.choice.n_used;
@@ -330,111 +332,122 @@ __global__ void __launch_bounds__(kThreads, 1) moe_few_down_kernel(const __grid_
     return;
   }
   DownWalk walk(a, n_used);
-  Cursor cur;
+  DownPiece p;
+  Cursor cur(s.ring, sm100::smem_u32(base + kRedBytes), a.stages, slot_bytes(a.tile, a.box));
   if (warp >= kWarps) {                   // the weights do not wait for the first kernel, the rows of h do
     if (lane != 0) return;
-    const bool weights = warp == kWarps;
-    bool ok = true;
-    if (!weights) {
+    if (warp == kWarps) {
+      while (walk.next(p)) {
+        const int col0 = p.tile * a.tile;
+        if (!feed<__nv_bfloat16>(maps, cur, 0, s.choice.used[p.u] * a.H + col0, min(a.tile, a.H - col0), p.c0, p.c1)) break;
+      }
+    } else {
       pdl_wait();
       asm volatile("fence.proxy.async;" ::: "memory");
+      while (walk.next(p) &&
+             feed<__nv_bfloat16>(h_maps, cur, (uint32_t)a.tile * kChunk, s.choice.start[p.u], box_rows(s.choice.rows[p.u]), p.c0, p.c1)) {}
     }
-    for (; walk.at < walk.end; walk.step()) {
-      ok = sm100::mbar_wait(&s.ring.empty[cur.stage], cur.phase ^ 1u, &s.ring.abort);
-      if (!ok) break;
-      uint8_t* slot = slots + (size_t)cur.stage * slot_bytes(a.tile, a.box);
-      uint64_t* bar = &s.ring.full[cur.stage];
-      if (weights) {
-        const int col0 = walk.tile * a.tile;
-        fetch<__nv_bfloat16>(maps, slot, s.choice.used[walk.u] * a.H + col0, min(a.tile, a.H - col0), walk.c, bar);
-      } else {
-        fetch<__nv_bfloat16>(h_maps, slot + a.tile * kChunk, s.choice.start[walk.u], box_rows(s.choice.rows[walk.u]), walk.c, bar);
-      }
-      cur.next(a.stages);
-    }
-    if (!ok) s.ring.abort = 1;
     return;
   }
   pdl_wait();
-  bool ok = true;
-  const uint32_t slots_at = sm100::smem_u32(slots);
+  int cut[2] = {-1, -1};                  // tiles shared with the CTA before and the CTA behind
   const int part = warp >> 2, wcol = warp & 3;
-  while (walk.at < walk.end) {
-    const int tile = walk.tile;
-    const long long first = (long long)tile * walk.per_tile, at0 = walk.at, stop = min(walk.end, first + walk.per_tile);
-    const int col0 = tile * a.tile, nr = min(a.tile, a.H - col0), groups = nr / 8;
+  bool more = walk.next(p);
+  while (more) {
+    const int tile = p.tile, col0 = tile * a.tile, nr = min(a.tile, a.H - col0), groups = nr / 8;
+    const bool starts = p.u == 0 && p.c0 == 0;
     const int g0 = S::group0(part, groups), mine = S::my_groups(part, groups);
     uint32_t off[S::GROUPS];
     #pragma unroll
     for (int n = 0; n < S::GROUPS; n++) off[n] = group_offset(nr, g0 + n, wcol);
     float acc[MT][S::GROUPS][4];
     clear<S>(acc);
-    // where the tokens' rows of h are in a stage of expert u: tokens that did not choose it count as zeros
-    int u = -1, box = 0, rows_at[MT][2];
-    for (; walk.at < stop; walk.step()) {
-      if (walk.u != u) {
-        u = walk.u;
-        box = box_rows(s.choice.rows[u]);
-        const int e = s.choice.used[u];
+    bool ends;
+    do {
+      // where the tokens' rows of h are in a stage of the expert: tokens that did not choose it count as zeros
+      const int box = box_rows(s.choice.rows[p.u]), e = s.choice.used[p.u];
+      int rows_at[MT][2];
+      #pragma unroll
+      for (int m = 0; m < MT; m++)
         #pragma unroll
-        for (int m = 0; m < MT; m++)
-          #pragma unroll
-          for (int h = 0; h < 2; h++) {
-            const int t = S::row(m, S::set(part), h, lane);
-            rows_at[m][h] = -1;
-            if (t < a.T)
-              for (int j = 0; j < a.top_k; j++)
-                if (s.choice.expert[t * a.top_k + j] == e) rows_at[m][h] = s.choice.at[t * a.top_k + j];
-          }
+        for (int h = 0; h < 2; h++) {
+          const int t = S::row(m, S::set(part), h, lane);
+          rows_at[m][h] = -1;
+          if (t < a.T)
+            for (int j = 0; j < a.top_k; j++)
+              if (s.choice.expert[t * a.top_k + j] == e) rows_at[m][h] = s.choice.at[t * a.top_k + j];
+        }
+      auto run = [&](auto tag) {
+        constexpr int G = decltype(tag)::value;
+        #pragma unroll 1
+        for (int c = p.c0; c < p.c1; c++) {
+          cur.wait_full();
+          __syncwarp();
+          Rows<S> rows;
+          rows.load(rows_at, cur.slot + (uint32_t)a.tile * kChunk, box, wcol, lane);
+          multiply<S, G>(acc, cur.slot, off, mine, rows, lane);
+          __syncwarp();
+          if (lane == 0) cur.release();
+          cur.next();
+        }
+      };
+      if (MAX == 16 && groups <= 2) run(std::integral_constant<int, 1>());
+      else if (MAX == 16 && groups <= 4) run(std::integral_constant<int, 2>());
+      else run(std::integral_constant<int, S::GROUPS>());
+      ends = p.u == n_used - 1 && p.c1 == walk.chunks;
+      more = walk.next(p);
+    } while (more && p.tile == tile);
+    // a tile cut by the end of a range: the sums go to the workspace, for the last CTA to arrive
+    const bool whole = starts && ends;
+    float* part_sums = a.partial + (2ll * blockIdx.x + (starts ? 1 : 0)) * a.T * a.tile;
+    add_columns<S>(acc, red, g0, mine, part, wcol, lane, [&](int t, int col, float v0, float v1) {
+      if (t >= a.T) return;
+      if (whole) *reinterpret_cast<__nv_bfloat162*>(a.out + (long long)t * a.H + col0 + col) = __floats2bfloat162_rn(v0, v1);
+      else *reinterpret_cast<float2*>(part_sums + (long long)t * a.tile + col) = make_float2(v0, v1);
+    });
+    if (!whole) cut[starts ? 1 : 0] = tile;
+  }
+  // the (at most two) tiles that this CTA shares with others
+  if (cut[0] >= 0 || cut[1] >= 0) {
+    auto owners = [&](int tile, int& c0, int& c1) {
+      const unsigned first = tile * walk.per_tile;
+      c0 = walk.split.owner(first);
+      c1 = walk.split.owner(first + walk.per_tile - 1);
+    };
+    __threadfence();
+    consumers_sync();
+    if (tid < 2) {
+      int last = 0;
+      if (cut[tid] >= 0) {
+        int c0, c1;
+        owners(cut[tid], c0, c1);
+        last = atomicAdd(a.counters + cut[tid], 1) == c1 - c0;
       }
-      if (ok && !sm100::mbar_wait(&s.ring.full[cur.stage], cur.phase, &s.ring.abort)) { ok = false; s.ring.abort = 1; }
-      __syncwarp();
-      const uint32_t slot = slots_at + (uint32_t)cur.stage * slot_bytes(a.tile, a.box);
-      Rows<S> rows;
-      rows.load(rows_at, slot + (uint32_t)a.tile * kChunk, box, wcol, lane);
-      multiply<S>(acc, slot, off, mine, rows, lane);
-      __syncwarp();
-      if (lane == 0) sm100::mbar_arrive(&s.ring.empty[cur.stage]);
-      cur.next(a.stages);
+      s.flag[tid] = last;
     }
-    const bool whole = at0 == first && stop == first + walk.per_tile;
-    // a tile cut by the end of a range: sums to the workspace, the last CTA to arrive adds them up
-    float* part = a.partial + (2ll * blockIdx.x + (at0 == first ? 1 : 0)) * a.T * a.tile;
-    #pragma unroll
-    for (int m = 0; m < MT; m++) {
-      float v[S::SETS][4];
-      add_columns<S>(acc[m], red, groups, warp, lane, v);
-      if (warp < groups)
-        #pragma unroll
-        for (int i = 0; i < 2 * S::SETS; i++) {
-          const int q = i >> 1, h = i & 1, t = S::row(m, q, h, lane), col = warp * 8 + (lane & 3) * 2;
-          if (t >= a.T) continue;
-          if (whole)
-            *reinterpret_cast<__nv_bfloat162*>(a.out + (long long)t * a.H + col0 + col) = __floats2bfloat162_rn(v[q][2 * h], v[q][2 * h + 1]);
-          else
-            *reinterpret_cast<float2*>(part + (long long)t * a.tile + col) = make_float2(v[q][2 * h], v[q][2 * h + 1]);
+    consumers_sync();
+    for (int i = 0; i < 2; i++) {
+      if (!s.flag[i]) continue;
+      __threadfence();
+      int c0, c1;
+      owners(cut[i], c0, c1);
+      const int col0 = cut[i] * a.tile, pairs = min(a.tile, a.H - col0) / 2;
+      for (int k = tid; k < a.T * pairs; k += kWarps * 32) {
+        const int t = k / pairs, col = (k - t * pairs) * 2;
+        // only the first one's range may have begun before the tile
+        const float* from = a.partial + 2ll * c0 * a.T * a.tile + (long long)t * a.tile + col;
+        float2 sum = __ldcg(reinterpret_cast<const float2*>(from + a.T * a.tile));
+        #pragma unroll 4
+        for (int c = 1; c <= c1 - c0; c++) {
+          const float2 v = __ldcg(reinterpret_cast<const float2*>(from + 2ll * c * a.T * a.tile));
+          sum.x += v.x;
+          sum.y += v.y;
         }
-    }
-    if (!whole) {
-      const int c0 = walk.split.owner(first), c1 = walk.split.owner(first + walk.per_tile - 1);
-      if (last_to_arrive(a.counters + tile, c1 - c0 + 1, &s.flag)) {
-        const int pairs = nr / 2;
-        for (int i = tid; i < a.T * pairs; i += kWarps * 32) {
-          const int t = i / pairs, col = (i - t * pairs) * 2;
-          float2 sum = make_float2(0.0f, 0.0f);
-          for (int k = c0; k <= c1; k++) {
-            const bool starts = max(walk.split.begin(k), first) == first;
-            const float2 v = __ldcg(reinterpret_cast<const float2*>(a.partial + (2ll * k + (starts ? 1 : 0)) * a.T * a.tile +
-                                                                    (long long)t * a.tile + col));
-            sum.x += v.x;
-            sum.y += v.y;
-          }
-          *reinterpret_cast<__nv_bfloat162*>(a.out + (long long)t * a.H + col0 + col) = __floats2bfloat162_rn(sum.x, sum.y);
-        }
+        *reinterpret_cast<__nv_bfloat162*>(a.out + (long long)t * a.H + col0 + col) = __floats2bfloat162_rn(sum.x, sum.y);
       }
     }
   }
-  if (!ok && a.error) atomicExch(a.error, 2);
+  if (!cur.ok && a.error) atomicExch(a.error, 2);
 }
 
 // ---- host side -------------------------------------------------------------------------------------------------------
@@ -454,13 +467,14 @@ bool few_plan(int T, int H, int I, int E, int top_k, FewPlan* p) {
   const long long steps = (long long)used * ((2 * I + kChunk - 1) / kChunk);
   p->down_tile = kMaxTile;
   while (p->down_tile > 8 && (H + p->down_tile - 1) / p->down_tile * steps < 8ll * p->sms) p->down_tile /= 2;
+  if ((H + p->down_tile - 1ll) / p->down_tile * steps * p->sms > 0xffffffffll || (long long)used * (2 * I / 8) * p->sms > 0xffffffffll) return false;
   p->h_bytes = round_up((size_t)T * top_k * I * 2, 256);
   p->partial_bytes = round_up((size_t)2 * p->sms * T * p->down_tile * 4, 256);
   p->counter_bytes = round_up((size_t)(H / 8) * 4, 256);
   return true;
 }
 
-template <int MAX, typename S>
+template <int MAX>
 cudaError_t few_launch(FewArgs a, const FewPlan& p, cudaStream_t st) {
   const CUtensorMapDataType bf16 = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   WeightMaps w13, w2, h;
@@ -470,13 +484,13 @@ cudaError_t few_launch(FewArgs a, const FewPlan& p, cudaStream_t st) {
   auto launch = [&](auto kernel, int tile, int box, const auto&... maps) {
     a.tile = tile;
     a.box = box;
-    a.stages = ring_stages(tile, box, sizeof(Shared));
+    a.stages = ring_stages(tile, box, sizeof(Shared<MAX>));
     const size_t smem = ring_smem(tile, box, a.stages);
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     return e != cudaSuccess ? e : launch_dependent(kernel, dim3(p.sms), dim3(kThreads), smem, st, maps..., a);
   };
   const cudaError_t e = launch(moe_few_up_kernel<MAX>, p.up_tile, 0, w13);
-  return e != cudaSuccess ? e : launch(moe_few_down_kernel<S>, p.down_tile, box_rows(a.T), w2, h);
+  return e != cudaSuccess ? e : launch(moe_few_down_kernel<MAX>, p.down_tile, box_rows(a.T), w2, h);
 }
 
 }  // namespace
@@ -509,7 +523,7 @@ extern "C" int rbv_moe_few_tokens(const void* x, long long ldx, const float* log
   a.out = static_cast<__nv_bfloat16*>(out);
   a.error = error_flag;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (T <= 16) return (int)few_launch<16, Spread<1, false>>(a, p, st);
-  if (T <= 32) return (int)few_launch<32, Spread<2, false>>(a, p, st);
-  return (int)few_launch<64, Spread<2, true>>(a, p, st);
+  if (T <= 16) return (int)few_launch<16>(a, p, st);
+  if (T <= 32) return (int)few_launch<32>(a, p, st);
+  return (int)few_launch<64>(a, p, st);
 }
