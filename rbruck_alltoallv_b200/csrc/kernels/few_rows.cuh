@@ -138,43 +138,34 @@ __device__ __forceinline__ void load_column(uint32_t dst, const CUtensorMap* m, 
 }
 
 // Fetches chunks c0 to c1 - 1 of `rows` rows (a multiple of 8) from `row0` on, one per stage, `off` bytes into it: box by box, in
-// a box column by column.  One thread, which gets a box on its way in 150 cycles or more whatever its size: there is one box
-// per stage for 64 rows (with a box per column the producer set the pace, 205 us against 119 for one token of a layer that
-// reads 704 MB).  False: a wait ran out, stop.
+// a box column by column.  Four lanes of a warp, one for each height of a box: a lane gets a box on its way in 150 cycles or
+// more whatever its size, so there is one box per height and stage (with a box per column the producer set the pace, 205 us
+// against 119 for one token of a layer that reads 704 MB).  False: a wait ran out, stop.
 template <typename E>                      // element: its size turns bytes along K into coordinates
 __device__ __forceinline__ bool feed(const WeightMaps& maps, Cursor& cur, uint32_t off, int row0, int rows, int c0, int c1) {
-  const uint32_t bytes = (uint32_t)rows * kChunk;
-  const int big = 28 - __clz(rows);        // the largest box that fits has 8 << big rows
+  const int lane = threadIdx.x & 31, height = 8 << lane;
+  const bool mine = (rows & height) != 0;
+  const int before = rows & ~(2 * height - 1);           // rows in larger boxes
+  const uint32_t bytes = (uint32_t)rows * kChunk, to = off + (uint32_t)before * kChunk;
+  const CUtensorMap *all = &maps.all[lane], *one = &maps.one[lane];
   int c = c0;
-  if (rows == 8 << big) {
-    const CUtensorMap* m = &maps.all[big];
-    #pragma unroll 1
-    for (; c < c1 && c < maps.whole; c++) {
-      cur.wait_empty();
-      if (!cur.ok) return false;
-      expect(cur.full, bytes);
-      load_box(cur.slot + off, m, row0, c * kCols, cur.full);
-      cur.next();
-    }
+  #pragma unroll 1
+  for (; c < c1 && c < maps.whole; c++) {
+    cur.wait_empty();
+    if (!cur.ok) return false;
+    if (lane == 0) expect(cur.full, bytes);
+    if (mine) load_box(cur.slot + to, all, row0 + before, c * kCols, cur.full);
+    cur.next();
   }
   #pragma unroll 1
   for (; c < c1; c++) {
     cur.wait_empty();
     if (!cur.ok) return false;
-    expect(cur.full, bytes);
-    uint32_t dst = cur.slot + off;
-    int at = 0;
-    #pragma unroll 1
-    for (int b = big; b >= 0; b--) {
-      if (!(rows & (8 << b))) continue;
-      if (c < maps.whole) load_box(dst, &maps.all[b], row0 + at, c * kCols, cur.full);
-      else
-        #pragma unroll 1
-        for (int j = 0; j < kCols; j++)
-          load_column(dst + (uint32_t)(j * (1024 << b)), &maps.one[b], (c * kChunk + j * 128) / (int)sizeof(E), row0 + at, cur.full);
-      dst += (uint32_t)kChunk << (b + 3);
-      at += 8 << b;
-    }
+    if (lane == 0) expect(cur.full, bytes);
+    if (mine)
+      #pragma unroll 1
+      for (int j = 0; j < kCols; j++)
+        load_column(cur.slot + to + (uint32_t)(j * 128 * height), one, (c * kChunk + j * 128) / (int)sizeof(E), row0 + before, cur.full);
     cur.next();
   }
   return true;
@@ -312,13 +303,14 @@ __device__ __forceinline__ void add_columns(const Acc (&acc)[S::MT][S::GROUPS][4
 }
 
 // ---- work split along K over CTAs ------------------------------------------------------------------------------------
-// `total` steps (tile by tile, each of `per_tile` steps along K) are cut into `parts` <= total contiguous ranges of equal
-// length (within one).  A tile whose steps lie in several ranges is finished by the last of their CTAs to arrive, which adds
-// the others' sums in the order of the ranges: the result does not depend on who that is.  (total * parts fits 32 bits.)
+// `total` steps (tile by tile, each of `per_tile` steps along K) are cut into `parts` contiguous ranges of equal length, within
+// one step, or within one tile where that costs less than to put tiles together again.  A tile whose steps lie in several
+// ranges is finished by the last of their CTAs to arrive, which adds the others' sums in the order of the ranges: the result
+// does not depend on who that is.  (total * parts fits 32 bits.)
 struct Split {
-  unsigned total, parts;
-  __device__ __forceinline__ unsigned begin(unsigned part) const { return part * total / parts; }
-  __device__ __forceinline__ unsigned owner(unsigned step) const { return ((step + 1) * parts - 1) / total; }
+  unsigned total, parts, grain;           // in units of `grain` steps, of which there are at least `parts`
+  __device__ __forceinline__ unsigned begin(unsigned part) const { return part * total / parts * grain; }
+  __device__ __forceinline__ unsigned owner(unsigned step) const { return ((step / grain + 1) * parts - 1) / total; }
 };
 
 // ---- host side -------------------------------------------------------------------------------------------------------

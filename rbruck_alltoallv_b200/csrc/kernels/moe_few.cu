@@ -39,7 +39,8 @@ struct FewArgs {
   int* counters;                          // one per column tile of the down product
   __nv_bfloat16* out;
   int* error;
-  int tile, box, stages;                  // weight rows of a piece and rows of A in a stage, at most; ring stages
+  int tile, box, stages, whole;                 // weight rows of a piece and rows of A in a stage, at most; ring stages;
+                                          // whole: tiles of the down product are not split
 };
 
 // The choice, as every CTA makes it.
@@ -177,7 +178,7 @@ struct UpWalk {
   __device__ __forceinline__ UpWalk(const FewArgs& a, int n_used) {
     per_expert = 2 * a.I / 8;
     tile = a.tile / 8;
-    const Split split{n_used * per_expert, gridDim.x};
+    const Split split{n_used * per_expert, gridDim.x, 1};
     at = split.begin(blockIdx.x);
     end = split.begin(blockIdx.x + 1);
     u = at / per_expert;
@@ -262,7 +263,7 @@ __global__ void __launch_bounds__(kThreads, 1) moe_few_up_kernel(const __grid_co
   UpPiece p;
   Cursor cur(s.ring, sm100::smem_u32(base + kRedBytes), a.stages, slot_bytes(a.tile, 0));
   if (warp >= kWarps) {
-    if (warp != kWarps || lane != 0) return;
+    if (warp != kWarps || lane >= 4) return;
     const int chunks = (2 * a.H + kChunk - 1) / kChunk;
     while (walk.next(p) && feed<__nv_bfloat16>(maps, cur, 0, s.choice.used[p.u] * 2 * a.I + p.row0, p.rows, 0, chunks)) {}
     return;
@@ -288,7 +289,9 @@ struct DownWalk {
     n_used = n_used_;
     chunks = (2 * a.I + kChunk - 1) / kChunk;
     per_tile = n_used * chunks;
-    split.total = (unsigned)((a.H + a.tile - 1) / a.tile) * per_tile;
+    const unsigned tiles = (a.H + a.tile - 1) / a.tile;
+    split.grain = a.whole ? per_tile : 1;
+    split.total = a.whole ? tiles : tiles * per_tile;
     split.parts = min(gridDim.x, split.total);
     at = end = 0;
     if (blockIdx.x < split.parts) { at = split.begin(blockIdx.x); end = split.begin(blockIdx.x + 1); }
@@ -335,7 +338,7 @@ __global__ void __launch_bounds__(kThreads, 1) moe_few_down_kernel(const __grid_
   DownPiece p;
   Cursor cur(s.ring, sm100::smem_u32(base + kRedBytes), a.stages, slot_bytes(a.tile, a.box));
   if (warp >= kWarps) {                   // the weights do not wait for the first kernel, the rows of h do
-    if (lane != 0) return;
+    if (lane >= 4) return;
     if (warp == kWarps) {
       while (walk.next(p)) {
         const int col0 = p.tile * a.tile;
@@ -451,7 +454,7 @@ __global__ void __launch_bounds__(kThreads, 1) moe_few_down_kernel(const __grid_
 }
 
 // ---- host side -------------------------------------------------------------------------------------------------------
-struct FewPlan { int sms, up_tile, down_tile; size_t h_bytes, partial_bytes, counter_bytes; };
+struct FewPlan { int sms, up_tile, down_tile, whole; size_t h_bytes, partial_bytes, counter_bytes; };
 
 size_t round_up(size_t v, size_t to) { return (v + to - 1) / to * to; }
 
@@ -463,10 +466,20 @@ bool few_plan(int T, int H, int I, int E, int top_k, FewPlan* p) {
   if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&p->sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return false;
   const int used = E < T * top_k ? E : T * top_k;   // experts in use, at most
   p->up_tile = tile_rows((long long)used * (2 * I / 8), p->sms);
-  // columns of the result in a piece: the most, in one box, that leave a CTA eight steps to share the work out evenly
-  const long long steps = (long long)used * ((2 * I + kChunk - 1) / kChunk);
-  p->down_tile = kMaxTile;
-  while (p->down_tile > 8 && (H + p->down_tile - 1) / p->down_tile * steps < 8ll * p->sms) p->down_tile /= 2;
+  // Columns of the result in a piece of the down product.  To put together a tile that several CTAs share takes as long as
+  // about 110 KB of weights per SM (2.5 us): where whole tiles, some width of them, leave no CTA more than that above an even
+  // share, they are not split.  Otherwise the widest, in one box, that leave a CTA eight steps to share the work out evenly.
+  const long long steps = (long long)used * ((2 * I + kChunk - 1) / kChunk), row = 2ll * used * I;
+  long long best = (long long)H * row / p->sms + (110 << 10);
+  p->whole = 0;
+  for (int tile = kMaxTile; tile >= 8; tile /= 2) {
+    const long long tiles = (H + tile - 1) / tile, most = (tiles + p->sms - 1) / p->sms * tile * row;
+    if (most < best) { best = most; p->whole = 1; p->down_tile = tile; }
+  }
+  if (!p->whole) {
+    p->down_tile = kMaxTile;
+    while (p->down_tile > 8 && (H + p->down_tile - 1) / p->down_tile * steps < 8ll * p->sms) p->down_tile /= 2;
+  }
   if ((H + p->down_tile - 1ll) / p->down_tile * steps * p->sms > 0xffffffffll || (long long)used * (2 * I / 8) * p->sms > 0xffffffffll) return false;
   p->h_bytes = round_up((size_t)T * top_k * I * 2, 256);
   p->partial_bytes = round_up((size_t)2 * p->sms * T * p->down_tile * 4, 256);
@@ -484,6 +497,7 @@ cudaError_t few_launch(FewArgs a, const FewPlan& p, cudaStream_t st) {
   auto launch = [&](auto kernel, int tile, int box, const auto&... maps) {
     a.tile = tile;
     a.box = box;
+    a.whole = p.whole;
     a.stages = ring_stages(tile, box, sizeof(Shared<MAX>));
     const size_t smem = ring_smem(tile, box, a.stages);
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
