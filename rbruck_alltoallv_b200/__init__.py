@@ -25,7 +25,8 @@ def __getattr__(name):
         from .parallel import comm as _c
         from .utils import selftest as _s
         return lambda *a, **k: _s.bench(_c.get_default_comm(), *a, **k)
-    if name in ("MoEExpertParallel", "grouped_gemm", "grouped_gemm_fp8", "moe_few_tokens"):
+    if name in ("MoEExpertParallel", "grouped_gemm", "grouped_gemm_fp8", "grouped_gemm_int8", "linear_int8", "quantize_rows_int8",
+                "quantize_weight_int8", "moe_few_tokens"):
         from .ops import moe as _m
         return getattr(_m, name)
     if name == "block_norm":

@@ -39,6 +39,9 @@ CUDA_SOURCES = [
     "kernels/grouped_gemm_fp8_pair_sm100.cu",
     "kernels/grouped_gemm_fp8_tok_sm100.cu",
     "kernels/grouped_gemm_mxfp8_sm100.cu",
+    "kernels/grouped_gemm_int8_sm100.cu",
+    "kernels/int8_quant.cu",
+    "kernels/linear_int8_few.cu",
     "kernels/fft_transpose.cu",
     "kernels/reshard.cu",
     "kernels/block_norm.cu",

@@ -117,6 +117,11 @@ def declare_moe(lib):
     lib.rbv_moe_route_local.argtypes = [vp, vp, i, i, i, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp]
     lib.rbv_moe_dispatch_local.argtypes = [vp, vp, i, i, vp, vp, vp, vp, vp, i, vp, vp, ll, vp, vp]
     lib.rbv_moe_combine_local.argtypes = [vp, vp, i, i, vp, vp, vp, vp]
+    lib.rbv_grouped_gemm_int8.argtypes = [vp, vp, ll, vp, vp, vp, vp, vp, i, i, i, i, i, vp, i, vp]
+    lib.rbv_quantize_rows_int8.argtypes = [vp, ll, vp, i, ll, vp, vp, vp]
+    lib.rbv_linear_int8_few_workspace.restype = ll
+    lib.rbv_linear_int8_few_workspace.argtypes = [i, i, i]
+    lib.rbv_linear_int8_few.argtypes = [vp, ll, i, vp, vp, i, i, vp, vp, vp, vp]
     lib.rbv_moe_few_workspace.restype = ll
     lib.rbv_moe_few_workspace.argtypes = [i] * 5
     lib.rbv_moe_few_tokens.argtypes = [vp, ll, vp, ll, i, i, i, i, i, vp, vp, vp, vp, vp, vp]

@@ -57,6 +57,24 @@ int rbv_grouped_gemm_fp8_pair(const void* A, const float* a_scale_t, long long a
 int rbv_grouped_gemm_fp8_tok(const void* A, const float* a_scale_t, long long a_rows, const void* B,
                              const float* b_scale, void* C, const int* group_start, const int* group_rows, int G,
                              int N, int K, int ldc, int epilogue, int* error_flag, int max_ctas, void* cuda_stream);
+/* 8-bit integers with one scale per row of A and one per row of B, exact 32-bit sums, bf16 results:
+ *   C[r][n] = a_scale[r] * b_scale[g][n] * sum_k A[r][k] * B[g][n][k], then the epilogues as above.
+ * A: [a_rows, K] int8, a_scale [a_rows];  B: [G, N, K] int8, b_scale [G][N].  N % 8 == 0, K % 16 == 0, K <= 131072.
+ * group_start and group_rows null with G = 1: one group of all rows.  error_flag may be null. */
+#define RBV_INT8_MAX_DEPTH 131072
+int rbv_grouped_gemm_int8(const void* A, const float* a_scale, long long a_rows, const void* B, const float* b_scale,
+                          void* C, const int* group_start, const int* group_rows, int G, int N, int K, int ldc,
+                          int epilogue, int* error_flag, int max_ctas, void* cuda_stream);
+/* bf16 [rows, K] (rows ldx elements apart, K % 8 == 0, ldx % 8 == 0) -> int8 [rows, K] + scale [rows]: scale = largest magnitude
+ * / 127, values rounded to nearest even.  A row with an infinity or a NaN gets the scale NaN, one whose values are all below
+ * 2^-100 zeros and the scale 1.  `used`: as below. */
+int rbv_quantize_rows_int8(const void* x_bf16, long long rows, const int* used, int K, long long ldx, void* out_int8,
+                           float* scale, void* cuda_stream);
+/* Linear of a few rows (1 <= M <= 64), quantised within the call: x [M, K] bf16, W [N, K] int8 with w_scale [N], out [M, N]
+ * bf16.  workspace: rbv_linear_int8_few_workspace(...) bytes of this call alone (-1 for sizes that are not taken). */
+long long rbv_linear_int8_few_workspace(int M, int N, int K);
+int rbv_linear_int8_few(const void* x, long long ldx, int M, const void* W, const float* w_scale, int N, int K, void* out,
+                        void* workspace, int* error_flag, void* cuda_stream);
 /* MXFP8 variant: e4m3 operands with one UE8M0 (power-of-two) scale per 32 elements along K on both operands, applied
  * by the tensor core (tcgen05.mma.kind::mxf8f6f4.block_scale) on CTA pairs.  Scales are packed four to a uint32 (the
  * four 32-blocks of one 128-wide K block, lowest byte first); the words of 128 consecutive rows form one 512-byte atom

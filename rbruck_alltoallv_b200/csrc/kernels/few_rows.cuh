@@ -320,6 +320,23 @@ inline int tile_rows(long long groups, int parts) {
   return (int)(n < 1 ? 8 : n > kMaxTile / 8 ? kMaxTile : n * 8);
 }
 
+// How `n` weight rows (or columns of the result) of row_bytes each, `experts` times, are cut: rows of a piece, and whether pieces
+// stay whole.  To put together a tile that several CTAs share takes as long as about 110 KB of weights per SM (2.5 us): where
+// whole tiles, some width of them, leave no CTA more than that above an even share, they are not split.  Otherwise the widest,
+// in one box, that leave a CTA eight steps to share the work out evenly.  False: too much for 32-bit step numbers.
+inline bool split_plan(long long n, long long row_bytes, long long experts, int sms, int* tile, int* whole) {
+  const long long steps = experts * ((row_bytes + kChunk - 1) / kChunk), row = experts * row_bytes;
+  long long best = n * row / sms + (110 << 10);
+  *whole = 0;
+  for (int t = kMaxTile; t >= 8; t /= 2) {
+    const long long tiles = (n + t - 1) / t, most = (tiles + sms - 1) / sms * t * row;
+    if (most < best) { best = most; *whole = 1; *tile = t; }
+  }
+  if (!*whole)
+    for (*tile = kMaxTile; *tile > 8 && (n + *tile - 1) / *tile * steps < 8ll * sms;) *tile /= 2;
+  return (n + *tile - 1) / *tile * steps * sms <= 0xffffffffll;
+}
+
 // Stages that fit beside `fixed` bytes of static shared memory.
 inline int ring_stages(int tile, int rows, size_t fixed) {
   const size_t room = 227 * 1024 - 1024 /*alignment*/ - fixed - kRedBytes, n = room / slot_bytes(tile, rows);

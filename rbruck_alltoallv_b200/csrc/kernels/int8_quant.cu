@@ -1,0 +1,146 @@
+// Rows of bf16 -> 8-bit integers with one scale per row:  s = max|x| / 127,  q = round-to-nearest-even(x / s).
+//
+// Bound by HBM: 2 bytes read and 1 written per element.  A row stays in the registers of the threads that share it between the
+// maximum and the quantisation (up to 16384 elements; longer rows are read twice).  The quotient is the correctly rounded
+// one, as x / s in 32 bits gives it: x times the reciprocal decides, except next to a half, where the division is done (a
+// division for every element would take longer than its bytes).  A row that holds an infinity or a NaN gets the scale NaN, so
+// that whatever is made of it is NaN; one whose values are all below 2^-100 counts as zeros (scale 1).
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+#include "kernels/pdl.cuh"
+#include "rbv/moe.h"
+
+namespace rbv {
+namespace {
+
+struct QuantArgs {
+  const __nv_bfloat16* x;
+  long long rows, ldx;
+  const int* used;            // optional: rows that hold anything
+  int K;                      // a multiple of 8
+  int8_t* q;                  // [rows, K]
+  float* scale;               // [rows]
+  int* zero;                  // optional: `zeros` words to set to zero (counters of the kernel behind this one)
+  int zeros;
+};
+
+// Largest magnitude of the eight values; a NaN turns into +inf, which the caller looks for.
+__device__ __forceinline__ float vec_max(uint4 v, float m) {
+  const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&v);
+  #pragma unroll
+  for (int j = 0; j < 4; j++) {
+    const float2 f = __bfloat1622float2(h[j]);
+    const float a = fabsf(f.x), b = fabsf(f.y);
+    m = fmaxf(m, a == a ? a : INFINITY);
+    m = fmaxf(m, b == b ? b : INFINITY);
+  }
+  return m;
+}
+
+__device__ __forceinline__ unsigned quantize(float x, float s, float inv) {
+  const float t = x * inv, r = rintf(t);
+  int i = __float2int_rn(t);
+  // |t| <= 127.01 and t is within 2^-22 of x / s, relatively: further than 2^-14 from a half both round alike
+  if (fabsf(fabsf(t - r) - 0.5f) < 6.2e-5f) i = __float2int_rn(__fdiv_rn(x, s));
+  return (unsigned)max(-127, min(127, i)) & 0xffu;
+}
+
+__device__ __forceinline__ uint2 quantize_vec(uint4 v, float s, float inv) {
+  const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&v);
+  unsigned w[2];
+  #pragma unroll
+  for (int j = 0; j < 2; j++) {
+    const float2 a = __bfloat1622float2(h[2 * j]), b = __bfloat1622float2(h[2 * j + 1]);
+    w[j] = quantize(a.x, s, inv) | (quantize(a.y, s, inv) << 8) | (quantize(b.x, s, inv) << 16) | (quantize(b.y, s, inv) << 24);
+  }
+  return make_uint2(w[0], w[1]);
+}
+
+// A row per blockDim.x threads (a warp, or the CTA); NV vectors per thread in registers, 0: read the row twice.
+template <int NV>
+__global__ void __launch_bounds__(512) quantize_rows_int8_kernel(const __grid_constant__ QuantArgs a) {
+  __shared__ float red[2][16];
+  pdl_wait();
+  pdl_trigger();      // after the wait: the kernel behind may read its weights before it waits for this one
+  if (a.zero && blockIdx.x == 0)
+    for (int i = threadIdx.y * blockDim.x + threadIdx.x; i < a.zeros; i += blockDim.x * blockDim.y) a.zero[i] = 0;
+  const long long rows = a.used ? min((long long)max(*a.used, 0), a.rows) : a.rows;
+  const int nvec = a.K / 8;
+  int turn = 0;
+  for (long long r = (long long)blockIdx.x * blockDim.y + threadIdx.y; r < rows; r += (long long)gridDim.x * blockDim.y) {
+    const uint4* x = reinterpret_cast<const uint4*>(a.x + r * a.ldx);
+    uint4 v[NV ? NV : 1];
+    float m = 0.0f;
+    if (NV) {
+      #pragma unroll
+      for (int i = 0; i < NV; i++) {
+        const int at = i * (int)blockDim.x + (int)threadIdx.x;
+        v[i] = make_uint4(0u, 0u, 0u, 0u);
+        if (at < nvec) v[i] = __ldg(x + at);
+      }
+      #pragma unroll
+      for (int i = 0; i < NV; i++) m = vec_max(v[i], m);
+    } else {
+      for (int at = threadIdx.x; at < nvec; at += blockDim.x) m = vec_max(__ldg(x + at), m);
+    }
+    #pragma unroll
+    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    if (blockDim.x > 32) {
+      const int lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+      if (lane == 0) red[turn][threadIdx.x >> 5] = m;
+      __syncthreads();
+      m = lane < warps ? red[turn][lane] : 0.0f;
+      turn ^= 1;
+      #pragma unroll
+      for (int o = 8; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+      m = __shfl_sync(0xffffffffu, m, 0);
+    }
+    const bool tiny = m < 0x1p-100f, bad = m == INFINITY;
+    const float s = tiny || bad ? 1.0f : __fdiv_rn(m, 127.0f), inv = tiny || bad ? 0.0f : __frcp_rn(s);
+    if (threadIdx.x == 0) a.scale[r] = bad ? __int_as_float(0x7fffffff) : s;
+    uint2* q = reinterpret_cast<uint2*>(a.q + r * a.K);
+    if (tiny || bad) {
+      for (int at = threadIdx.x; at < nvec; at += blockDim.x) q[at] = make_uint2(0u, 0u);
+    } else if (NV) {
+      #pragma unroll
+      for (int i = 0; i < NV; i++) {
+        const int at = i * (int)blockDim.x + (int)threadIdx.x;
+        if (at < nvec) q[at] = quantize_vec(v[i], s, inv);
+      }
+    } else {
+      for (int at = threadIdx.x; at < nvec; at += blockDim.x) q[at] = quantize_vec(__ldg(x + at), s, inv);
+    }
+  }
+}
+
+}  // namespace
+
+cudaError_t launch_quantize_rows_int8(const void* x, long long rows, const int* used, int K, long long ldx, void* q, float* scale,
+                                      int* zero, int zeros, cudaStream_t st) {
+  if (rows < 1 || K < 8 || K % 8 || ldx % 8) return cudaErrorInvalidValue;
+  if ((reinterpret_cast<uintptr_t>(x) & 15) || (reinterpret_cast<uintptr_t>(q) & 7)) return cudaErrorMisalignedAddress;
+  int dev = 0, sms = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  if (e != cudaSuccess) return e;
+  const QuantArgs a{static_cast<const __nv_bfloat16*>(x), rows, ldx, used, K, static_cast<int8_t*>(q), scale, zero, zeros};
+  const int nvec = K / 8;
+  const int threads = nvec <= 32 ? 32 : nvec <= 512 ? (nvec + 31) / 32 * 32 : 512, per_cta = threads == 32 ? 4 : 1;
+  const int nv = (nvec + threads - 1) / threads;
+  const long long want = (rows + per_cta - 1) / per_cta, most = (long long)sms * (2048 / (threads * per_cta));
+  const dim3 grid((unsigned)(want < most ? want : most)), block(threads, per_cta);
+  if (nv <= 1) return launch_dependent(quantize_rows_int8_kernel<1>, grid, block, 0, st, a);
+  if (nv <= 2) return launch_dependent(quantize_rows_int8_kernel<2>, grid, block, 0, st, a);
+  if (nv <= 4) return launch_dependent(quantize_rows_int8_kernel<4>, grid, block, 0, st, a);
+  return launch_dependent(quantize_rows_int8_kernel<0>, grid, block, 0, st, a);
+}
+
+}  // namespace rbv
+
+extern "C" int rbv_quantize_rows_int8(const void* x_bf16, long long rows, const int* used, int K, long long ldx, void* out_int8,
+                                      float* scale, void* cuda_stream) {
+  return (int)rbv::launch_quantize_rows_int8(x_bf16, rows, used, K, ldx, out_int8, scale, nullptr, 0, static_cast<cudaStream_t>(cuda_stream));
+}

@@ -466,21 +466,7 @@ bool few_plan(int T, int H, int I, int E, int top_k, FewPlan* p) {
   if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&p->sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return false;
   const int used = E < T * top_k ? E : T * top_k;   // experts in use, at most
   p->up_tile = tile_rows((long long)used * (2 * I / 8), p->sms);
-  // Columns of the result in a piece of the down product.  To put together a tile that several CTAs share takes as long as
-  // about 110 KB of weights per SM (2.5 us): where whole tiles, some width of them, leave no CTA more than that above an even
-  // share, they are not split.  Otherwise the widest, in one box, that leave a CTA eight steps to share the work out evenly.
-  const long long steps = (long long)used * ((2 * I + kChunk - 1) / kChunk), row = 2ll * used * I;
-  long long best = (long long)H * row / p->sms + (110 << 10);
-  p->whole = 0;
-  for (int tile = kMaxTile; tile >= 8; tile /= 2) {
-    const long long tiles = (H + tile - 1) / tile, most = (tiles + p->sms - 1) / p->sms * tile * row;
-    if (most < best) { best = most; p->whole = 1; p->down_tile = tile; }
-  }
-  if (!p->whole) {
-    p->down_tile = kMaxTile;
-    while (p->down_tile > 8 && (H + p->down_tile - 1) / p->down_tile * steps < 8ll * p->sms) p->down_tile /= 2;
-  }
-  if ((H + p->down_tile - 1ll) / p->down_tile * steps * p->sms > 0xffffffffll || (long long)used * (2 * I / 8) * p->sms > 0xffffffffll) return false;
+  if (!split_plan(H, 2ll * I, used, p->sms, &p->down_tile, &p->whole) || (long long)used * (2 * I / 8) * p->sms > 0xffffffffll) return false;
   p->h_bytes = round_up((size_t)T * top_k * I * 2, 256);
   p->partial_bytes = round_up((size_t)2 * p->sms * T * p->down_tile * 4, 256);
   p->counter_bytes = round_up((size_t)(H / 8) * 4, 256);

@@ -199,6 +199,15 @@ __device__ __forceinline__ void umma_bf16_pair(uint32_t d_tmem, uint64_t a_desc,
       ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
       : "memory");
 }
+// The same for 8-bit integers, signed x signed -> 32-bit integers: A[256 x 32] * B[N x 32]^T.
+__device__ __forceinline__ void umma_i8_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
 // One arrival on the barrier at this shared-memory offset in BOTH CTAs of the pair when the MMAs issued so far have
 // completed (a barrier signal, not a load).
 __device__ __forceinline__ void umma_commit_pair(uint64_t* bar) {
@@ -218,6 +227,11 @@ __device__ __forceinline__ uint64_t umma_desc_sw128(const void* smem_tile) {
 __host__ __device__ constexpr uint32_t umma_idesc(int M, int N, int ab_format /*0 f16, 1 bf16; f8: 0 e4m3*/) {
   return (1u << 4) | ((uint32_t)ab_format << 7) | ((uint32_t)ab_format << 10) | ((uint32_t)(N >> 3) << 17) |
          ((uint32_t)(M >> 4) << 24);
+}
+
+// Instruction descriptor of kind::i8: s32 accumulate, signed A and B, K-major.
+__host__ __device__ constexpr uint32_t umma_idesc_i8(int M, int N) {
+  return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
 }
 
 // Rows of a group that lie inside A.  An expert may be routed more rows than its GPU has room for: the dispatch drops them,

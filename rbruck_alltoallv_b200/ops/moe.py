@@ -266,6 +266,142 @@ def grouped_gemm_mxfp8_swiglu_q(Aq: torch.Tensor, sfa: torch.Tensor, Bq: torch.T
     return out_q, out_sf
 
 
+# ---- 8-bit integers: one scale per token and one per output channel, exact 32-bit sums -------------------------------------
+INT8_MAX_DEPTH = 131072          # K at which 127 * 127 * K still fits a 32-bit integer
+
+
+def _int8_rows(x: torch.Tensor):
+    """``x`` [rows, K] bf16 as the kernels read it: packed rows that start at 16-byte boundaries."""
+    if x.dtype != torch.bfloat16 or x.dim() != 2:
+        raise ValueError(f"rows must be a bf16 matrix, not {tuple(x.shape)} in {x.dtype}")
+    if x.shape[1] < 16 or x.shape[1] % 16 or x.shape[1] > INT8_MAX_DEPTH:
+        raise ValueError(f"depths of 16 to {INT8_MAX_DEPTH} in steps of 16 are supported, not {x.shape[1]}")
+    if not x.is_cuda:
+        raise ValueError("the rows must be on a GPU")
+    if x.stride(1) != 1 or x.data_ptr() % 16 or (x.shape[0] > 1 and (x.stride(0) % 8 or x.stride(0) < x.shape[1])):
+        x = x.clone(memory_format=torch.contiguous_format)
+    return x
+
+
+def quantize_rows_int8(x: torch.Tensor, used: Optional[torch.Tensor] = None):
+    """bf16 [rows, K] -> (int8 [rows, K], fp32 scales [rows]): ``scale = max|row| / 127``, values rounded to nearest even.  With
+    ``used`` (int32 CUDA tensor) only the first ``used[0]`` rows are quantised, the others are left undefined.  A row with an
+    infinity or a NaN gets the scale NaN (so that what is made of it is NaN), one whose values are all below 2^-100 becomes
+    zeros with the scale 1.  Rows may be strided; K is a multiple of 16."""
+    x = _int8_rows(x)
+    rows, K = x.shape
+    q = torch.empty(rows, K, dtype=torch.int8, device=x.device)
+    sc = torch.empty(rows, dtype=torch.float32, device=x.device)
+    if rows == 0:
+        return q, sc
+    with torch.cuda.device(x.device):
+        rc = _native.cuda_lib().rbv_quantize_rows_int8(_p(x), rows, _p(used), K, x.stride(0) if rows > 1 else K, _p(q), _p(sc),
+                                                       _native.current_stream(x.device.index))
+    if rc:
+        raise RuntimeError(f"int8 quantisation launch failed (CUDA error {rc})")
+    return q, sc
+
+
+def quantize_weight_int8(w: torch.Tensor):
+    """bf16 / fp32 [..., N, K] -> (int8 [..., N, K], fp32 scales [..., N]), one scale per output channel."""
+    f = w.float()
+    amax = f.abs().amax(dim=-1)
+    scale = torch.where(amax > 0, amax / 127.0, torch.ones_like(amax))
+    q = torch.round(f / scale[..., None]).clamp_(-127, 127).to(torch.int8)
+    return q.contiguous(), scale.contiguous()
+
+
+def dequantize_int8(q: torch.Tensor, scale: torch.Tensor) -> torch.Tensor:
+    """fp32 values that ``q`` [..., K] and its scales [...] stand for (rows or weights)."""
+    return q.float() * scale[..., None]
+
+
+def _int8_weight(w: torch.Tensor, scale: torch.Tensor, dim: int):
+    if w.dim() != dim or w.dtype != torch.int8 or scale.dtype != torch.float32 or scale.shape != w.shape[:-1]:
+        raise ValueError(f"weights must be int8 with {dim} dimensions and one fp32 scale per channel, not {tuple(w.shape)} in "
+                         f"{w.dtype} with scales {tuple(scale.shape)} in {scale.dtype}")
+    N, K = w.shape[-2:]
+    if N < 8 or N % 8 or K < 16 or K % 16 or K > INT8_MAX_DEPTH:
+        raise ValueError(f"channels in steps of 8 and depths of 16 to {INT8_MAX_DEPTH} in steps of 16 are supported, not {N} x {K}")
+    if not w.is_contiguous() or not scale.is_contiguous() or w.data_ptr() % 16 or scale.data_ptr() % 16:
+        raise ValueError("weights and scales must be contiguous and 16-byte aligned")
+
+
+def grouped_gemm_int8(Aq: torch.Tensor, a_scale: torch.Tensor, Bq: torch.Tensor, b_scale: torch.Tensor,
+                      group_start: torch.Tensor, group_rows: torch.Tensor, out: Optional[torch.Tensor] = None,
+                      swiglu: bool = False, error: Optional[torch.Tensor] = None, max_ctas: int = 0) -> torch.Tensor:
+    """``out[rows of g] = epi(a_scale[row] * b_scale[g][channel] * (Aq[rows of g] @ Bq[g].T))`` with 8-bit integer operands and
+    exact 32-bit integer sums (``csrc/kernels/grouped_gemm_int8_sm100.cu``); bf16 output.
+
+    ``Aq`` [M, K] int8 with ``a_scale`` [M], ``Bq`` [G, N, K] int8 with ``b_scale`` [G, N], ``group_start`` / ``group_rows`` int32
+    CUDA tensors [G], G <= 64; N a multiple of 8, K of 16.  With ``swiglu`` the rows of ``Bq[g]`` interleave gate and up projections
+    and ``out`` is [M, N // 2].  Rows of ``out`` outside the groups are left as they are."""
+    _int8_weight(Bq, b_scale, 3)
+    G, N, K = Bq.shape
+    if Aq.dim() != 2 or Aq.dtype != torch.int8 or Aq.shape[1] != K or a_scale.shape != Aq.shape[:1] or a_scale.dtype != torch.float32:
+        raise ValueError(f"rows must be int8 [M, {K}] with fp32 scales [M], not {tuple(Aq.shape)} in {Aq.dtype} with {tuple(a_scale.shape)}")
+    if not Aq.is_contiguous() or not a_scale.is_contiguous() or Aq.data_ptr() % 16:
+        raise ValueError("rows and scales must be contiguous and 16-byte aligned")
+    if not 1 <= G <= 64 or any(t.shape != (G,) or t.dtype != torch.int32 or not t.is_contiguous() for t in (group_start, group_rows)):
+        raise ValueError(f"group_start and group_rows must be int32 [{G}], with at most 64 groups")
+    M, n_out = Aq.shape[0], N // 2 if swiglu else N
+    if not Aq.is_cuda or any(t.device != Aq.device for t in (a_scale, Bq, b_scale, group_start, group_rows)):
+        raise ValueError("all tensors must be on one GPU")
+    if out is None:
+        out = torch.empty(M, n_out, dtype=torch.bfloat16, device=Aq.device)
+    elif (out.shape != (M, n_out) or out.dtype != torch.bfloat16 or out.device != Aq.device or out.stride(1) != 1 or out.stride(0) % 2
+          or out.data_ptr() % 4 or (M > 1 and out.stride(0) < n_out)):
+        raise ValueError(f"out must be a bf16 tensor [{M}, {n_out}] with packed, 4-byte aligned rows on the same GPU")
+    if M == 0:
+        return out
+    with torch.cuda.device(Aq.device):
+        rc = _native.cuda_lib().rbv_grouped_gemm_int8(_p(Aq), _p(a_scale), M, _p(Bq), _p(b_scale), _p(out), _p(group_start),
+                                                      _p(group_rows), G, N, K, out.stride(0) if M > 1 else n_out, 1 if swiglu else 0,
+                                                      _p(error), int(max_ctas), _native.current_stream(Aq.device.index))
+    if rc:
+        raise RuntimeError(f"int8 grouped GEMM launch failed (CUDA error {rc})")
+    return out
+
+
+def linear_int8(x: torch.Tensor, weight: torch.Tensor, scale: torch.Tensor, out: Optional[torch.Tensor] = None,
+                error: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``out[r][n] = s_r * scale[n] * sum_k q[r][k] * weight[n][k]`` where ``q``, ``s`` is ``x`` quantised row by row
+    (:func:`quantize_rows_int8`): a linear layer with 8-bit integer weights.
+
+    ``x`` [rows, K] bf16, ``weight`` [N, K] int8 and ``scale`` [N] fp32 (:func:`quantize_weight_int8`), ``out`` [rows, N] bf16; N a
+    multiple of 8, K of 16.  Up to 64 rows the weights are streamed past the rows, split evenly among the SMs
+    (``csrc/kernels/linear_int8_few.cu``); more rows go through the grouped GEMM as one group."""
+    _int8_weight(weight, scale, 2)
+    x = _int8_rows(x)
+    (M, K), N = x.shape, weight.shape[0]
+    if weight.shape[1] != K:
+        raise ValueError(f"rows of {K} do not fit weights {tuple(weight.shape)}")
+    dev = x.device
+    if weight.device != dev or scale.device != dev:
+        raise ValueError("all tensors must be on one GPU")
+    if out is None:
+        out = torch.empty(M, N, dtype=torch.bfloat16, device=dev)
+    elif out.shape != (M, N) or out.dtype != torch.bfloat16 or out.device != dev or not out.is_contiguous() or out.data_ptr() % 16:
+        raise ValueError(f"out must be a contiguous, 16-byte aligned bf16 tensor [{M}, {N}] on the same GPU")
+    if M == 0:
+        return out
+    lib = _native.cuda_lib()
+    with torch.cuda.device(dev):
+        st, ldx = _native.current_stream(dev.index), x.stride(0) if M > 1 else K
+        if M <= FEW_TOKENS:
+            ws = torch.empty(lib.rbv_linear_int8_few_workspace(M, N, K), dtype=torch.uint8, device=dev)     # of this call alone
+            rc = lib.rbv_linear_int8_few(_p(x), ldx, M, _p(weight), _p(scale), N, K, _p(out), _p(ws), _p(error), st)
+        else:
+            q = torch.empty(M, K, dtype=torch.int8, device=dev)
+            sc = torch.empty(M, dtype=torch.float32, device=dev)
+            rc = (lib.rbv_quantize_rows_int8(_p(x), M, None, K, ldx, _p(q), _p(sc), st)
+                  or lib.rbv_grouped_gemm_int8(_p(q), _p(sc), M, _p(weight), _p(scale), _p(out), None, None, 1, N, K, N, 0,
+                                               _p(error), 0, st))
+    if rc:
+        raise RuntimeError(f"int8 linear launch failed (CUDA error {rc})")
+    return out
+
+
 def pack_gate_up(gate: torch.Tensor, up: torch.Tensor) -> torch.Tensor:
     """Interleaves [G, I, H] gate and up weights into the [G, 2I, H] layout the SwiGLU epilogue expects."""
     G, I, H = gate.shape
@@ -352,8 +488,14 @@ class MoEExpertParallel:
         self.w13 = (torch.randn(self.El, 2 * inter, hidden, device=dev, generator=g) * init_std).to(bf)
         self.w2 = (torch.randn(self.El, hidden, inter, device=dev, generator=g) * init_std).to(bf)
         self.mx = fp8 == "mx"          # MXFP8: power-of-two scales per 32 elements, applied by the tensor core
+        self.int8 = fp8 == "int8"      # 8-bit integers: one scale per row and per output channel
         self.fp8 = bool(fp8)
-        if self.mx:
+        if self.int8:
+            if hidden % 16 or inter % 16:
+                raise ValueError("int8 experts need hidden and FFN sizes that are multiples of 16")
+            self.w13_q, self.w13_s = quantize_weight_int8(self.w13)
+            self.w2_q, self.w2_s = quantize_weight_int8(self.w2)
+        elif self.mx:
             self.w13_q, self.w13_s = quantize_weight_mxfp8(self.w13)
             self.w2_q, self.w2_s = quantize_weight_mxfp8(self.w2)
         elif self.fp8:   # expert weights as e4m3 with one scale per 128 x 128 block
@@ -371,7 +513,7 @@ class MoEExpertParallel:
             self.xq = comm.symm_empty((self.cap, hidden), torch.uint8)
             self.sfrow = comm.symm_empty((self.cap, hidden // 128), i32)
             self.xs = torch.full((hidden // 128, self.cap), 0x7f7f7f7f, dtype=i32, device=dev)   # atom order
-        elif self.P == 1 and self.fp8 and not self.mx:
+        elif self.P == 1 and self.fp8 and not self.mx and not self.int8:
             self.xrecv = None
             self.xq8 = torch.empty(self.cap, hidden, dtype=torch.uint8, device=dev)
             self.xs8 = torch.empty(hidden // 128, self.cap, dtype=torch.float32, device=dev)
@@ -481,6 +623,14 @@ class MoEExpertParallel:
             else:
                 grouped_gemm_mxfp8(hq, hs, self.w2_q, self.w2_s, self.group_start, self.group_rows, out=self.y,
                                    error=self.error[2:3])
+        elif self.int8:
+            # a row's scale is that of the whole row, so it is quantised when it is complete, right before each GEMM
+            xq, xs = quantize_rows_int8(self.xrecv, self.totals)
+            grouped_gemm_int8(xq, xs, self.w13_q, self.w13_s, self.group_start, self.group_rows, out=self.h, swiglu=True,
+                              error=self.error[1:2])
+            hq, hs = quantize_rows_int8(self.h, self.totals)
+            grouped_gemm_int8(hq, hs, self.w2_q, self.w2_s, self.group_start, self.group_rows, out=self.y,
+                              error=self.error[2:3])
         elif self.fp8:
             # activations are quantised row-wise (1 x 128 blocks), by the dispatch or right before each GEMM
             xq, xs = fp8_rows or quantize_rows_fp8(self.xrecv, self.totals)

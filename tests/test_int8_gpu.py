@@ -1,0 +1,258 @@
+"""GPU tests of the 8-bit integer products.
+
+The quantised values and scales are compared bit for bit with x / s in 32 bits.  The products' integer sums are exact, so
+against 64 bits a result is off by its rounding to bf16 (2^-8 of it) and three roundings in 32 bits (of the sum, and of two
+products; 2^-22 is allowed); with SwiGLU by what those do to gate and up (|silu'| <= 1.1) and 2^-20 for the exponential and
+the division."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+BF, I8, I32 = torch.bfloat16, torch.int8, torch.int32
+
+
+def _gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def _plain_rows(x):
+    f = x.float()
+    most = f.abs().amax(-1)
+    # (a division of tensors: torch divides by a Python number by multiplying with its rounded reciprocal, which is not max / 127)
+    s = torch.where(most > 0, most / torch.full_like(most, 127.0), torch.ones_like(most))
+    return torch.round(f / s[:, None]).clamp(-127, 127).to(I8), s
+
+
+def _rows(M, K, seed=0):
+    g = _gen(seed)
+    x = torch.randn(M, K, device="cuda", generator=g) * torch.exp(2 * torch.randn(M, 1, device="cuda", generator=g))
+    return x.to(BF)
+
+
+def _weight(shape, seed=1):
+    g = _gen(seed)
+    w = torch.randint(-127, 128, shape, device="cuda", generator=g, dtype=torch.int16).to(I8)
+    return w, (0.5 + torch.rand(shape[:-1], device="cuda", generator=g)) * 1e-3
+
+
+def _want(q, s, w, c, swiglu=False):
+    """(value, bound before the last rounding)"""
+    y = (q.double() @ w.double().t()) * s.double()[:, None] * c.double()
+    err = y.abs() * 2.0 ** -22
+    if swiglu:
+        gate, up = y[:, 0::2], y[:, 1::2]
+        err = 1.1 * up.abs() * err[:, 0::2] + gate.abs() * err[:, 1::2]
+        y = torch.nn.functional.silu(gate) * up
+        err = err + y.abs() * 2.0 ** -20
+    return y, err
+
+
+def _check(got, want):
+    y, err = want
+    assert got.shape == y.shape
+    bad = ~((got.double() - y).abs() <= (y.abs() + err) * 2.0 ** -8 + err + 1e-38)
+    assert not bad.any(), f"{int(bad.sum())} of {bad.numel()}, first {bad.nonzero()[0].tolist()}"
+
+
+@pytest.mark.parametrize("M,K", [(1, 16), (3, 256), (2, 272), (5, 4096), (700, 1408), (4, 8208), (3, 16384), (2, 20000), (1, 131072), (40000, 32)])
+def test_rows_bit_for_bit(M, K):
+    from rbruck_alltoallv_b200.ops.moe import quantize_rows_int8
+    x = _rows(M, K, seed=K)
+    q, s = quantize_rows_int8(x)
+    want, ws = _plain_rows(x)
+    assert torch.equal(s, ws) and torch.equal(q, want)
+
+
+def test_rows_next_to_halves():
+    """Values whose quotient is a half, or next to one: every bf16 in a binade against several maxima."""
+    from rbruck_alltoallv_b200.ops.moe import quantize_rows_int8
+    v = torch.arange(128, 256, device="cuda").float()
+    values = torch.cat([v * 2.0 ** -p for p in range(0, 14)])
+    values = torch.cat([values, -values, torch.zeros(64, device="cuda")])
+    top = torch.arange(128, 256, device="cuda").float() * 2.0
+    x = torch.cat([values.expand(128, -1), top[:, None].expand(128, 16)], dim=1).to(BF)
+    x = torch.minimum(torch.maximum(x, -x[:, -1:]), x[:, -1:]).contiguous()
+    q, s = quantize_rows_int8(x)
+    want, ws = _plain_rows(x)
+    assert torch.equal(s, ws) and torch.equal(q, want)
+
+
+def test_rows_strides_used_and_odd_rows():
+    from rbruck_alltoallv_b200.ops.moe import dequantize_int8, quantize_rows_int8
+    x = _rows(20, 64)
+    want, ws = _plain_rows(x)
+    for off in (0, 8, 3):
+        wide = torch.zeros(20, 100 + 4, dtype=BF, device="cuda")
+        wide[:, off:off + 64] = x
+        q, s = quantize_rows_int8(wide[:, off:off + 64])
+        assert torch.equal(q, want) and torch.equal(s, ws)
+    q, s = quantize_rows_int8(x.t().contiguous().t())
+    assert torch.equal(q, want) and torch.equal(s, ws)
+    q, s = quantize_rows_int8(x, torch.tensor([7], dtype=I32, device="cuda"))
+    assert torch.equal(q[:7], want[:7]) and torch.equal(s[:7], ws[:7])
+    x[0], x[1], x[2, 5], x[3, 6], x[4, 0] = 0, 2.0 ** -120, math.nan, math.inf, -math.inf
+    x[5] = torch.finfo(BF).max
+    q, s = quantize_rows_int8(x)
+    assert (q[:2] == 0).all() and (s[:2] == 1).all() and s[2:5].isnan().all() and (q[5] == 127).all() and s[5].isfinite()
+    assert torch.equal(q[6:], want[6:]) and dequantize_int8(q, s)[2:5].isnan().all()
+    q, s = quantize_rows_int8(x[:0])
+    assert q.shape == (0, 64) and s.shape == (0,)
+
+
+LINEAR = [(8, 16), (256, 4096), (1000, 2816), (4096, 512), (264, 14336), (72, 1040), (28672, 256), (16, 131072)]
+
+
+@pytest.mark.parametrize("M", [1, 2, 8, 9, 16, 17, 32, 33, 64, 65, 77, 300])
+@pytest.mark.parametrize("N,K", LINEAR)
+def test_linear(M, N, K):
+    from rbruck_alltoallv_b200.ops.moe import linear_int8
+    x, (w, c) = _rows(M, K, seed=M), _weight((N, K), seed=N)
+    err = torch.zeros(1, dtype=I32, device="cuda")
+    got = linear_int8(x, w, c, error=err)
+    assert err.item() == 0
+    _check(got, _want(*_plain_rows(x), w, c))
+
+
+def test_linear_extremes_are_exact():
+    """The largest sum of the largest depth, 131072 * 127 * 127, and its negative."""
+    from rbruck_alltoallv_b200.ops.moe import linear_int8
+    K = 131072
+    w = torch.full((16, K), 127, dtype=I8, device="cuda")
+    w[1] = -127
+    for M in (1, 70):
+        x = torch.ones(M, K, dtype=BF, device="cuda")
+        got = linear_int8(x, w, torch.ones(16, device="cuda"))
+        want = torch.full((M, 16), 127.0 * 127 * K * (1 / 127.0), device="cuda")
+        want[:, 1] *= -1
+        assert torch.equal(got, want.to(BF))
+
+
+def test_linear_strides_out_and_bad_rows():
+    from rbruck_alltoallv_b200.ops.moe import linear_int8
+    w, c = _weight((48, 96))
+    for M in (5, 80):
+        x = _rows(M, 96)
+        want = linear_int8(x, w, c)
+        wide = torch.zeros(M, 160, dtype=BF, device="cuda")
+        wide[:, 8:104] = x
+        out = torch.full((M + 2, 48), 7.0, dtype=BF, device="cuda")
+        assert torch.equal(linear_int8(wide[:, 8:104], w, c, out=out[1:M + 1]), want)
+        assert (out[0] == 7).all() and (out[M + 1] == 7).all() and torch.equal(out[1:M + 1], want)
+        wide[:, 3:99] = x
+        assert torch.equal(linear_int8(wide[:, 3:99], w, c), want)
+        assert torch.equal(linear_int8(x[:1].expand(M, 96), w, c), want[:1].expand(M, 48))
+        x[2, 7] = math.inf
+        got = linear_int8(x, w, c)
+        rest = [r for r in range(M) if r != 2]
+        assert got[2].isnan().all() and torch.equal(got[rest], want[rest])
+    assert linear_int8(x[:0], w, c).shape == (0, 48)
+
+
+@pytest.mark.parametrize("swiglu", [False, True])
+@pytest.mark.parametrize("rows,N,K", [([1], 256, 128), ([31, 32, 33], 512, 192), ([0, 255, 0, 256, 257], 264, 272), ([288, 1, 511], 1000, 16),
+                                      ([513, 1025], 256, 1040), ([5] * 64, 72, 400), ([0, 0, 3], 8, 4096), ([64, 64], 2048, 2816),
+                                      ([65, 2], 4096, 256)])
+def test_grouped(rows, N, K, swiglu):
+    from rbruck_alltoallv_b200.ops.moe import grouped_gemm_int8
+    G, M = len(rows), sum(rows)
+    q, s = _plain_rows(_rows(M + 3, K, seed=M))
+    w, c = _weight((G, N, K), seed=N)
+    if swiglu:
+        c = c * 0.05
+    start = [sum(rows[:g]) for g in range(G)]
+    gs, gr = (torch.tensor(v, dtype=I32, device="cuda") for v in (start, rows))
+    n_out = N // 2 if swiglu else N
+    wide = torch.full((M + 3, n_out + 6), 7.0, dtype=BF, device="cuda")
+    out = wide[:, 2:2 + n_out]
+    err = torch.zeros(1, dtype=I32, device="cuda")
+    grouped_gemm_int8(q, s, w, c, gs, gr, out=out, swiglu=swiglu, error=err)
+    assert err.item() == 0
+    assert (out[M:] == 7).all() and (wide[:, :2] == 7).all() and (wide[:, 2 + n_out:] == 7).all()
+    for g, (at, n) in enumerate(zip(start, rows)):
+        if n:
+            _check(out[at:at + n], _want(q[at:at + n], s[at:at + n], w[g], c[g], swiglu))
+
+
+def test_groups_beyond_the_rows_are_left_out():
+    from rbruck_alltoallv_b200.ops.moe import grouped_gemm_int8
+    q, s = _plain_rows(_rows(40, 64))
+    w, c = _weight((2, 64, 64))
+    gs, gr = torch.tensor([0, 30], dtype=I32, device="cuda"), torch.tensor([30, 50], dtype=I32, device="cuda")
+    err = torch.zeros(1, dtype=I32, device="cuda")
+    out = grouped_gemm_int8(q, s, w, c, gs, gr, error=err)
+    _check(out[30:], _want(q[30:], s[30:], w[1], c[1]))
+    assert err.item() == 6
+
+
+def test_streams_and_graphs():
+    from rbruck_alltoallv_b200.ops.moe import linear_int8
+    w, c = _weight((1024, 2048))
+    for M in (3, 100):
+        x, y = _rows(M, 2048, seed=1), _rows(M, 2048, seed=2)
+        want, want_y = linear_int8(x, w, c), linear_int8(y, w, c)
+        one, two = torch.cuda.Stream(), torch.cuda.Stream()
+        torch.cuda.synchronize()
+        got = []
+        for _ in range(20):
+            with torch.cuda.stream(one):
+                a = linear_int8(x, w, c)
+            with torch.cuda.stream(two):
+                b = linear_int8(y, w, c)
+            got.append((a, b))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, want) and torch.equal(b, want_y) for a, b in got)
+        g1, g2 = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g1):
+            a = linear_int8(x, w, c)
+        with torch.cuda.graph(g2):
+            b = linear_int8(y, w, c)
+        x.mul_(-3.0)
+        want = linear_int8(x, w, c)
+        torch.cuda.synchronize()
+        for _ in range(5):
+            with torch.cuda.stream(one):
+                g1.replay()
+            with torch.cuda.stream(two):
+                g2.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(a, want) and torch.equal(b, want_y)
+
+
+@pytest.mark.parametrize("T,H,I,E", [(64, 256, 512, 8), (33, 272, 1040, 4), (500, 512, 256, 16)])
+def test_layer_with_int8_experts(T, H, I, E):
+    """The layer against the same steps in 64 bits with the same quantisers: two roundings to bf16 (the FFN's intermediate, which
+    may move a quantised value by one step of 1/127 of the row's largest, and the expert's result) before the last one."""
+    from rbruck_alltoallv_b200.models.moe_layer import MoELayer
+    from rbruck_alltoallv_b200.parallel.comm import Communicator
+    comm = Communicator(nranks=1, heap_bytes=64 << 20, arena_bytes=1 << 20)
+    try:
+        layer = MoELayer(comm, E, H, I, T, seed=3, fp8="int8")
+        ep = layer.ep
+        x = torch.randn(T, H, device="cuda", generator=_gen(8)).to(BF)
+        logits = torch.randn(T, E, device="cuda", generator=_gen(9))
+        got = layer(x, logits)
+        ep.check()
+        p, which = torch.topk(torch.softmax(logits.double(), -1), 2, dim=-1)
+        p = p / p.sum(-1, keepdim=True)
+        want, bound = torch.zeros(T, H, dtype=torch.float64, device="cuda"), torch.zeros(T, H, dtype=torch.float64, device="cuda")
+        for e in range(E):
+            rows, k = (which == e).nonzero(as_tuple=True)
+            if not len(rows):
+                continue
+            q, s = _plain_rows(x[rows])
+            mid, _ = _want(q, s, ep.w13_q[e], ep.w13_s[e], True)
+            hq, hs = _plain_rows(mid.to(BF))
+            w2 = ep.w2_q[e].double()
+            y = (hq.double() @ w2.t()) * hs.double()[:, None] * ep.w2_s[e].double()
+            # every intermediate value off by one bf16 step at most (2^-7 of it) and so by that plus one quantisation step
+            step = mid.abs() * 2.0 ** -7 + hs.double()[:, None] * 1.01
+            off = ((step != 0) * step) @ w2.abs().t() * ep.w2_s[e].double()
+            want.index_add_(0, rows, p[rows, k, None] * y)
+            bound.index_add_(0, rows, p[rows, k, None] * (off + y.abs() * 2.0 ** -7))
+        assert ((got.double() - want).abs() <= bound + want.abs() * 2.0 ** -7).all()
+        # and far closer than that bound as a whole: hardly a value moves
+        assert (got.double() - want).norm() <= 0.02 * want.norm()
+    finally:
+        comm.close()

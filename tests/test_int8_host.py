@@ -1,0 +1,71 @@
+"""8-bit integer products without a GPU: what is refused, and the weight quantiser."""
+import pytest
+import torch
+
+from rbruck_alltoallv_b200.ops.moe import (dequantize_int8, grouped_gemm_int8, linear_int8, quantize_rows_int8,
+                                           quantize_weight_int8)
+
+BF, I8, I32 = torch.bfloat16, torch.int8, torch.int32
+
+
+def _linear(M=3, N=16, K=32):
+    return dict(x=torch.zeros(M, K, dtype=BF), weight=torch.zeros(N, K, dtype=I8), scale=torch.ones(N))
+
+
+@pytest.mark.parametrize("change,words", [
+    (dict(x=torch.zeros(3, 32)), "bf16 matrix"),
+    (dict(x=torch.zeros(32, dtype=BF)), "bf16 matrix"),
+    (_linear(K=24), "steps of 16"),
+    (_linear(K=131088), "131072"),
+    (_linear(N=12), "steps of 8"),
+    (dict(weight=torch.zeros(16, 32, dtype=torch.uint8)), "int8"),
+    (dict(scale=torch.ones(15)), "one fp32 scale per channel"),
+    (dict(scale=torch.ones(16, dtype=BF)), "one fp32 scale per channel"),
+    (dict(weight=torch.zeros(32, 16, dtype=I8).t()), "contiguous"),
+    (dict(weight=torch.zeros(16 * 32 + 1, dtype=I8)[1:].view(16, 32)), "16-byte aligned"),
+    (dict(), "on a GPU"),
+])
+def test_linear_refusals(change, words):
+    with pytest.raises(ValueError, match=words):
+        linear_int8(**{**_linear(), **change})
+
+
+def _grouped(M=5, G=2, N=16, K=32):
+    return dict(Aq=torch.zeros(M, K, dtype=I8), a_scale=torch.ones(M), Bq=torch.zeros(G, N, K, dtype=I8), b_scale=torch.ones(G, N),
+                group_start=torch.zeros(G, dtype=I32), group_rows=torch.zeros(G, dtype=I32))
+
+
+@pytest.mark.parametrize("change,words", [
+    (dict(Aq=torch.zeros(5, 16, dtype=I8)), "rows must be int8"),
+    (dict(Aq=torch.zeros(5, 32, dtype=torch.uint8)), "rows must be int8"),
+    (dict(a_scale=torch.ones(4)), "rows must be int8"),
+    (dict(Aq=torch.zeros(32, 5, dtype=I8).t()), "contiguous"),
+    (_grouped(N=20), "steps of 8"),
+    (_grouped(K=40), "steps of 16"),
+    (dict(group_rows=torch.zeros(2)), "int32"),
+    (dict(group_start=torch.zeros(3, dtype=I32)), "int32"),
+    (_grouped(G=65), "at most 64"),
+    (dict(), "on one GPU"),
+])
+def test_grouped_refusals(change, words):
+    with pytest.raises(ValueError, match=words):
+        grouped_gemm_int8(**{**_grouped(), **change})
+
+
+def test_rows_refusals():
+    with pytest.raises(ValueError, match="bf16 matrix"):
+        quantize_rows_int8(torch.zeros(2, 32, dtype=torch.float16))
+    with pytest.raises(ValueError, match="on a GPU"):
+        quantize_rows_int8(torch.zeros(2, 32, dtype=BF))
+
+
+def test_weight_quantiser():
+    """Half a step of the scale at most (the quotient and the product back, up to 127 steps, are rounded to 24 bits: 127 * 2^-23
+    of a step more), the largest value exactly at 127, zero channels with the scale 1."""
+    w = torch.randn(3, 8, 48, generator=torch.Generator().manual_seed(1)).to(BF)
+    w[1, 4] = 0
+    q, s = quantize_weight_int8(w)
+    assert q.dtype == I8 and q.shape == w.shape and s.shape == (3, 8) and s[1, 4] == 1 and (q[1, 4] == 0).all()
+    assert ((dequantize_int8(q, s) - w.float()).abs() <= s[..., None] * (0.5 + 127 * 2 ** -22)).all()
+    top = q.abs().amax(-1)
+    assert (top[s != 1] == 127).all()
