@@ -1,9 +1,10 @@
 """In-tree native builds.
 
-Two shared libraries are produced beside this file:
+Three shared libraries are produced beside this file:
 
 * ``librbv_host.so``  -- plan compiler + CPU executor (g++, no CUDA dependency),
-* ``librbv_cuda.so``  -- communicator, kernels and the C API (nvcc, sm_100a only).
+* ``librbv_cuda.so``  -- communicator, kernels and the C API (nvcc, sm_100a only),
+* ``_rbv_torch.so``    -- bindings of the operators on torch tensors, linked against ``librbv_cuda.so`` (g++).
 
 A library is rebuilt only when the hash of its sources and flags changes; the hash is kept in a
 ``.stamp`` file next to the library so that a tree copied to another machine is not rebuilt.
@@ -58,6 +59,9 @@ NVCC_FLAGS = [
     "-Xcompiler", "-Wall",
     "--expt-relaxed-constexpr",
 ]
+TORCH_MODULE = "_rbv_torch"
+TORCH_SOURCES = ["api/torch_ops.cpp"]
+
 GXX_FLAGS = ["-O2", "-std=c++17", "-fPIC", "-shared", "-Wall"]
 
 
@@ -153,9 +157,36 @@ def build_cuda(force: bool = False, verbose: bool = False, ptxas_verbose: bool =
     return lib
 
 
+def build_torch(force: bool = False, verbose: bool = False) -> Path:
+    """The bindings: one source against torch's headers, which takes most of a minute, and again only when it, the C headers or
+    torch have changed."""
+    import sysconfig
+
+    import torch
+
+    lib = PKG / (TORCH_MODULE + ".so")
+    srcs = [CSRC / s for s in TORCH_SOURCES]
+    root = Path(torch.__file__).resolve().parent
+    cuda = Path(_nvcc()).resolve().parent.parent
+    flags = ["-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", f"-DTORCH_EXTENSION_NAME={TORCH_MODULE}",
+             f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
+    digest = _hash(srcs + sorted(INCLUDE.rglob("*.h")), flags + [torch.__version__, sys.version])
+    if force or _needs_build(lib, digest):
+        includes = [root / "include", root / "include" / "torch" / "csrc" / "api" / "include", cuda / "include",
+                    sysconfig.get_paths()["include"]]
+        tmp = lib.with_suffix(f".tmp{os.getpid()}.so")
+        _run(["g++", *flags, f"-I{INCLUDE}", *[x for i in includes for x in ("-isystem", str(i))], *map(str, srcs), "-o", str(tmp),
+              f"-L{PKG}", "-l:librbv_cuda.so", "-Wl,-rpath,$ORIGIN", f"-L{root / 'lib'}", "-lc10", "-lc10_cuda", "-ltorch_cpu",
+              "-ltorch_python"], verbose)
+        os.replace(tmp, lib)
+        lib.with_suffix(".stamp").write_text(digest)
+    return lib
+
+
 def build_all(force: bool = False, verbose: bool = False) -> None:
     build_host(force, verbose)
     build_cuda(force, verbose)
+    build_torch(force, verbose)
 
 
 if __name__ == "__main__":

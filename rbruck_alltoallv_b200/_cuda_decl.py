@@ -81,9 +81,6 @@ def declare_cuda(lib):
     lib.rbv_ctx_set_eager.argtypes = [C.c_void_p, C.c_ulonglong]
     lib.rbv_ctx_set_cooperative.argtypes = [C.c_void_p, C.c_int]
     declare_moe(lib)
-    lib.rbv_block_norm.argtypes = [C.c_char_p, C.c_void_p]
-    lib.rbv_block_norm_backward.argtypes = [C.c_char_p, C.c_void_p]
-    lib.rbv_block_norm_parts.argtypes = [C.c_longlong, C.c_int, C.c_int]
     lib.rbv_reshard_heads.argtypes = [C.c_void_p, C.POINTER(C.c_void_p), C.POINTER(C.c_void_p), C.c_longlong,
                                       C.c_longlong, C.c_int, C.c_void_p]
     lib.rbv_alltoallv_noalloc.argtypes = [C.c_int, C.c_int, C.POINTER(C.c_void_p), C.POINTER(C.c_void_p), C.c_void_p,
@@ -117,14 +114,6 @@ def declare_moe(lib):
     lib.rbv_moe_route_local.argtypes = [vp, vp, i, i, i, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp]
     lib.rbv_moe_dispatch_local.argtypes = [vp, vp, i, i, vp, vp, vp, vp, vp, i, vp, vp, ll, vp, vp]
     lib.rbv_moe_combine_local.argtypes = [vp, vp, i, i, vp, vp, vp, vp]
-    lib.rbv_grouped_gemm_int8.argtypes = [vp, vp, ll, vp, vp, vp, vp, vp, i, i, i, i, i, vp, i, vp]
-    lib.rbv_quantize_rows_int8.argtypes = [vp, ll, vp, i, ll, vp, vp, vp]
-    lib.rbv_linear_int8_few_workspace.restype = ll
-    lib.rbv_linear_int8_few_workspace.argtypes = [i, i, i]
-    lib.rbv_linear_int8_few.argtypes = [vp, ll, i, vp, vp, i, i, vp, vp, vp, vp]
-    lib.rbv_moe_few_workspace.restype = ll
-    lib.rbv_moe_few_workspace.argtypes = [i] * 5
-    lib.rbv_moe_few_tokens.argtypes = [vp, ll, vp, ll, i, i, i, i, i, vp, vp, vp, vp, vp, vp]
     lib.rbv_moe_route.argtypes = [vp, i, i, vp, vp, vp, vp]
     lib.rbv_moe_layout.argtypes = [vp, i, i, i, vp, vp, vp, vp, vp, vp]
     lib.rbv_moe_layout_aligned.argtypes = [vp, i, i, i, vp, vp, vp, vp, vp, i, vp]

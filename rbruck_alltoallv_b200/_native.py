@@ -10,6 +10,7 @@ from . import _build
 _lock = threading.Lock()
 _host = None
 _cuda = None
+_torch_ops = None
 
 c_int_p = C.POINTER(C.c_int)
 c_ll_p = C.POINTER(C.c_longlong)
@@ -84,10 +85,27 @@ def cuda_lib():
         return _cuda
 
 
+def torch_ops():
+    """The bindings of the operators on torch tensors (``csrc/api/torch_ops.cpp``); their kernels are in the CUDA library."""
+    global _torch_ops
+    if _torch_ops is None:
+        import importlib.util
+        cuda_lib()                       # (built first where it is missing: the bindings are linked against it)
+        with _lock:
+            if _torch_ops is None:
+                path = _build.PKG / (_build.TORCH_MODULE + ".so")
+                if not path.exists() or os.environ.get("RBV_REBUILD"):
+                    path = _build.build_torch()
+                spec = importlib.util.spec_from_file_location(_build.TORCH_MODULE, path)
+                module = importlib.util.module_from_spec(spec)
+                spec.loader.exec_module(module)
+                _torch_ops = module
+    return _torch_ops
+
+
 def current_stream(device: int) -> int:
     """Handle of torch's current stream on a device.  (``torch.cuda.current_stream`` makes a Stream object for it first,
     which takes longer than many of the launches here.)"""
     import torch
     raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
     return raw(device) if raw is not None else torch.cuda.current_stream(device).cuda_stream
-

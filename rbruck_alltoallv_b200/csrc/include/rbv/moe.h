@@ -10,7 +10,7 @@
 #include "rbv/rbruckv.h"
 
 #ifdef __cplusplus
-namespace rbv { constexpr int kMoeMaxGroups = 64; constexpr int kMoeMaxExperts = 256; constexpr int kMoeFewMaxTopK = 8; }
+namespace rbv { constexpr int kMoeMaxGroups = 64; constexpr int kMoeMaxExperts = 256; }
 extern "C" {
 #endif
 
@@ -101,6 +101,9 @@ int rbv_quantize_rows_fp8(const void* x_bf16, long long rows, int K, int ldx, vo
 int rbv_quantize_used_rows_fp8(const void* x_bf16, long long rows, const int* used, int K, int ldx, void* out_fp8,
                                float* scale_t, void* cuda_stream);
 
+/* Rows that the kernels for few rows take at most, and experts per token of the layer for few tokens. */
+#define RBV_FEW_ROWS 64
+#define RBV_FEW_MAX_TOP_K 8
 /* A whole layer for a few tokens (1 <= T <= 64) with every expert on this GPU, in two kernels: choice of the top_k (<= 8)
  * largest of E (<= 256) logits per token (ties: lower expert; -inf is never chosen, a token without any other logit gets a
  * row of zeros; a NaN counts as largest and makes the token's row NaN), softmax over the chosen ones, SwiGLU FFN, weighted sum.

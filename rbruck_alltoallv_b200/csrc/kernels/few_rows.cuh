@@ -21,12 +21,14 @@
 // One bulk copy per weight row and chunk in place of the boxes reached a quarter of the bandwidth: 401 us against 125 for one
 // token of a layer that reads 704 MB.
 #pragma once
+#include <atomic>
 #include <cstdint>
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
 #include "kernels/sm100_ptx.cuh"
+#include "rbv/moe.h"
 
 namespace rbv {
 namespace few {
@@ -35,7 +37,7 @@ constexpr int kChunk = 512;               // bytes of a row per stage
 constexpr int kCols = 4;                  // columns of 128 bytes in it
 constexpr int kWarps = 8;                 // consumer warps: kCols x 2
 constexpr int kThreads = (kWarps + 2) * 32;         // and two producers, one for the weights and one for the rows of A
-constexpr int kMaxRows = 64;              // rows of A
+constexpr int kMaxRows = RBV_FEW_ROWS;    // rows of A
 constexpr int kMaxTile = 64;              // weight rows of a piece
 constexpr int kMaxStages = 32;
 
@@ -43,6 +45,7 @@ constexpr int kMaxStages = 32;
 // `one` of a single column.
 struct WeightMaps {
   CUtensorMap all[4], one[4];
+  int heights;                             // 8, 16, 32, 64 in the bits of a mask: the boxes there are
   int whole;                               // chunks that `all` covers; the rest of a row that does not end with a column: `one`
 };
 
@@ -169,6 +172,11 @@ __device__ __forceinline__ bool feed(const WeightMaps& maps, Cursor& cur, uint32
     cur.next();
   }
   return true;
+}
+
+__device__ __forceinline__ void prefetch_maps(const WeightMaps& maps) {      // a warp
+  const int lane = threadIdx.x & 31;
+  if (lane < 4 && maps.whole && (maps.heights & (8 << lane))) sm100::tma_prefetch_desc(&maps.all[lane]);
 }
 
 // Where in a stage of `rows` weight rows the 8 rows of group g are, column j.
@@ -342,11 +350,31 @@ inline int ring_stages(int tile, int rows, size_t fixed) {
   const size_t room = 227 * 1024 - 1024 /*alignment*/ - fixed - kRedBytes, n = room / slot_bytes(tile, rows);
   return n > (size_t)kMaxStages ? kMaxStages : (int)n;
 }
+// Once per kernel and device: as much dynamic shared memory as there is beside `fixed` bytes.  (A call on one token takes less
+// time on the GPU than a handful of runtime calls.)
+template <auto* Kernel>
+inline cudaError_t allow_smem_once(size_t fixed) {
+  static std::atomic<unsigned long long> done{0};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess || (dev < 64 && (done.load(std::memory_order_relaxed) >> dev & 1))) return e;
+  e = cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(227 * 1024 - fixed));
+  if (e == cudaSuccess && dev < 64) done.fetch_or(1ull << dev, std::memory_order_relaxed);
+  return e;
+}
 inline size_t ring_smem(int tile, int rows, int stages) { return 1024 + kRedBytes + (size_t)slot_bytes(tile, rows) * stages; }
 
-// Weights of `rows` rows of row_bytes (a multiple of 16) each, elements of `size` bytes; 128-byte swizzle.
+// Boxes for pieces of at most `rows` rows, all multiples of 8 among them.
+inline int heights_up_to(int rows) {
+  int all = 0;
+  for (int h = 8; h <= rows; h *= 2) all |= h;
+  return all;
+}
+
+// Weights of `rows` rows of row_bytes (a multiple of 16) each, elements of `size` bytes; 128-byte swizzle.  Bits 3 to 6 of
+// `heights`: the boxes that pieces are made of (a map takes a third of a microsecond to make).
 inline bool weight_maps(WeightMaps* m, const void* base, unsigned long long rows, unsigned long long row_bytes, CUtensorMapDataType type,
-                        int size) {
+                        int size, int heights) {
   typedef CUresult (*Encode)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
                              const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
   static const Encode encode = [] {
@@ -357,6 +385,7 @@ inline bool weight_maps(WeightMaps* m, const void* base, unsigned long long rows
   }();
   if (!encode) return false;
   const unsigned per_col = 128u / (unsigned)size;
+  m->heights = heights;
   const cuuint64_t cols = row_bytes / 128;                 // whole columns
   const bool even = row_bytes % 128 == 0;
   m->whole = (int)(even ? (cols + kCols - 1) / kCols : cols / kCols);      // (columns behind the last one read as zeros)
@@ -364,6 +393,7 @@ inline bool weight_maps(WeightMaps* m, const void* base, unsigned long long rows
   const cuuint64_t dims2[2] = {row_bytes / size, rows}, strides2[1] = {row_bytes};
   const cuuint32_t ones[3] = {1, 1, 1};
   for (int b = 0; b < 4; b++) {
+    if (!(heights & (8 << b))) continue;
     const cuuint32_t box3[3] = {per_col, 8u << b, (cuuint32_t)kCols}, box2[2] = {per_col, 8u << b};
     if (m->whole > 0 && encode(&m->all[b], type, 3, const_cast<void*>(base), dims3, strides3, box3, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
                                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)

@@ -73,7 +73,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_int8_few_kernel(const __gr
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(dyn) + 1023) & ~uintptr_t(1023));
   uint4* red = reinterpret_cast<uint4*>(base);
   if (tid == 0) ring_init(ring, a.stages, 2);
-  if (warp >= kWarps && lane < 4 && maps.whole) sm100::tma_prefetch_desc(warp == kWarps ? &maps.all[lane] : &q_maps.all[lane]);
+  if (warp >= kWarps) prefetch_maps(warp == kWarps ? maps : q_maps);
   pdl_trigger();
   __syncthreads();
   LinearWalk walk(a);
@@ -201,15 +201,15 @@ template <int MAX>
 cudaError_t linear_launch(const LinearArgs& args, const int8_t* q, const void* w, const LinearPlan& p, cudaStream_t st) {
   LinearArgs a = args;
   WeightMaps maps, q_maps;
-  if (!weight_maps(&maps, w, (unsigned long long)a.N, (unsigned long long)a.K, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1) ||
-      !weight_maps(&q_maps, q, (unsigned long long)a.M, (unsigned long long)a.K, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1))
+  if (!weight_maps(&maps, w, (unsigned long long)a.N, (unsigned long long)a.K, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p.tile | a.N % p.tile) ||
+      !weight_maps(&q_maps, q, (unsigned long long)a.M, (unsigned long long)a.K, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, box_rows(a.M)))
     return cudaErrorUnknown;
   a.tile = p.tile;
   a.whole = p.whole;
   a.box = box_rows(a.M);
   a.stages = ring_stages(a.tile, a.box, sizeof(Ring) + 64);
   const size_t smem = ring_smem(a.tile, a.box, a.stages);
-  const cudaError_t e = cudaFuncSetAttribute(linear_int8_few_kernel<MAX>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  const cudaError_t e = allow_smem_once<linear_int8_few_kernel<MAX>>(sizeof(Ring) + 64);
   return e != cudaSuccess ? e : launch_dependent(linear_int8_few_kernel<MAX>, dim3(p.sms), dim3(kThreads), smem, st, maps, q_maps, a);
 }
 

@@ -46,7 +46,7 @@ struct FewArgs {
 // The choice, as every CTA makes it.
 template <int TOKENS>
 struct Choice {
-  static constexpr int kMaxSlots = TOKENS * kMoeFewMaxTopK;
+  static constexpr int kMaxSlots = TOKENS * RBV_FEW_MAX_TOP_K;
   short expert[kMaxSlots];                // of slot t * top_k + j; negative: none
   float weight[kMaxSlots];
   short at[kMaxSlots];                    // row of the slot among its expert's rows
@@ -253,7 +253,7 @@ __global__ void __launch_bounds__(kThreads, 1) moe_few_up_kernel(const __grid_co
   uint8_t* base = aligned_smem(dyn);
   uint4* red = reinterpret_cast<uint4*>(base);
   if (threadIdx.x == 0) ring_init(s.ring, a.stages, 1);
-  if (warp == kWarps && lane < 4 && maps.whole) sm100::tma_prefetch_desc(&maps.all[lane]);
+  if (warp == kWarps) prefetch_maps(maps);
   pdl_wait();
   pdl_trigger();      // after the wait: the down kernel reads the logits before it waits for this one
   if (blockIdx.x == 0)
@@ -324,7 +324,7 @@ __global__ void __launch_bounds__(kThreads, 1) moe_few_down_kernel(const __grid_
   uint8_t* base = aligned_smem(dyn);
   uint4* red = reinterpret_cast<uint4*>(base);
   if (tid == 0) ring_init(s.ring, a.stages, 2);
-  if (warp >= kWarps && lane < 4 && maps.whole) sm100::tma_prefetch_desc(warp == kWarps ? &maps.all[lane] : &h_maps.all[lane]);
+  if (warp >= kWarps) prefetch_maps(warp == kWarps ? maps : h_maps);
   pdl_trigger();
   choose(s.choice, a);
   const int n_used = s.choice.n_used;
@@ -459,7 +459,7 @@ struct FewPlan { int sms, up_tile, down_tile, whole; size_t h_bytes, partial_byt
 size_t round_up(size_t v, size_t to) { return (v + to - 1) / to * to; }
 
 bool few_plan(int T, int H, int I, int E, int top_k, FewPlan* p) {
-  if (T < 1 || T > kMaxRows || E < 1 || E > kMoeMaxExperts || top_k < 1 || top_k > kMoeFewMaxTopK || top_k > E) return false;
+  if (T < 1 || T > kMaxRows || E < 1 || E > kMoeMaxExperts || top_k < 1 || top_k > RBV_FEW_MAX_TOP_K || top_k > E) return false;
   if (H < 8 || I < 8 || H % 8 || I % 8 || 2ll * E * I > 0x7fffffffll || (long long)E * H > 0x7fffffffll) return false;
   if (H > (1 << 24) || I > (1 << 24)) return false;      // (row lengths in bytes, and coordinates a box beyond them, fit an int)
   int dev = 0;
@@ -473,24 +473,26 @@ bool few_plan(int T, int H, int I, int E, int top_k, FewPlan* p) {
   return true;
 }
 
+template <int MAX, auto* Kernel, typename... Maps>
+cudaError_t launch_ring(FewArgs a, int tile, int box, int sms, cudaStream_t st, const Maps&... maps) {
+  a.tile = tile;
+  a.box = box;
+  a.stages = ring_stages(tile, box, sizeof(Shared<MAX>));
+  const cudaError_t e = allow_smem_once<Kernel>(sizeof(Shared<MAX>));
+  return e != cudaSuccess ? e : launch_dependent(Kernel, dim3(sms), dim3(kThreads), ring_smem(tile, box, a.stages), st, maps..., a);
+}
+
 template <int MAX>
 cudaError_t few_launch(FewArgs a, const FewPlan& p, cudaStream_t st) {
   const CUtensorMapDataType bf16 = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   WeightMaps w13, w2, h;
-  if (!weight_maps(&w13, a.w13, 2ull * a.E * a.I, 2ull * a.H, bf16, 2) || !weight_maps(&w2, a.w2, (unsigned long long)a.E * a.H, 2ull * a.I, bf16, 2) ||
-      !weight_maps(&h, a.h, (unsigned long long)a.T * a.top_k, 2ull * a.I, bf16, 2))
+  if (!weight_maps(&w13, a.w13, 2ull * a.E * a.I, 2ull * a.H, bf16, 2, heights_up_to(p.up_tile)) ||
+      !weight_maps(&w2, a.w2, (unsigned long long)a.E * a.H, 2ull * a.I, bf16, 2, p.down_tile | a.H % p.down_tile) ||
+      !weight_maps(&h, a.h, (unsigned long long)a.T * a.top_k, 2ull * a.I, bf16, 2, heights_up_to(box_rows(a.T))))
     return cudaErrorUnknown;
-  auto launch = [&](auto kernel, int tile, int box, const auto&... maps) {
-    a.tile = tile;
-    a.box = box;
-    a.whole = p.whole;
-    a.stages = ring_stages(tile, box, sizeof(Shared<MAX>));
-    const size_t smem = ring_smem(tile, box, a.stages);
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    return e != cudaSuccess ? e : launch_dependent(kernel, dim3(p.sms), dim3(kThreads), smem, st, maps..., a);
-  };
-  const cudaError_t e = launch(moe_few_up_kernel<MAX>, p.up_tile, 0, w13);
-  return e != cudaSuccess ? e : launch(moe_few_down_kernel<MAX>, p.down_tile, box_rows(a.T), w2, h);
+  a.whole = p.whole;
+  const cudaError_t e = launch_ring<MAX, moe_few_up_kernel<MAX>>(a, p.up_tile, 0, p.sms, st, w13);
+  return e != cudaSuccess ? e : launch_ring<MAX, moe_few_down_kernel<MAX>>(a, p.down_tile, box_rows(a.T), p.sms, st, w2, h);
 }
 
 }  // namespace

@@ -270,36 +270,12 @@ def grouped_gemm_mxfp8_swiglu_q(Aq: torch.Tensor, sfa: torch.Tensor, Bq: torch.T
 INT8_MAX_DEPTH = 131072          # K at which 127 * 127 * K still fits a 32-bit integer
 
 
-def _int8_rows(x: torch.Tensor):
-    """``x`` [rows, K] bf16 as the kernels read it: packed rows that start at 16-byte boundaries."""
-    if x.dtype != torch.bfloat16 or x.dim() != 2:
-        raise ValueError(f"rows must be a bf16 matrix, not {tuple(x.shape)} in {x.dtype}")
-    if x.shape[1] < 16 or x.shape[1] % 16 or x.shape[1] > INT8_MAX_DEPTH:
-        raise ValueError(f"depths of 16 to {INT8_MAX_DEPTH} in steps of 16 are supported, not {x.shape[1]}")
-    if not x.is_cuda:
-        raise ValueError("the rows must be on a GPU")
-    if x.stride(1) != 1 or x.data_ptr() % 16 or (x.shape[0] > 1 and (x.stride(0) % 8 or x.stride(0) < x.shape[1])):
-        x = x.clone(memory_format=torch.contiguous_format)
-    return x
-
-
 def quantize_rows_int8(x: torch.Tensor, used: Optional[torch.Tensor] = None):
     """bf16 [rows, K] -> (int8 [rows, K], fp32 scales [rows]): ``scale = max|row| / 127``, values rounded to nearest even.  With
     ``used`` (int32 CUDA tensor) only the first ``used[0]`` rows are quantised, the others are left undefined.  A row with an
     infinity or a NaN gets the scale NaN (so that what is made of it is NaN), one whose values are all below 2^-100 becomes
     zeros with the scale 1.  Rows may be strided; K is a multiple of 16."""
-    x = _int8_rows(x)
-    rows, K = x.shape
-    q = torch.empty(rows, K, dtype=torch.int8, device=x.device)
-    sc = torch.empty(rows, dtype=torch.float32, device=x.device)
-    if rows == 0:
-        return q, sc
-    with torch.cuda.device(x.device):
-        rc = _native.cuda_lib().rbv_quantize_rows_int8(_p(x), rows, _p(used), K, x.stride(0) if rows > 1 else K, _p(q), _p(sc),
-                                                       _native.current_stream(x.device.index))
-    if rc:
-        raise RuntimeError(f"int8 quantisation launch failed (CUDA error {rc})")
-    return q, sc
+    return _native.torch_ops().quantize_rows_int8(x, used)
 
 
 def quantize_weight_int8(w: torch.Tensor):
@@ -316,17 +292,6 @@ def dequantize_int8(q: torch.Tensor, scale: torch.Tensor) -> torch.Tensor:
     return q.float() * scale[..., None]
 
 
-def _int8_weight(w: torch.Tensor, scale: torch.Tensor, dim: int):
-    if w.dim() != dim or w.dtype != torch.int8 or scale.dtype != torch.float32 or scale.shape != w.shape[:-1]:
-        raise ValueError(f"weights must be int8 with {dim} dimensions and one fp32 scale per channel, not {tuple(w.shape)} in "
-                         f"{w.dtype} with scales {tuple(scale.shape)} in {scale.dtype}")
-    N, K = w.shape[-2:]
-    if N < 8 or N % 8 or K < 16 or K % 16 or K > INT8_MAX_DEPTH:
-        raise ValueError(f"channels in steps of 8 and depths of 16 to {INT8_MAX_DEPTH} in steps of 16 are supported, not {N} x {K}")
-    if not w.is_contiguous() or not scale.is_contiguous() or w.data_ptr() % 16 or scale.data_ptr() % 16:
-        raise ValueError("weights and scales must be contiguous and 16-byte aligned")
-
-
 def grouped_gemm_int8(Aq: torch.Tensor, a_scale: torch.Tensor, Bq: torch.Tensor, b_scale: torch.Tensor,
                       group_start: torch.Tensor, group_rows: torch.Tensor, out: Optional[torch.Tensor] = None,
                       swiglu: bool = False, error: Optional[torch.Tensor] = None, max_ctas: int = 0) -> torch.Tensor:
@@ -336,31 +301,7 @@ def grouped_gemm_int8(Aq: torch.Tensor, a_scale: torch.Tensor, Bq: torch.Tensor,
     ``Aq`` [M, K] int8 with ``a_scale`` [M], ``Bq`` [G, N, K] int8 with ``b_scale`` [G, N], ``group_start`` / ``group_rows`` int32
     CUDA tensors [G], G <= 64; N a multiple of 8, K of 16.  With ``swiglu`` the rows of ``Bq[g]`` interleave gate and up projections
     and ``out`` is [M, N // 2].  Rows of ``out`` outside the groups are left as they are."""
-    _int8_weight(Bq, b_scale, 3)
-    G, N, K = Bq.shape
-    if Aq.dim() != 2 or Aq.dtype != torch.int8 or Aq.shape[1] != K or a_scale.shape != Aq.shape[:1] or a_scale.dtype != torch.float32:
-        raise ValueError(f"rows must be int8 [M, {K}] with fp32 scales [M], not {tuple(Aq.shape)} in {Aq.dtype} with {tuple(a_scale.shape)}")
-    if not Aq.is_contiguous() or not a_scale.is_contiguous() or Aq.data_ptr() % 16:
-        raise ValueError("rows and scales must be contiguous and 16-byte aligned")
-    if not 1 <= G <= 64 or any(t.shape != (G,) or t.dtype != torch.int32 or not t.is_contiguous() for t in (group_start, group_rows)):
-        raise ValueError(f"group_start and group_rows must be int32 [{G}], with at most 64 groups")
-    M, n_out = Aq.shape[0], N // 2 if swiglu else N
-    if not Aq.is_cuda or any(t.device != Aq.device for t in (a_scale, Bq, b_scale, group_start, group_rows)):
-        raise ValueError("all tensors must be on one GPU")
-    if out is None:
-        out = torch.empty(M, n_out, dtype=torch.bfloat16, device=Aq.device)
-    elif (out.shape != (M, n_out) or out.dtype != torch.bfloat16 or out.device != Aq.device or out.stride(1) != 1 or out.stride(0) % 2
-          or out.data_ptr() % 4 or (M > 1 and out.stride(0) < n_out)):
-        raise ValueError(f"out must be a bf16 tensor [{M}, {n_out}] with packed, 4-byte aligned rows on the same GPU")
-    if M == 0:
-        return out
-    with torch.cuda.device(Aq.device):
-        rc = _native.cuda_lib().rbv_grouped_gemm_int8(_p(Aq), _p(a_scale), M, _p(Bq), _p(b_scale), _p(out), _p(group_start),
-                                                      _p(group_rows), G, N, K, out.stride(0) if M > 1 else n_out, 1 if swiglu else 0,
-                                                      _p(error), int(max_ctas), _native.current_stream(Aq.device.index))
-    if rc:
-        raise RuntimeError(f"int8 grouped GEMM launch failed (CUDA error {rc})")
-    return out
+    return _native.torch_ops().grouped_gemm_int8(Aq, a_scale, Bq, b_scale, group_start, group_rows, out, swiglu, error, max_ctas)
 
 
 def linear_int8(x: torch.Tensor, weight: torch.Tensor, scale: torch.Tensor, out: Optional[torch.Tensor] = None,
@@ -371,35 +312,7 @@ def linear_int8(x: torch.Tensor, weight: torch.Tensor, scale: torch.Tensor, out:
     ``x`` [rows, K] bf16, ``weight`` [N, K] int8 and ``scale`` [N] fp32 (:func:`quantize_weight_int8`), ``out`` [rows, N] bf16; N a
     multiple of 8, K of 16.  Up to 64 rows the weights are streamed past the rows, split evenly among the SMs
     (``csrc/kernels/linear_int8_few.cu``); more rows go through the grouped GEMM as one group."""
-    _int8_weight(weight, scale, 2)
-    x = _int8_rows(x)
-    (M, K), N = x.shape, weight.shape[0]
-    if weight.shape[1] != K:
-        raise ValueError(f"rows of {K} do not fit weights {tuple(weight.shape)}")
-    dev = x.device
-    if weight.device != dev or scale.device != dev:
-        raise ValueError("all tensors must be on one GPU")
-    if out is None:
-        out = torch.empty(M, N, dtype=torch.bfloat16, device=dev)
-    elif out.shape != (M, N) or out.dtype != torch.bfloat16 or out.device != dev or not out.is_contiguous() or out.data_ptr() % 16:
-        raise ValueError(f"out must be a contiguous, 16-byte aligned bf16 tensor [{M}, {N}] on the same GPU")
-    if M == 0:
-        return out
-    lib = _native.cuda_lib()
-    with torch.cuda.device(dev):
-        st, ldx = _native.current_stream(dev.index), x.stride(0) if M > 1 else K
-        if M <= FEW_TOKENS:
-            ws = torch.empty(lib.rbv_linear_int8_few_workspace(M, N, K), dtype=torch.uint8, device=dev)     # of this call alone
-            rc = lib.rbv_linear_int8_few(_p(x), ldx, M, _p(weight), _p(scale), N, K, _p(out), _p(ws), _p(error), st)
-        else:
-            q = torch.empty(M, K, dtype=torch.int8, device=dev)
-            sc = torch.empty(M, dtype=torch.float32, device=dev)
-            rc = (lib.rbv_quantize_rows_int8(_p(x), M, None, K, ldx, _p(q), _p(sc), st)
-                  or lib.rbv_grouped_gemm_int8(_p(q), _p(sc), M, _p(weight), _p(scale), _p(out), None, None, 1, N, K, N, 0,
-                                               _p(error), 0, st))
-    if rc:
-        raise RuntimeError(f"int8 linear launch failed (CUDA error {rc})")
-    return out
+    return _native.torch_ops().linear_int8(x, weight, scale, out, error)
 
 
 def pack_gate_up(gate: torch.Tensor, up: torch.Tensor) -> torch.Tensor:
@@ -424,47 +337,7 @@ def moe_few_tokens(x: torch.Tensor, logits: torch.Tensor, w13: torch.Tensor, w2:
     ``top_k`` is spread over those, and one without any other gets a row of zeros (a padded slot of a batch).  A NaN among a
     token's logits makes its row NaN.  The number of tokens may change from call to call; weights are read for the experts that
     some token chooses, once each.  ``error`` (int32 CUDA tensor): set to non-zero if a bounded wait ran out."""
-    if x.dim() != 2 or logits.dim() != 2 or w13.dim() != 3 or w2.dim() != 3:
-        raise ValueError("x [T, H], logits [T, E], w13 [E, 2 I, H] and w2 [E, H, I] are wanted")
-    T, H = x.shape
-    E, _, I = w2.shape
-    if x.dtype != torch.bfloat16 or w13.dtype != torch.bfloat16 or w2.dtype != torch.bfloat16 or logits.dtype != torch.float32:
-        raise ValueError("x and the weights must be bf16, the logits fp32")
-    if logits.shape != (T, E) or w13.shape != (E, 2 * I, H) or w2.shape[1] != H:
-        raise ValueError(f"shapes do not fit: x {tuple(x.shape)}, logits {tuple(logits.shape)}, w13 {tuple(w13.shape)}, "
-                         f"w2 {tuple(w2.shape)}")
-    if T > FEW_TOKENS:
-        raise ValueError(f"{T} tokens: moe_few_tokens takes at most {FEW_TOKENS}; MoEExpertParallel.forward is for more")
-    if H < 8 or I < 8 or H % 8 or I % 8 or not 1 <= E <= 256 or not 1 <= top_k <= min(FEW_MAX_TOP_K, E):
-        raise ValueError(f"hidden {H} and FFN width {I} must be multiples of 8, experts {E} at most 256, top_k {top_k} at most "
-                         f"{FEW_MAX_TOP_K} and the experts")
-    if not (w13.is_contiguous() and w2.is_contiguous()) or (w13.data_ptr() | w2.data_ptr()) % 16:
-        raise ValueError("the weights must be contiguous and 16-byte aligned")
-    if not x.is_cuda or any(t.device != x.device for t in (logits, w13, w2)):
-        raise ValueError("all tensors must be on one GPU")
-    if out is None:
-        out = torch.empty(T, H, dtype=torch.bfloat16, device=x.device)
-    elif out.shape != (T, H) or out.dtype != torch.bfloat16 or not out.is_contiguous() or out.device != x.device or out.data_ptr() % 16:
-        raise ValueError("out must be a contiguous, 16-byte aligned bf16 tensor [T, H] on the same GPU")
-    if T == 0:
-        return out
-    if x.stride(1) != 1 or x.data_ptr() % 16 or (T > 1 and (x.stride(0) % 8 or x.stride(0) < H)):
-        x = x.clone(memory_format=torch.contiguous_format)
-    if (logits.stride(1) != 1 and E > 1) or (T > 1 and logits.stride(0) < E):
-        logits = logits.contiguous()
-    index = x.device.index
-    if torch.cuda.current_device() != index:
-        with torch.cuda.device(index):
-            return moe_few_tokens(x, logits, w13, w2, top_k, out, error)
-    lib = _native.cuda_lib()
-    # the workspace belongs to this call alone: calls on other streams and captured ones have their own
-    ws = torch.empty(lib.rbv_moe_few_workspace(T, H, I, E, top_k), dtype=torch.uint8, device=x.device)
-    rc = lib.rbv_moe_few_tokens(x.data_ptr(), x.stride(0) if T > 1 else H, logits.data_ptr(), logits.stride(0) if T > 1 else E, T, H,
-                                I, E, top_k, w13.data_ptr(), w2.data_ptr(), out.data_ptr(), ws.data_ptr(), _p(error),
-                                _native.current_stream(index))
-    if rc:
-        raise RuntimeError(f"few-token MoE launch failed (CUDA error {rc})")
-    return out
+    return _native.torch_ops().moe_few_tokens(x, logits, w13, w2, top_k, out, error)
 
 
 class MoEExpertParallel:

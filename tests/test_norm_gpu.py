@@ -215,3 +215,29 @@ def test_streams_and_graphs():
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(captured, fresh)) and all(torch.equal(a, b) for a, b in zip(second, fresh))
     assert not torch.equal(want[0], fresh[0])
+
+
+def test_some_gradients_and_no_second_ones():
+    """Gradients only for what asks for them; accumulated by backward(); a graph of the backward pass is refused when it is used."""
+    from rbruck_alltoallv_b200.ops.norm import block_norm
+    v, dr2, du = _make(30, 72, BF, F32, F32, "channel", seed=4)
+    r, z, w1, g, w2 = _double(v)
+    want = norm_oracle.backward(r, z, w1, g, 0.5, w2, 1e-6, dr2.double(), du.double())
+    for asked in (["gate"], ["branch"], ["residual", "pre_weight"], ["post_weight", "branch"], []):
+        leaves = {n: t.detach().clone().requires_grad_(n in asked) for n, t in v.items()}
+        out = block_norm(leaves["residual"], leaves["branch"], leaves["post_weight"], leaves["gate"], 0.5, leaves["pre_weight"])
+        assert all(o.requires_grad == bool(asked) for o in out)
+        if asked:
+            torch.autograd.backward(out, (dr2, du))
+        for n, t in leaves.items():
+            assert (t.grad is not None) == (n in asked)
+            if n in asked:
+                _close(n, t.grad, want[n])
+    x = v["branch"].detach().clone().requires_grad_()
+    out = block_norm(v["residual"], x, v["post_weight"], v["gate"], 0.5, v["pre_weight"])
+    (first,) = torch.autograd.grad(out, x, (dr2, du), create_graph=True)
+    _close("branch", first.detach(), want["branch"])
+    with pytest.raises(RuntimeError):                 # (autograd itself finds that nothing leads from there to x)
+        torch.autograd.grad(first.float().sum(), x)
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        first.float().sum().backward()
