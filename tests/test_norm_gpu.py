@@ -241,3 +241,13 @@ def test_some_gradients_and_no_second_ones():
         torch.autograd.grad(first.float().sum(), x)
     with pytest.raises(RuntimeError, match="differentiable once"):
         first.float().sum().backward()
+
+
+@pytest.mark.parametrize("T", [149, 150, 152, 300, 1189])
+@pytest.mark.parametrize("H", [1024, 1032, 2048, 4096, 6144, 8200, 16384])
+@pytest.mark.parametrize("kind,res,gate", [(BF, BF, "channel"), (BF, F32, "full"), (F32, F32, "token"), (HF, HF, "none")])
+def test_several_rows_per_cta(T, H, kind, res, gate):
+    """More rows than SMs, of 2 KB and more: the kernels with several rows in work, at the ends of their shapes."""
+    if H > 8192 and T > 160:
+        T = 160
+    _check(*_make(T, H, kind, res, F32, gate, seed=T + H))
