@@ -47,7 +47,7 @@ constexpr int I_TMEM_COLS = 512;
 constexpr size_t I_SMEM = (size_t)ISTAGES_SMALL * ISTAGE_BYTES_SMALL + 1024 /*alignment slack*/;
 static_assert(ISTAGES * ISTAGE_BYTES <= ISTAGES_SMALL * ISTAGE_BYTES_SMALL, "shared memory");
 
-// Token boxes of 16, 32, 64 and 128 rows: a CTA's half of a tile is fetched with the smallest that covers it.
+// Token boxes of 16, 32, 64 and 128 rows: a CTA's half of a tile (a multiple of 16 rows) is put together from them.
 struct I8Maps { CUtensorMap w, tok[4]; };
 
 struct I8Params {
@@ -87,10 +87,6 @@ struct I8Walk {
     return r;
   }
 };
-
-// Index of the token box for `half` rows, and its rows.
-__device__ __forceinline__ int i8_box(int half) { return half <= 16 ? 0 : half <= 32 ? 1 : half <= 64 ? 2 : 3; }
-__device__ __forceinline__ uint32_t i8_box_bytes(int half) { return (16u << i8_box(half)) * IK; }
 
 }  // namespace
 
@@ -149,8 +145,7 @@ grouped_gemm_int8_kernel(const __grid_constant__ I8Maps maps, const __grid_const
         const I8Tile tl = walk.at(p, t, s_rows, s_start);
         if (!tl.valid) break;
         const int half = tl.nt / 2;
-        const CUtensorMap* tok = &maps.tok[i8_box(half)];
-        const uint32_t bytes = 2u * (IW_BYTES + i8_box_bytes(half));
+        const uint32_t bytes = 2u * (uint32_t)(IW_BYTES + half * IK);
         const int w_row = tl.g * p.N + tl.n0 + (int)rank * IH;
         const int t_row = tl.tok0 + (int)rank * half;
         for (int kb = 0; kb < num_kb; kb++) {
@@ -159,7 +154,13 @@ grouped_gemm_int8_kernel(const __grid_constant__ I8Maps maps, const __grid_const
           if (leader) mbar_arrive_expect_tx(&full_bar[stage], bytes);
           const uint32_t bar0 = mapa_u32(smem_u32(&full_bar[stage]), 0);
           tma_load_2d_pair(sw, &maps.w, kb * IK, w_row, bar0);
-          tma_load_2d_pair(sw + IW_BYTES, tok, kb * IK, t_row, bar0);
+          int at = 0;
+          #pragma unroll
+          for (int b = 3; b >= 0; b--)
+            if (half & (16 << b)) {
+              tma_load_2d_pair(sw + IW_BYTES + at * IK, &maps.tok[b], kb * IK, t_row + at, bar0);
+              at += 16 << b;
+            }
           if (++stage == stages) { stage = 0; phase ^= 1u; }
         }
       }

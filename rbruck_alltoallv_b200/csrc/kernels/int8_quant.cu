@@ -27,36 +27,45 @@ struct QuantArgs {
   int zeros;
 };
 
-// Largest magnitude of the eight values; a NaN turns into +inf, which the caller looks for.
-__device__ __forceinline__ float vec_max(uint4 v, float m) {
+// Largest magnitudes of the even and the odd ones of eight values; a NaN stays.
+__device__ __forceinline__ __nv_bfloat162 vec_max(uint4 v, __nv_bfloat162 m) {
   const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&v);
+  #pragma unroll
+  for (int j = 0; j < 4; j++) m = __hmax2_nan(m, __habs2(h[j]));
+  return m;
+}
+__device__ __forceinline__ float no_nan(float m) { return m == m ? m : INFINITY; }
+
+__device__ __forceinline__ unsigned quantize_slowly(float x, float s) {
+  return (unsigned)max(-127, min(127, __float2int_rn(__fdiv_rn(x, s)))) & 0xffu;
+}
+
+// t = x * inv is within 2^-22 of x / s, relatively, and |t| <= 127.01: where t is further than 2^-14 from a half both round alike.
+// Adding 1.5 * 2^23 rounds t to an integer, which then stands in the low byte.
+__device__ __forceinline__ uint2 quantize_vec(uint4 v, float s, float inv) {
+  const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&v);
+  constexpr float kMagic = 12582912.0f;
+  unsigned u[8];
+  float far = 0.0f;                        // largest distance from the integer next to it
   #pragma unroll
   for (int j = 0; j < 4; j++) {
     const float2 f = __bfloat1622float2(h[j]);
-    const float a = fabsf(f.x), b = fabsf(f.y);
-    m = fmaxf(m, a == a ? a : INFINITY);
-    m = fmaxf(m, b == b ? b : INFINITY);
+    const float a = __fmul_rn(f.x, inv), b = __fmul_rn(f.y, inv), ua = __fadd_rn(a, kMagic), ub = __fadd_rn(b, kMagic);
+    far = fmaxf(far, fabsf(__fsub_rn(a, __fsub_rn(ua, kMagic))));
+    far = fmaxf(far, fabsf(__fsub_rn(b, __fsub_rn(ub, kMagic))));
+    u[2 * j] = __float_as_uint(ua);
+    u[2 * j + 1] = __float_as_uint(ub);
   }
-  return m;
-}
-
-__device__ __forceinline__ unsigned quantize(float x, float s, float inv) {
-  const float t = x * inv, r = rintf(t);
-  int i = __float2int_rn(t);
-  // |t| <= 127.01 and t is within 2^-22 of x / s, relatively: further than 2^-14 from a half both round alike
-  if (fabsf(fabsf(t - r) - 0.5f) < 6.2e-5f) i = __float2int_rn(__fdiv_rn(x, s));
-  return (unsigned)max(-127, min(127, i)) & 0xffu;
-}
-
-__device__ __forceinline__ uint2 quantize_vec(uint4 v, float s, float inv) {
-  const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&v);
-  unsigned w[2];
-  #pragma unroll
-  for (int j = 0; j < 2; j++) {
-    const float2 a = __bfloat1622float2(h[2 * j]), b = __bfloat1622float2(h[2 * j + 1]);
-    w[j] = quantize(a.x, s, inv) | (quantize(a.y, s, inv) << 8) | (quantize(b.x, s, inv) << 16) | (quantize(b.y, s, inv) << 24);
+  if (far > 0.5f - 6.2e-5f) {              // one in a thousand
+    #pragma unroll
+    for (int j = 0; j < 4; j++) {
+      const float2 f = __bfloat1622float2(h[j]);
+      u[2 * j] = quantize_slowly(f.x, s);
+      u[2 * j + 1] = quantize_slowly(f.y, s);
+    }
   }
-  return make_uint2(w[0], w[1]);
+  return make_uint2(__byte_perm(__byte_perm(u[0], u[1], 0x0040), __byte_perm(u[2], u[3], 0x0040), 0x5410),
+                    __byte_perm(__byte_perm(u[4], u[5], 0x0040), __byte_perm(u[6], u[7], 0x0040), 0x5410));
 }
 
 // A row per blockDim.x threads (a warp, or the CTA); NV vectors per thread in registers, 0: read the row twice.
@@ -73,7 +82,7 @@ __global__ void __launch_bounds__(512) quantize_rows_int8_kernel(const __grid_co
   for (long long r = (long long)blockIdx.x * blockDim.y + threadIdx.y; r < rows; r += (long long)gridDim.x * blockDim.y) {
     const uint4* x = reinterpret_cast<const uint4*>(a.x + r * a.ldx);
     uint4 v[NV ? NV : 1];
-    float m = 0.0f;
+    __nv_bfloat162 both = __float2bfloat162_rn(0.0f);
     if (NV) {
       #pragma unroll
       for (int i = 0; i < NV; i++) {
@@ -82,10 +91,11 @@ __global__ void __launch_bounds__(512) quantize_rows_int8_kernel(const __grid_co
         if (at < nvec) v[i] = __ldg(x + at);
       }
       #pragma unroll
-      for (int i = 0; i < NV; i++) m = vec_max(v[i], m);
+      for (int i = 0; i < NV; i++) both = vec_max(v[i], both);
     } else {
-      for (int at = threadIdx.x; at < nvec; at += blockDim.x) m = vec_max(__ldg(x + at), m);
+      for (int at = threadIdx.x; at < nvec; at += blockDim.x) both = vec_max(__ldg(x + at), both);
     }
+    float m = fmaxf(no_nan(__low2float(both)), no_nan(__high2float(both)));       // (a NaN counts as an infinity: both make the row NaN)
     #pragma unroll
     for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
     if (blockDim.x > 32) {
@@ -128,7 +138,10 @@ cudaError_t launch_quantize_rows_int8(const void* x, long long rows, const int* 
   if (e != cudaSuccess) return e;
   const QuantArgs a{static_cast<const __nv_bfloat16*>(x), rows, ldx, used, K, static_cast<int8_t*>(q), scale, zero, zeros};
   const int nvec = K / 8;
-  const int threads = nvec <= 32 ? 32 : nvec <= 512 ? (nvec + 31) / 32 * 32 : 512, per_cta = threads == 32 ? 4 : 1;
+  // Few rows: as many threads per row as it has vectors, for latency.  More rows than SMs: four vectors per thread, so that an SM
+  // has some eight rows on the way (with 512 threads per row of 4096 it had three: 16384 rows took 95 us, now XXQ).
+  const int want_nv = rows > sms ? 4 : 1, lanes = (nvec + want_nv - 1) / want_nv;
+  const int threads = lanes <= 32 ? 32 : lanes <= 512 ? (lanes + 31) / 32 * 32 : 512, per_cta = threads == 32 ? 4 : 1;
   const int nv = (nvec + threads - 1) / threads;
   const long long want = (rows + per_cta - 1) / per_cta, most = (long long)sms * (2048 / (threads * per_cta));
   const dim3 grid((unsigned)(want < most ? want : most)), block(threads, per_cta);
