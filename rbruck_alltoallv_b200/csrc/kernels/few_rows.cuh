@@ -122,7 +122,7 @@ struct Cursor {
 };
 
 // Shared memory of a CTA: the buffer in which warps add their sums, then the stages, 1024-byte aligned.
-constexpr uint32_t kRedBytes = 2 * 2 * kCols * 32 * 16;       // two groups of weight rows at a time per part
+constexpr uint32_t kRedBytes = 2 * 4 * kCols * 32 * 16;       // four groups of weight rows at a time per part
 // A stage: `tile` weight rows and, where those of A go through shared memory too, `rows` of them (0 otherwise).
 __host__ __device__ inline uint32_t slot_bytes(int tile, int rows) { return (uint32_t)(tile + rows) * kChunk; }
 // Rows of the box that holds r rows of A.
@@ -288,24 +288,29 @@ __device__ __forceinline__ void multiply(Acc (&acc)[S::MT][S::GROUPS][4], uint32
 template <typename S, typename Acc, typename Put>
 __device__ __forceinline__ void add_columns(const Acc (&acc)[S::MT][S::GROUPS][4], uint4* red, int g0, int groups, int part, int col,
                                             int lane, Put&& put) {
-  uint4* mine = red + part * (2 * kCols * 32);
-  const int sub = col >> 1, h = col & 1;   // which of two groups, and which half of a tile's rows, this warp adds
+  uint4* mine = red + part * (4 * kCols * 32);
   #pragma unroll
   for (int m = 0; m < S::MT; m++)
     #pragma unroll
-    for (int n = 0; n < S::GROUPS; n += 2) {
+    for (int n = 0; n < S::GROUPS; n += 4) {
       if (n >= groups) break;
-      mine[col * 32 + lane] = *reinterpret_cast<const uint4*>(acc[m][n]);
-      mine[(kCols + col) * 32 + lane] = *reinterpret_cast<const uint4*>(acc[m][n + 1]);
-      part_sync(part);
-      Acc v0 = 0, v1 = 0;
       #pragma unroll
-      for (int j = 0; j < kCols; j++) {
-        const uint2 u = reinterpret_cast<const uint2*>(mine + (sub * kCols + j) * 32 + lane)[h];
-        v0 += *reinterpret_cast<const Acc*>(&u.x);
-        v1 += *reinterpret_cast<const Acc*>(&u.y);
+      for (int i = 0; i < 4; i++) mine[(i * kCols + col) * 32 + lane] = *reinterpret_cast<const uint4*>(acc[m][n + i]);
+      part_sync(part);
+      if (n + col < groups) {              // warp `col` adds the columns of group n + col
+        Acc v[4] = {0, 0, 0, 0};
+        #pragma unroll
+        for (int j = 0; j < kCols; j++) {
+          const uint4 u = mine[(col * kCols + j) * 32 + lane];
+          v[0] += *reinterpret_cast<const Acc*>(&u.x);
+          v[1] += *reinterpret_cast<const Acc*>(&u.y);
+          v[2] += *reinterpret_cast<const Acc*>(&u.z);
+          v[3] += *reinterpret_cast<const Acc*>(&u.w);
+        }
+        #pragma unroll
+        for (int h = 0; h < 2; h++)
+          put(S::row(m, S::set(part), h, lane), (g0 + n + col) * 8 + (lane & 3) * 2, v[2 * h], v[2 * h + 1]);
       }
-      if (n + sub < groups) put(S::row(m, S::set(part), h, lane), (g0 + n + sub) * 8 + (lane & 3) * 2, v0, v1);
       part_sync(part);
     }
 }

@@ -197,51 +197,68 @@ struct UpWalk {
   }
 };
 
-template <typename S, int TOKENS>
-__device__ __forceinline__ void up_piece(const FewArgs& a, Shared<TOKENS>& s, uint4* red, Cursor& cur, const UpPiece& p, int warp, int lane) {
-  const int R = s.choice.rows[p.u], groups = p.rows / 8, part = warp >> 2, col = warp & 3;
-  const int g0 = S::group0(part, groups), mine = S::my_groups(part, groups);
-  uint32_t off[S::GROUPS];
-  #pragma unroll
-  for (int n = 0; n < S::GROUPS; n++) off[n] = group_offset(p.rows, g0 + n, col);
-  const short* list = s.choice.list + s.choice.start[p.u];
-  const uint8_t* src[S::MT][2];
-  #pragma unroll
-  for (int m = 0; m < S::MT; m++)
-    #pragma unroll
-    for (int h = 0; h < 2; h++) {
-      const int r = S::row(m, S::set(part), h, lane);
-      src[m][h] = r < R ? a.x + (long long)(list[r] / a.top_k) * a.ldx : nullptr;
-    }
-  float acc[S::MT][S::GROUPS][4];
-  clear<S>(acc);
+// The pieces from p on whose experts have at most S's rows: consumer warps.  The rows of the next piece's first chunks are
+// fetched before the sums of a piece are put together: they come from L2 as late as a tenth of a piece.  (`more`: p is one.)
+template <int MAX> __device__ __forceinline__ int row_class(int rows) { return MAX == 16 || rows <= 16 ? 16 : MAX == 32 || rows <= 32 ? 32 : 64; }
+
+template <typename S, int MAX, int CLASS>
+__device__ __forceinline__ void up_pieces(const FewArgs& a, Shared<MAX>& s, uint4* red, Cursor& cur, UpWalk& walk, UpPiece& p, bool& more,
+                                          int warp, int lane) {
+  const int part = warp >> 2, col = warp & 3;
   const int row_bytes = 2 * a.H, chunks = (row_bytes + kChunk - 1) / kChunk;
-  auto run = [&](auto tag) {
-    constexpr int G = decltype(tag)::value;
-    Rows<S> ahead[S::AHEAD + 1];             // (beyond the last chunk nothing is read)
+  const uint8_t* src[S::MT][2];
+  Rows<S> ahead[S::AHEAD + 1];             // (beyond the last chunk nothing is read)
+  auto start = [&](const UpPiece& piece) {
+    const int R = s.choice.rows[piece.u];
+    const short* list = s.choice.list + s.choice.start[piece.u];
+    #pragma unroll
+    for (int m = 0; m < S::MT; m++)
+      #pragma unroll
+      for (int h = 0; h < 2; h++) {
+        const int r = S::row(m, S::set(part), h, lane);
+        src[m][h] = r < R ? a.x + (long long)(list[r] / a.top_k) * a.ldx : nullptr;
+      }
     #pragma unroll
     for (int i = 0; i < S::AHEAD; i++) ahead[i].load(src, row_bytes, i, col, lane);
-    #pragma unroll 1
-    for (int c = 0; c < chunks; c++) {
-      ahead[S::AHEAD].load(src, row_bytes, c + S::AHEAD, col, lane);
-      cur.wait_full();
-      __syncwarp();
-      multiply<S, G>(acc, cur.slot, off, mine, ahead[0], lane);
-      __syncwarp();
-      if (lane == 0) cur.release();
-      cur.next();
-      #pragma unroll
-      for (int i = 0; i < S::AHEAD; i++) ahead[i] = ahead[i + 1];
-    }
   };
-  if (S::GROUPS == 4 && S::MT == 1 && groups <= 4) run(std::integral_constant<int, 2>());
-  else run(std::integral_constant<int, S::GROUPS>());
-  add_columns<S>(acc, red, g0, mine, part, col, lane, [&](int r, int row, float gate, float up) {
-    if (r >= R) return;
-    const int i = s.choice.start[p.u] + r;
-    const float y = s.choice.weight[s.choice.list[i]] * (gate / (1.0f + __expf(-gate)) * up);
-    a.h[(long long)i * a.I + (p.row0 + row) / 2] = __float2bfloat16_rn(y);
-  });
+  start(p);
+  do {
+    const int R = s.choice.rows[p.u], groups = p.rows / 8;
+    const int g0 = S::group0(part, groups), mine = S::my_groups(part, groups);
+    uint32_t off[S::GROUPS];
+    #pragma unroll
+    for (int n = 0; n < S::GROUPS; n++) off[n] = group_offset(p.rows, g0 + n, col);
+    float acc[S::MT][S::GROUPS][4];
+    clear<S>(acc);
+    auto run = [&](auto tag) {
+      constexpr int G = decltype(tag)::value;
+      #pragma unroll 1
+      for (int c = 0; c < chunks; c++) {
+        ahead[S::AHEAD].load(src, row_bytes, c + S::AHEAD, col, lane);
+        cur.wait_full();
+        __syncwarp();
+        multiply<S, G>(acc, cur.slot, off, mine, ahead[0], lane);
+        __syncwarp();
+        if (lane == 0) cur.release();
+        cur.next();
+        #pragma unroll
+        for (int i = 0; i < S::AHEAD; i++) ahead[i] = ahead[i + 1];
+      }
+    };
+    if (S::GROUPS == 4 && S::MT == 1 && groups <= 4) run(std::integral_constant<int, 2>());
+    else run(std::integral_constant<int, S::GROUPS>());
+    const UpPiece done = p;
+    more = walk.next(p);
+    const bool same = more && row_class<MAX>(s.choice.rows[p.u]) == CLASS;
+    if (same) start(p);
+    add_columns<S>(acc, red, g0, mine, part, col, lane, [&](int r, int row, float gate, float up) {
+      if (r >= R) return;
+      const int i = s.choice.start[done.u] + r;
+      const float y = s.choice.weight[s.choice.list[i]] * (gate / (1.0f + __expf(-gate)) * up);
+      a.h[(long long)i * a.I + (done.row0 + row) / 2] = __float2bfloat16_rn(y);
+    });
+    if (!same) return;
+  } while (true);
 }
 
 // MAX: tokens, and with them rows of an expert, at most: 16, 32 or 64.
@@ -268,11 +285,12 @@ __global__ void __launch_bounds__(kThreads, 1) moe_few_up_kernel(const __grid_co
     while (walk.next(p) && feed<__nv_bfloat16>(maps, cur, 0, s.choice.used[p.u] * 2 * a.I + p.row0, p.rows, 0, chunks)) {}
     return;
   }
-  while (walk.next(p)) {
-    const int R = s.choice.rows[p.u];
-    if (MAX == 16 || R <= 16) up_piece<Spread<1, false>>(a, s, red, cur, p, warp, lane);
-    else if (MAX == 32 || R <= 32) up_piece<Spread<2, false>>(a, s, red, cur, p, warp, lane);
-    else up_piece<Spread<2, true>>(a, s, red, cur, p, warp, lane);
+  bool more = walk.next(p);
+  while (more) {
+    const int rows = row_class<MAX>(s.choice.rows[p.u]);
+    if (MAX == 16 || rows == 16) up_pieces<Spread<1, false>, MAX, 16>(a, s, red, cur, walk, p, more, warp, lane);
+    else if (MAX == 32 || rows == 32) up_pieces<Spread<2, false>, MAX, 32>(a, s, red, cur, walk, p, more, warp, lane);
+    else up_pieces<Spread<2, true>, MAX, 64>(a, s, red, cur, walk, p, more, warp, lane);
   }
   if (!cur.ok && a.error) atomicExch(a.error, 1);
 }
