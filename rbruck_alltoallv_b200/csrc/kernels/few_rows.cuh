@@ -350,9 +350,12 @@ inline bool split_plan(long long n, long long row_bytes, long long experts, int 
   return (n + *tile - 1) / *tile * steps * sms <= 0xffffffffll;
 }
 
-// Stages that fit beside `fixed` bytes of static shared memory.
+// Dynamic shared memory that a CTA can have beside `fixed` bytes of static variables (which the compiler may round up).
+inline size_t ring_room(size_t fixed) { return 227 * 1024 - (fixed + 511) / 256 * 256; }
+
+// Stages that fit.
 inline int ring_stages(int tile, int rows, size_t fixed) {
-  const size_t room = 227 * 1024 - 1024 /*alignment*/ - fixed - kRedBytes, n = room / slot_bytes(tile, rows);
+  const size_t room = ring_room(fixed) - 1024 /*alignment*/ - kRedBytes, n = room / slot_bytes(tile, rows);
   return n > (size_t)kMaxStages ? kMaxStages : (int)n;
 }
 // Once per kernel and device: as much dynamic shared memory as there is beside `fixed` bytes.  (A call on one token takes less
@@ -363,7 +366,7 @@ inline cudaError_t allow_smem_once(size_t fixed) {
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess || (dev < 64 && (done.load(std::memory_order_relaxed) >> dev & 1))) return e;
-  e = cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(227 * 1024 - fixed));
+  e = cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)ring_room(fixed));
   if (e == cudaSuccess && dev < 64) done.fetch_or(1ull << dev, std::memory_order_relaxed);
   return e;
 }

@@ -51,12 +51,12 @@ struct Choice {
   float weight[kMaxSlots];
   short at[kMaxSlots];                    // row of the slot among its expert's rows
   short list[kMaxSlots];                  // slots by used expert
-  short used[kMoeMaxExperts];             // experts that have rows, in order
+  short used[kMoeMaxExperts];             // experts that have rows
   short index[kMoeMaxExperts];            // place of an expert in `used`
-  short start[kMoeMaxExperts + 1];        // first entry of `list` of a used expert
-  short rows[kMoeMaxExperts];             // rows of an expert
+  short start[kMoeMaxExperts];            // first entry of `list` of a used expert
+  short rows[kMoeMaxExperts];             // rows of a used expert
   int warp_used[8], warp_rows[8];
-  int n_used, n_slots;
+  int n_used;
 };
 
 // Larger keys for larger logits, NaN above all, equal for both zeros; kMasked and below: -inf.
@@ -122,6 +122,37 @@ __device__ __forceinline__ void choose(Choice<TOKENS>& c, const FewArgs& a) {   
     }
   }
   __syncthreads();
+  if (slots <= 32) {
+    // a warp sees all slots: experts in the order of their first slot
+    if (warp == 0) {
+      const int e = lane < slots ? c.expert[lane] : -1;
+      const unsigned live = __ballot_sync(0xffffffffu, e >= 0), same = __match_any_sync(0xffffffffu, e) & live, below = (1u << lane) - 1u;
+      const bool first = e >= 0 && (same & below) == 0;
+      const unsigned firsts = __ballot_sync(0xffffffffu, first);
+      const int n = __popc(same), u = __popc(firsts & below);
+      int start = first ? n : 0;
+      #pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, start, o);
+        if (lane >= o) start += v;
+      }
+      start -= first ? n : 0;
+      start = __shfl_sync(0xffffffffu, start, same ? __ffs(same) - 1 : 0);
+      if (first) {
+        c.used[u] = (short)e;
+        c.start[u] = (short)start;
+        c.rows[u] = (short)n;
+      }
+      if (e >= 0) {
+        const int at = __popc(same & below);
+        c.at[lane] = (short)at;
+        c.list[start + at] = (short)lane;
+      }
+      if (lane == 0) c.n_used = __popc(firsts);
+    }
+    __syncthreads();
+    return;
+  }
   // rows of every expert, in the order of the slots
   int n = 0;
   if (tid < a.E) {
@@ -139,11 +170,10 @@ __device__ __forceinline__ void choose(Choice<TOKENS>& c, const FewArgs& a) {   
     }
     if (lane == 31) { c.warp_used[warp] = __popc(has); c.warp_rows[warp] = before; }
     consumers_sync();
-    int u = __popc(has & ((1u << lane) - 1u)), r = before - n, all_used = 0, all_rows = 0;
+    int u = __popc(has & ((1u << lane) - 1u)), r = before - n, all_used = 0;
     for (int w = 0; w < 8; w++) {
       if (w < warp) { u += c.warp_used[w]; r += c.warp_rows[w]; }
       all_used += c.warp_used[w];
-      all_rows += c.warp_rows[w];
     }
     if (n > 0) {
       c.used[u] = (short)tid;
@@ -151,7 +181,7 @@ __device__ __forceinline__ void choose(Choice<TOKENS>& c, const FewArgs& a) {   
       c.start[u] = (short)r;
       c.rows[u] = (short)n;
     }
-    if (tid == 0) { c.n_used = all_used; c.n_slots = all_rows; }
+    if (tid == 0) c.n_used = all_used;
   }
   __syncthreads();
   for (int s = tid; s < slots; s += blockDim.x)

@@ -3,7 +3,8 @@ from __future__ import annotations
 
 import torch
 
-from ..ops.moe import MoEExpertParallel, reference_forward
+from ..ops.moe import MoEExpertParallel, linear_int8, quantize_weight_int8, reference_forward
+from ..ops.norm import block_norm
 
 
 class MoELayer:
@@ -34,6 +35,32 @@ class MoELayer:
     __call__ = forward
 
 
+class MoEBlock:
+    """The FFN block of a transformer around a :class:`MoELayer` with a router weight: RMS norm in front of the experts, RMS norm
+    of their output, a gate and a residual scale (``residual + scale * gate * norm(experts(norm(residual)))``), and the norm in
+    front of the next block where ``next_weight`` is given.
+
+    ``pre_weight``, ``post_weight``, ``next_weight`` [H] and ``gate`` (per channel, token or element; optional) as
+    :func:`~rbruck_alltoallv_b200.ops.norm.block_norm` takes them; the residual is bf16 or fp32."""
+
+    def __init__(self, layer: MoELayer, pre_weight, post_weight, gate=None, scale=1.0, next_weight=None, eps=1e-6):
+        if layer.router_weight is None:
+            raise ValueError("the block's layer needs a router weight")
+        self.layer, self.pre_weight, self.post_weight, self.gate = layer, pre_weight, post_weight, gate
+        self.scale, self.next_weight, self.eps = scale, next_weight, eps
+
+    def forward(self, residual, normed=None, decode=False):
+        """``(residual, normed)`` behind the block from those in front of it; ``normed`` may be left out for the first block.
+        ``decode``: any number of tokens up to 64, through the layer's :meth:`~MoELayer.decode`."""
+        if normed is None:
+            _, normed = block_norm(residual, pre_weight=self.pre_weight, eps=self.eps)
+        normed = normed.to(torch.bfloat16)
+        out = self.layer.decode(normed) if decode else self.layer(normed)
+        return block_norm(residual, out, self.post_weight, self.gate, self.scale, self.next_weight, self.eps)
+
+    __call__ = forward
+
+
 def smoke_moe(comm=None):
     """Tiny single-GPU forward checked against the fp32 reference."""
     from ..parallel.comm import Communicator
@@ -57,5 +84,24 @@ def smoke_moe(comm=None):
         mx.ep.check()
         rel = (out.float() - ref).norm().item() / ref.norm().item()
         assert rel < 0.08, f"MXFP8 MoE smoke deviates {rel:.3f} from the fp32 reference"
+        # a few decoded tokens, int8 experts, an int8 projection, and the block around the layer, forward and backward of its norms
+        few = layer.decode(x[:5], logits[:5])
+        assert (few.float() - ref[:5]).abs().max().item() <= 0.02 * scale + 1e-3, "few-token MoE smoke mismatch"
+        i8 = MoELayer(own, E, H, I, T, seed=1, fp8="int8")
+        rel = (i8(x, logits).float() - ref).norm().item() / ref.norm().item()
+        i8.ep.check()
+        assert rel < 0.08, f"int8 MoE smoke deviates {rel:.3f} from the fp32 reference"
+        w = torch.randn(I, H, device="cuda", generator=g)
+        y, want = linear_int8(x[:3], *quantize_weight_int8(w)).float(), x[:3].float() @ w.t()
+        assert (y - want).norm() < 0.03 * want.norm(), "int8 linear smoke mismatch"
+        layer.router_weight = torch.randn(E, H, device="cuda", generator=g)
+        ones = torch.ones(H, device="cuda")
+        r, u = MoEBlock(layer, ones, ones, scale=0.5, next_weight=ones)(x)
+        layer.ep.check()
+        assert r.shape == u.shape == x.shape and u.isfinite().all()
+        z = torch.randn(T, H, device="cuda", generator=g).requires_grad_()
+        (dz,) = torch.autograd.grad(block_norm(r.float(), z, ones)[0].sum(), z)
+        # (a norm does not change with its input's length: its gradient has no part along it, but for eps)
+        assert ((dz * z).sum(-1).abs() <= 1e-4 * dz.norm(dim=-1) * z.norm(dim=-1)).all()
     finally:
         own.close()

@@ -18,8 +18,8 @@ import numpy as np
 import torch
 import torch.distributed as dist
 
-from ..ops.moe import (MoEExpertParallel, grouped_gemm, grouped_gemm_fp8, grouped_gemm_mxfp8, quantize_rows_fp8,
-                       quantize_rows_mxfp8, reference_forward)
+from ..ops.moe import (FEW_TOKENS, MoEExpertParallel, grouped_gemm, grouped_gemm_fp8, grouped_gemm_int8, grouped_gemm_mxfp8,
+                       quantize_rows_fp8, quantize_rows_int8, quantize_rows_mxfp8, reference_forward)
 from ..parallel.comm import Communicator
 
 
@@ -72,6 +72,7 @@ def main() -> int:
     ap.add_argument("--fp8", action="store_true", help="expert GEMMs in block-scaled e4m3 (1x128 / 128x128 scales)")
     ap.add_argument("--mx", action="store_true",
                     help="expert GEMMs in MXFP8 (e4m3, power-of-two scales per 32 elements, scaled by the tensor core)")
+    ap.add_argument("--int8", action="store_true", help="expert GEMMs in 8-bit integers (one scale per row and output channel)")
     ap.add_argument("--check", action="store_true", help="compare with the fp32 reference (small sizes only)")
     ap.add_argument("--out", default="")
     a = ap.parse_args()
@@ -85,7 +86,7 @@ def main() -> int:
     heap = 2 * (cap_rows + 128 * El) * H * 2 + (64 << 20)
     comm = Communicator(nranks=world, heap_bytes=heap, arena_bytes=1 << 20)
     E = El * world
-    layer = MoEExpertParallel(comm, E, H, I, T, seed=3, fp8="mx" if a.mx else a.fp8)
+    layer = MoEExpertParallel(comm, E, H, I, T, seed=3, fp8="mx" if a.mx else "int8" if a.int8 else a.fp8)
     g = torch.Generator(device="cuda")
     g.manual_seed(100 + comm.proc)
     x = torch.randn(T, H, device="cuda", generator=g).to(torch.bfloat16)
@@ -94,7 +95,7 @@ def main() -> int:
     layer.forward(x, logits, out)
     layer.check()
     rows = int(layer.totals[0].item())
-    res = {"gpus": world, "expert_gemm_dtype": "mxfp8" if a.mx else ("fp8_e4m3_block_scaled" if a.fp8 else "bf16"), "tokens_per_gpu": T, "hidden": H, "inter": I, "experts": E, "rows_received_rank0": rows}
+    res = {"gpus": world, "expert_gemm_dtype": "mxfp8" if a.mx else "int8" if a.int8 else ("fp8_e4m3_block_scaled" if a.fp8 else "bf16"), "tokens_per_gpu": T, "hidden": H, "inter": I, "experts": E, "rows_received_rank0": rows}
     if a.check:
         if world > 1:
             w13 = [torch.empty_like(layer.w13) for _ in range(world)]
@@ -108,7 +109,7 @@ def main() -> int:
         err = (out.float() - ref).abs().max().item()
         res["max_abs_err"] = err
         res["ref_scale"] = ref.abs().max().item()
-        tol = 0.25 if (a.fp8 or a.mx) else 0.02      # fp8 operands: compared against the unquantised bf16 weights
+        tol = 0.25 if (a.fp8 or a.mx or a.int8) else 0.02      # 8-bit operands: compared against the unquantised bf16 weights
         res["check"] = "ok" if err <= tol * res["ref_scale"] + 1e-3 else "FAILED"
     t_all = _time(lambda: layer.forward(x, logits, out), a.steps, a.warmup)
     layer.check()
@@ -122,6 +123,14 @@ def main() -> int:
                                                 out=layer.h, swiglu=True, error=layer.error[1:2]), a.steps, a.warmup)
         t_g2 = _time(lambda: grouped_gemm_mxfp8(hq, hs, layer.w2_q, layer.w2_s, layer.group_start, layer.group_rows,
                                                 out=layer.y, error=layer.error[2:3]), a.steps, a.warmup)
+    elif a.int8:
+        xq, xs = quantize_rows_int8(layer.xrecv, layer.totals)
+        hq, hs = quantize_rows_int8(layer.h, layer.totals)
+        res["ms_quantize_x"] = float(np.median(_time(lambda: quantize_rows_int8(layer.xrecv, layer.totals), a.steps, a.warmup)))
+        t_g1 = _time(lambda: grouped_gemm_int8(xq, xs, layer.w13_q, layer.w13_s, layer.group_start, layer.group_rows, out=layer.h,
+                                               swiglu=True, error=layer.error[1:2]), a.steps, a.warmup)
+        t_g2 = _time(lambda: grouped_gemm_int8(hq, hs, layer.w2_q, layer.w2_s, layer.group_start, layer.group_rows, out=layer.y,
+                                               error=layer.error[2:3]), a.steps, a.warmup)
     elif a.fp8:
         hq, hs = quantize_rows_fp8(layer.h, layer.totals)
         t_g1 = _time(lambda: grouped_gemm_fp8(xq, xs, layer.w13_q, layer.w13_s, layer.group_start, layer.group_rows,
@@ -138,6 +147,8 @@ def main() -> int:
                                           swiglu=True, error=layer.error[1:2]), a.steps, a.warmup)
         t_g2 = _time(lambda: grouped_gemm(layer.h, layer.w2, layer.group_start, layer.group_rows, out=layer.y,
                                           error=layer.error[2:3]), a.steps, a.warmup)
+    if world == 1 and not layer.fp8 and T <= FEW_TOKENS:
+        res["ms_decode"] = float(np.median(_time(lambda: layer.decode(x, logits, out), a.steps, a.warmup)))
     layer.check()
     rows_t = torch.tensor([rows], device="cuda", dtype=torch.float64)
     if world > 1:

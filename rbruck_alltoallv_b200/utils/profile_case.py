@@ -17,6 +17,10 @@
     python -m rbruck_alltoallv_b200.utils.profile_case moe_mx      # MoE layer with MXFP8 experts (quantising dispatch, pushed combine)
     python -m rbruck_alltoallv_b200.utils.profile_case transpose   # fused pencil transpose, 384^3 complex64
     python -m rbruck_alltoallv_b200.utils.profile_case eager       # eager protocol, Zipf blocks <= 64 KB, radix 2
+    python -m rbruck_alltoallv_b200.utils.profile_case moe_few     # few-token MoE layer, 7 tokens, 4 experts, 4096 / 14336, top-2
+    python -m rbruck_alltoallv_b200.utils.profile_case gemm_int8   # int8 up/gate GEMM, 2 experts x 2048 rows, 4096 -> 2 x 14336
+    python -m rbruck_alltoallv_b200.utils.profile_case int8_few    # int8 linear, 4 rows, 8192 -> 28672
+    python -m rbruck_alltoallv_b200.utils.profile_case norm        # norms around a block, 8192 x 4096 bf16, both passes
     python -m rbruck_alltoallv_b200.utils.profile_case moe         # MoE layer, 8192 tokens x 4096, 8 experts, FFN 1024
 """
 from __future__ import annotations
@@ -128,6 +132,53 @@ def _transpose():
     comm.close()
 
 
+def _moe_few():
+    from ..ops.moe import moe_few_tokens
+    T, H, I, E = 7, 4096, 14336, 4
+    w13 = torch.randn(E, 2 * I, H, device="cuda", dtype=torch.bfloat16).mul_(0.02)
+    w2 = torch.randn(E, H, I, device="cuda", dtype=torch.bfloat16).mul_(0.02)
+    x = torch.randn(T, H, device="cuda").to(torch.bfloat16)
+    logits = torch.randn(T, E, device="cuda")
+    for _ in range(3):
+        moe_few_tokens(x, logits, w13, w2)
+    torch.cuda.synchronize()
+
+
+def _gemm_int8():
+    from ..ops.moe import grouped_gemm_int8, quantize_rows_int8
+    G, rows, H, I = 2, 2048, 4096, 14336
+    q, s = quantize_rows_int8(torch.randn(G * rows, H, device="cuda").to(torch.bfloat16))
+    w = torch.randint(-127, 128, (G, 2 * I, H), device="cuda", dtype=torch.int8)
+    ws = torch.full((G, 2 * I), 2e-4, device="cuda")
+    gs = torch.tensor([0, rows], dtype=torch.int32, device="cuda")
+    gr = torch.tensor([rows, rows], dtype=torch.int32, device="cuda")
+    for _ in range(3):
+        grouped_gemm_int8(q, s, w, ws, gs, gr, swiglu=True)
+    torch.cuda.synchronize()
+
+
+def _int8_few():
+    from ..ops.moe import linear_int8
+    N, K = 28672, 8192
+    w = torch.randint(-127, 128, (N, K), device="cuda", dtype=torch.int8)
+    ws = torch.full((N,), 2e-4, device="cuda")
+    x = torch.randn(4, K, device="cuda").to(torch.bfloat16)
+    for _ in range(3):
+        linear_int8(x, w, ws)
+    torch.cuda.synchronize()
+
+
+def _norm():
+    from ..ops.norm import block_norm
+    T, H = 8192, 4096
+    r, z = (torch.randn(T, H, device="cuda").to(torch.bfloat16).requires_grad_() for _ in range(2))
+    w1, w2, gate = (torch.ones(H, device="cuda", requires_grad=True) for _ in range(3))
+    for _ in range(3):
+        out = block_norm(r, z, w1, gate, 0.5, w2)
+        torch.autograd.grad(out, (r, z, w1, w2, gate), out)
+    torch.cuda.synchronize()
+
+
 def main() -> int:
     case = sys.argv[1] if len(sys.argv) > 1 else "a2av"
     if case == "a2av":
@@ -154,6 +205,14 @@ def main() -> int:
         _transpose()
     elif case == "eager":
         _a2av("rbruck", small=True, r=2, eager=True)
+    elif case == "moe_few":
+        _moe_few()
+    elif case == "gemm_int8":
+        _gemm_int8()
+    elif case == "int8_few":
+        _int8_few()
+    elif case == "norm":
+        _norm()
     elif case == "moe":
         _moe()
     elif case == "moe_mx":
