@@ -6,9 +6,9 @@
 // A CTA streams pieces of W through a ring in shared memory.  One producer warp fetches, for `nr` weight rows (a multiple
 // of 8, at most 64) and a chunk of 512 bytes along K, four columns of 128 bytes with TMA, all four in one box of 64, 32, 16
 // or 8 rows (K beyond the end reads as zero).  Each of eight consumer warps takes one column, and half of the weight rows or of the
-// rows of A; the sums of the four columns are added when the K range of a piece is done.  The rows of A come from L2, either
-// straight into the registers of the lanes that multiply with them, a chunk or two ahead, or, where they lie one behind the
-// other, with TMA through the ring (a second producer): under load L2 takes longer than a stage.
+// rows of A; the sums of the four columns are added when the K range of a piece is done.  The rows of A come through the ring
+// too, fetched by a second producer warp, in one box where they lie one behind the other and four at a time where they do not:
+// under load L2 takes longer than a stage, and registers do not reach far enough ahead.
 //
 // The rows of A are the M (16) of mma.sync and the weight rows its N (8): few rows waste multiplications, which are free
 // here, and not memory traffic, and a CTA's share of the weights can be cut at any multiple of 8 rows.  (tcgen05 would take
@@ -19,7 +19,7 @@
 // two rows that a quarter of a warp reads at a time.
 //
 // One bulk copy per weight row and chunk in place of the boxes reached a quarter of the bandwidth: 401 us against 125 for one
-// token of a layer that reads 704 MB.
+// token of a layer that reads 704 MB; rows of A loaded into registers two chunks ahead, 459 us against YY for 32 tokens of it.
 #pragma once
 #include <atomic>
 #include <cstdint>
@@ -123,7 +123,7 @@ struct Cursor {
 
 // Shared memory of a CTA: the buffer in which warps add their sums, then the stages, 1024-byte aligned.
 constexpr uint32_t kRedBytes = 2 * 4 * kCols * 32 * 16;       // four groups of weight rows at a time per part
-// A stage: `tile` weight rows and, where those of A go through shared memory too, `rows` of them (0 otherwise).
+// A stage: `tile` weight rows and `rows` of A.
 __host__ __device__ inline uint32_t slot_bytes(int tile, int rows) { return (uint32_t)(tile + rows) * kChunk; }
 // Rows of the box that holds r rows of A.
 __host__ __device__ inline int box_rows(int r) { return r <= 8 ? 8 : r <= 16 ? 16 : r <= 32 ? 32 : 64; }
@@ -174,6 +174,38 @@ __device__ __forceinline__ bool feed(const WeightMaps& maps, Cursor& cur, uint32
   return true;
 }
 
+// The same for rows of A that lie anywhere in a matrix: `rows` of them, row i at at(i), into a box of box_rows(rows).  A whole warp;
+// an instruction fetches 128 bytes of four rows (`map`: boxes of one row).
+template <typename E, typename At>
+__device__ __forceinline__ bool feed_gathered(const CUtensorMap* map, Cursor& cur, uint32_t off, int rows, int c0, int c1, At&& at) {
+  const int lane = threadIdx.x & 31, fours = (rows + 3) / 4, items = fours * kCols;
+  const uint32_t col_bytes = (uint32_t)box_rows(rows) * 128u;
+  int row[2][4], x[2];
+  uint32_t to[2];
+  #pragma unroll
+  for (int k = 0; k < 2; k++) {            // (kMaxRows / 4 * kCols = 64 of them at most)
+    const int item = lane + 32 * k, col = item & 3, q = item >> 2;
+    #pragma unroll
+    for (int i = 0; i < 4; i++) row[k][i] = item < items ? at(min(4 * q + i, rows - 1)) : 0;
+    x[k] = col * 128 / (int)sizeof(E);
+    to[k] = off + (uint32_t)col * col_bytes + (uint32_t)q * 512u;
+  }
+  #pragma unroll 1
+  for (int c = c0; c < c1; c++) {
+    cur.wait_empty();
+    if (!cur.ok) return false;
+    if (lane == 0) expect(cur.full, (uint32_t)items * 512u);
+    #pragma unroll
+    for (int k = 0; k < 2; k++)
+      if (lane + 32 * k < items)
+        asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6, %7}], [%2];"
+                     ::"r"(cur.slot + to[k]), "l"(map), "r"(cur.full), "r"(x[k] + c * (kChunk / (int)sizeof(E))), "r"(row[k][0]), "r"(row[k][1]),
+                       "r"(row[k][2]), "r"(row[k][3]) : "memory");
+    cur.next();
+  }
+  return true;
+}
+
 __device__ __forceinline__ void prefetch_maps(const WeightMaps& maps) {      // a warp
   const int lane = threadIdx.x & 31;
   if (lane < 4 && maps.whole && (maps.heights & (8 << lane))) sm100::tma_prefetch_desc(&maps.all[lane]);
@@ -198,7 +230,6 @@ struct Spread {
   static constexpr int MT = MT_;
   static constexpr bool HALVES = HALVES_;
   static constexpr int SETS = HALVES ? 2 : 1;
-  static constexpr int AHEAD = HALVES ? 0 : MT == 1 ? 2 : 1;      // chunks that rows of A from memory are ahead, as registers allow
   static constexpr int GROUPS = HALVES ? kMaxTile / 8 : kMaxTile / 16;      // groups of 8 weight rows of a warp, at most
   // row of A of tile m, upper or lower half h of a warp in part q
   __device__ static __forceinline__ int row(int m, int q, int h, int lane) { return 16 * (m + q * MT) + 8 * h + (lane >> 2); }
@@ -213,19 +244,6 @@ struct Spread {
 template <typename S>
 struct Rows {
   uint4 v[S::MT][2][2];                    // tile, half of the tile, half of the 32 bytes
-  // from memory (nobody writes there meanwhile); `src`: the rows, null for those that do not exist
-  __device__ __forceinline__ void load(const uint8_t* const (&src)[S::MT][2], int row_bytes, int c, int col, int lane) {
-    const int k = c * kChunk + col * 128 + (lane & 3) * 32;
-    #pragma unroll
-    for (int m = 0; m < S::MT; m++)
-      #pragma unroll
-      for (int h = 0; h < 2; h++)
-        #pragma unroll
-        for (int s = 0; s < 2; s++) {
-          v[m][h][s] = make_uint4(0u, 0u, 0u, 0u);
-          if (src[m][h] && k + 16 * s < row_bytes) v[m][h][s] = __ldg(reinterpret_cast<const uint4*>(src[m][h] + k + 16 * s));
-        }
-  }
   // from a box of a stage; `at`: rows of it, negative for those that do not exist
   __device__ __forceinline__ void load(const int (&at)[S::MT][2], uint32_t box, int rows, int col, int lane) {
     const uint32_t base = box + (uint32_t)(col * rows * 128), t = (uint32_t)lane & 3;
@@ -372,6 +390,19 @@ inline cudaError_t allow_smem_once(size_t fixed) {
 }
 inline size_t ring_smem(int tile, int rows, int stages) { return 1024 + kRedBytes + (size_t)slot_bytes(tile, rows) * stages; }
 
+typedef CUresult (*TensorMapEncoder)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                     const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion,
+                                     CUtensorMapFloatOOBfill);
+inline TensorMapEncoder tensor_map_encoder() {       // null: the driver has none
+  static const TensorMapEncoder encode = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    return cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess
+               ? reinterpret_cast<TensorMapEncoder>(p) : nullptr;
+  }();
+  return encode;
+}
+
 // Boxes for pieces of at most `rows` rows, all multiples of 8 among them.
 inline int heights_up_to(int rows) {
   int all = 0;
@@ -379,26 +410,30 @@ inline int heights_up_to(int rows) {
   return all;
 }
 
-// Weights of `rows` rows of row_bytes (a multiple of 16) each, elements of `size` bytes; 128-byte swizzle.  Bits 3 to 6 of
+// Rows for feed_gathered: `rows` of `len` bytes, `row_bytes` apart (multiples of 16).
+inline bool gather_map(CUtensorMap* m, const void* base, unsigned long long rows, unsigned long long len, unsigned long long row_bytes,
+                       CUtensorMapDataType type, int size) {
+  const cuuint64_t dims[2] = {len / size, rows}, strides[1] = {row_bytes};
+  const cuuint32_t box[2] = {128u / (unsigned)size, 1}, ones[2] = {1, 1};
+  return tensor_map_encoder() && tensor_map_encoder()(m, type, 2, const_cast<void*>(base), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                                                      CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                                      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// Weights of `rows` rows of row_bytes (a multiple of 16) each, `step` bytes apart, elements of `size` bytes; 128-byte swizzle.  Bits 3 to 6 of
 // `heights`: the boxes that pieces are made of (a map takes a third of a microsecond to make).
 inline bool weight_maps(WeightMaps* m, const void* base, unsigned long long rows, unsigned long long row_bytes, CUtensorMapDataType type,
-                        int size, int heights) {
-  typedef CUresult (*Encode)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
-                             const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-  static const Encode encode = [] {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    return cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess
-               ? reinterpret_cast<Encode>(p) : nullptr;
-  }();
+                        int size, int heights, unsigned long long step = 0) {
+  if (!step) step = row_bytes;
+  const TensorMapEncoder encode = tensor_map_encoder();
   if (!encode) return false;
   const unsigned per_col = 128u / (unsigned)size;
   m->heights = heights;
   const cuuint64_t cols = row_bytes / 128;                 // whole columns
   const bool even = row_bytes % 128 == 0;
   m->whole = (int)(even ? (cols + kCols - 1) / kCols : cols / kCols);      // (columns behind the last one read as zeros)
-  const cuuint64_t dims3[3] = {per_col, rows, cols}, strides3[2] = {row_bytes, 128};
-  const cuuint64_t dims2[2] = {row_bytes / size, rows}, strides2[1] = {row_bytes};
+  const cuuint64_t dims3[3] = {per_col, rows, cols}, strides3[2] = {step, 128};
+  const cuuint64_t dims2[2] = {row_bytes / size, rows}, strides2[1] = {step};
   const cuuint32_t ones[3] = {1, 1, 1};
   for (int b = 0; b < 4; b++) {
     if (!(heights & (8 << b))) continue;

@@ -227,80 +227,66 @@ struct UpWalk {
   }
 };
 
-// The pieces from p on whose experts have at most S's rows: consumer warps.  The rows of the next piece's first chunks are
-// fetched before the sums of a piece are put together: they come from L2 as late as a tenth of a piece.  (`more`: p is one.)
-template <int MAX> __device__ __forceinline__ int row_class(int rows) { return MAX == 16 || rows <= 16 ? 16 : MAX == 32 || rows <= 32 ? 32 : 64; }
-
-template <typename S, int MAX, int CLASS>
-__device__ __forceinline__ void up_pieces(const FewArgs& a, Shared<MAX>& s, uint4* red, Cursor& cur, UpWalk& walk, UpPiece& p, bool& more,
-                                          int warp, int lane) {
-  const int part = warp >> 2, col = warp & 3;
-  const int row_bytes = 2 * a.H, chunks = (row_bytes + kChunk - 1) / kChunk;
-  const uint8_t* src[S::MT][2];
-  Rows<S> ahead[S::AHEAD + 1];             // (beyond the last chunk nothing is read)
-  auto start = [&](const UpPiece& piece) {
-    const int R = s.choice.rows[piece.u];
-    const short* list = s.choice.list + s.choice.start[piece.u];
+template <typename S, int MAX>
+__device__ __forceinline__ void up_piece(const FewArgs& a, Shared<MAX>& s, uint4* red, Cursor& cur, const UpPiece& p, int warp, int lane) {
+  const int R = s.choice.rows[p.u], groups = p.rows / 8, box = MAX == 16 ? a.box : box_rows(R), part = warp >> 2, col = warp & 3;
+  const int g0 = S::group0(part, groups), mine = S::my_groups(part, groups);
+  const int chunks = (2 * a.H + kChunk - 1) / kChunk;
+  uint32_t off[S::GROUPS];
+  #pragma unroll
+  for (int n = 0; n < S::GROUPS; n++) off[n] = group_offset(p.rows, g0 + n, col);
+  int rows_at[S::MT][2];
+  #pragma unroll
+  for (int m = 0; m < S::MT; m++)
     #pragma unroll
-    for (int m = 0; m < S::MT; m++)
-      #pragma unroll
-      for (int h = 0; h < 2; h++) {
-        const int r = S::row(m, S::set(part), h, lane);
-        src[m][h] = r < R ? a.x + (long long)(list[r] / a.top_k) * a.ldx : nullptr;
-      }
-    #pragma unroll
-    for (int i = 0; i < S::AHEAD; i++) ahead[i].load(src, row_bytes, i, col, lane);
+    for (int h = 0; h < 2; h++) {
+      const int r = S::row(m, S::set(part), h, lane);
+      rows_at[m][h] = r >= R ? -1 : MAX == 16 ? s.choice.list[s.choice.start[p.u] + r] / a.top_k : r;
+    }
+  float acc[S::MT][S::GROUPS][4];
+  clear<S>(acc);
+  auto run = [&](auto tag) {
+    constexpr int G = decltype(tag)::value;
+    #pragma unroll 1
+    for (int c = 0; c < chunks; c++) {
+      cur.wait_full();
+      __syncwarp();
+      Rows<S> rows;
+      rows.load(rows_at, cur.slot + (uint32_t)a.tile * kChunk, box, col, lane);
+      multiply<S, G>(acc, cur.slot, off, mine, rows, lane);
+      __syncwarp();
+      if (lane == 0) cur.release();
+      cur.next();
+    }
   };
-  start(p);
-  do {
-    const int R = s.choice.rows[p.u], groups = p.rows / 8;
-    const int g0 = S::group0(part, groups), mine = S::my_groups(part, groups);
-    uint32_t off[S::GROUPS];
-    #pragma unroll
-    for (int n = 0; n < S::GROUPS; n++) off[n] = group_offset(p.rows, g0 + n, col);
-    float acc[S::MT][S::GROUPS][4];
-    clear<S>(acc);
-    auto run = [&](auto tag) {
-      constexpr int G = decltype(tag)::value;
-      #pragma unroll 1
-      for (int c = 0; c < chunks; c++) {
-        ahead[S::AHEAD].load(src, row_bytes, c + S::AHEAD, col, lane);
-        cur.wait_full();
-        __syncwarp();
-        multiply<S, G>(acc, cur.slot, off, mine, ahead[0], lane);
-        __syncwarp();
-        if (lane == 0) cur.release();
-        cur.next();
-        #pragma unroll
-        for (int i = 0; i < S::AHEAD; i++) ahead[i] = ahead[i + 1];
-      }
-    };
-    if (S::GROUPS == 4 && S::MT == 1 && groups <= 4) run(std::integral_constant<int, 2>());
-    else run(std::integral_constant<int, S::GROUPS>());
-    const UpPiece done = p;
-    more = walk.next(p);
-    const bool same = more && row_class<MAX>(s.choice.rows[p.u]) == CLASS;
-    if (same) start(p);
-    add_columns<S>(acc, red, g0, mine, part, col, lane, [&](int r, int row, float gate, float up) {
-      if (r >= R) return;
-      const int i = s.choice.start[done.u] + r;
-      const float y = s.choice.weight[s.choice.list[i]] * (gate / (1.0f + __expf(-gate)) * up);
-      a.h[(long long)i * a.I + (done.row0 + row) / 2] = __float2bfloat16_rn(y);
-    });
-    if (!same) return;
-  } while (true);
+  if (S::GROUPS == 4 && S::MT == 1 && groups <= 4) run(std::integral_constant<int, 2>());
+  else run(std::integral_constant<int, S::GROUPS>());
+  add_columns<S>(acc, red, g0, mine, part, col, lane, [&](int r, int row, float gate, float up) {
+    if (r >= R) return;
+    const int i = s.choice.start[p.u] + r;
+    const float y = s.choice.weight[s.choice.list[i]] * (gate / (1.0f + __expf(-gate)) * up);
+    a.h[(long long)i * a.I + (p.row0 + row) / 2] = __float2bfloat16_rn(y);
+  });
 }
 
-// MAX: tokens, and with them rows of an expert, at most: 16, 32 or 64.
+// MAX: tokens, and with them rows of an expert, at most: 16, 32 or 64.  Up to 16 tokens all of them are fetched for every expert,
+// in one box (4 or 8 KB beside up to 32 of weights); beyond that the expert's own, gathered four at a time (one token of 64
+// experts: 14.4 us gathered, 12.6 in a box; for 32 tokens a box would be half as much as the weights).
+template <int MAX> using XMap = std::conditional_t<MAX == 16, WeightMaps, CUtensorMap>;
 template <int MAX>
-__global__ void __launch_bounds__(kThreads, 1) moe_few_up_kernel(const __grid_constant__ WeightMaps maps, const __grid_constant__ FewArgs a) {
+__global__ void __launch_bounds__(kThreads, 1) moe_few_up_kernel(const __grid_constant__ WeightMaps maps, const __grid_constant__ XMap<MAX> x_map,
+                                                                 const __grid_constant__ FewArgs a) {
   extern __shared__ uint8_t dyn[];
   __shared__ Shared<MAX> s;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   uint8_t* base = aligned_smem(dyn);
   uint4* red = reinterpret_cast<uint4*>(base);
-  if (threadIdx.x == 0) ring_init(s.ring, a.stages, 1);
+  if (threadIdx.x == 0) ring_init(s.ring, a.stages, 2);
   if (warp == kWarps) prefetch_maps(maps);
+  if (warp == kWarps + 1) {
+    if constexpr (MAX == 16) prefetch_maps(x_map);
+    else if (lane == 0) sm100::tma_prefetch_desc(&x_map);
+  }
   pdl_wait();
   pdl_trigger();      // after the wait: the down kernel reads the logits before it waits for this one
   if (blockIdx.x == 0)
@@ -308,19 +294,32 @@ __global__ void __launch_bounds__(kThreads, 1) moe_few_up_kernel(const __grid_co
   choose(s.choice, a);
   UpWalk walk(a, s.choice.n_used);
   UpPiece p;
-  Cursor cur(s.ring, sm100::smem_u32(base + kRedBytes), a.stages, slot_bytes(a.tile, 0));
-  if (warp >= kWarps) {
-    if (warp != kWarps || lane >= 4) return;
-    const int chunks = (2 * a.H + kChunk - 1) / kChunk;
+  Cursor cur(s.ring, sm100::smem_u32(base + kRedBytes), a.stages, slot_bytes(a.tile, a.box));
+  const int chunks = (2 * a.H + kChunk - 1) / kChunk;
+  if (warp == kWarps) {
+    if (lane >= 4) return;
     while (walk.next(p) && feed<__nv_bfloat16>(maps, cur, 0, s.choice.used[p.u] * 2 * a.I + p.row0, p.rows, 0, chunks)) {}
     return;
   }
-  bool more = walk.next(p);
-  while (more) {
-    const int rows = row_class<MAX>(s.choice.rows[p.u]);
-    if (MAX == 16 || rows == 16) up_pieces<Spread<1, false>, MAX, 16>(a, s, red, cur, walk, p, more, warp, lane);
-    else if (MAX == 32 || rows == 32) up_pieces<Spread<2, false>, MAX, 32>(a, s, red, cur, walk, p, more, warp, lane);
-    else up_pieces<Spread<2, true>, MAX, 64>(a, s, red, cur, walk, p, more, warp, lane);
+  if (warp == kWarps + 1) {
+    asm volatile("fence.proxy.async;" ::: "memory");
+    if constexpr (MAX == 16) {
+      if (lane >= 4) return;
+      while (walk.next(p) && feed<__nv_bfloat16>(x_map, cur, (uint32_t)a.tile * kChunk, 0, a.box, 0, chunks)) {}
+    } else {
+      while (walk.next(p)) {
+        const short* list = s.choice.list + s.choice.start[p.u];
+        if (!feed_gathered<__nv_bfloat16>(&x_map, cur, (uint32_t)a.tile * kChunk, s.choice.rows[p.u], 0, chunks,
+                                          [&](int r) { return list[r] / a.top_k; })) break;
+      }
+    }
+    return;
+  }
+  while (walk.next(p)) {
+    const int R = s.choice.rows[p.u];
+    if (MAX == 16 || R <= 16) up_piece<Spread<1, false>>(a, s, red, cur, p, warp, lane);
+    else if (MAX == 32 || R <= 32) up_piece<Spread<2, false>>(a, s, red, cur, p, warp, lane);
+    else up_piece<Spread<2, true>>(a, s, red, cur, p, warp, lane);
   }
   if (!cur.ok && a.error) atomicExch(a.error, 1);
 }
@@ -538,8 +537,13 @@ cudaError_t few_launch(FewArgs a, const FewPlan& p, cudaStream_t st) {
       !weight_maps(&w2, a.w2, (unsigned long long)a.E * a.H, 2ull * a.I, bf16, 2, p.down_tile | a.H % p.down_tile) ||
       !weight_maps(&h, a.h, (unsigned long long)a.T * a.top_k, 2ull * a.I, bf16, 2, heights_up_to(box_rows(a.T))))
     return cudaErrorUnknown;
+  XMap<MAX> x;
+  bool ok;
+  if constexpr (MAX == 16) ok = weight_maps(&x, a.x, (unsigned long long)a.T, 2ull * a.H, bf16, 2, box_rows(a.T), (unsigned long long)a.ldx);
+  else ok = gather_map(&x, a.x, (unsigned long long)a.T, 2ull * a.H, (unsigned long long)a.ldx, bf16, 2);
+  if (!ok) return cudaErrorUnknown;
   a.whole = p.whole;
-  const cudaError_t e = launch_ring<MAX, moe_few_up_kernel<MAX>>(a, p.up_tile, 0, p.sms, st, w13);
+  const cudaError_t e = launch_ring<MAX, moe_few_up_kernel<MAX>>(a, p.up_tile, box_rows(a.T), p.sms, st, w13, x);
   return e != cudaSuccess ? e : launch_ring<MAX, moe_few_down_kernel<MAX>>(a, p.down_tile, box_rows(a.T), p.sms, st, w2, h);
 }
 
