@@ -360,16 +360,60 @@ struct DownWalk {
   }
 };
 
+// More than 16 tokens: an expert's rows by themselves, as in the up product; their sums over the expert's K are added to the
+// tokens' sums in shared memory, expert by expert.
+template <typename S, int MAX>
+__device__ __forceinline__ void down_piece(const FewArgs& a, Shared<MAX>& s, uint4* red, float* sums, Cursor& cur, const DownPiece& p, int groups,
+                                           int warp, int lane) {
+  const int R = s.choice.rows[p.u], box = box_rows(R), part = warp >> 2, col = warp & 3;
+  const int g0 = S::group0(part, groups), mine = S::my_groups(part, groups);
+  uint32_t off[S::GROUPS];
+  #pragma unroll
+  for (int n = 0; n < S::GROUPS; n++) off[n] = group_offset(groups * 8, g0 + n, col);
+  int rows_at[S::MT][2];
+  #pragma unroll
+  for (int m = 0; m < S::MT; m++)
+    #pragma unroll
+    for (int h = 0; h < 2; h++) {
+      const int r = S::row(m, S::set(part), h, lane);
+      rows_at[m][h] = r < R ? r : -1;
+    }
+  float acc[S::MT][S::GROUPS][4];
+  clear<S>(acc);
+  #pragma unroll 1
+  for (int c = p.c0; c < p.c1; c++) {
+    cur.wait_full();
+    __syncwarp();
+    Rows<S> rows;
+    rows.load(rows_at, cur.slot + (uint32_t)a.tile * kChunk, box, col, lane);
+    multiply<S, S::GROUPS>(acc, cur.slot, off, mine, rows, lane);
+    __syncwarp();
+    if (lane == 0) cur.release();
+    cur.next();
+  }
+  const short* list = s.choice.list + s.choice.start[p.u];
+  add_columns<S>(acc, red, g0, mine, part, col, lane, [&](int r, int n, float v0, float v1) {
+    if (r >= R) return;
+    float2* at = reinterpret_cast<float2*>(sums + list[r] / a.top_k * kMaxTile + n);
+    float2 v = *at;
+    v.x += v0;
+    v.y += v1;
+    *at = v;
+  });
+  consumers_sync();                       // the next piece may divide rows and columns among the warps in another way
+}
+
 template <int MAX>
 __global__ void __launch_bounds__(kThreads, 1) moe_few_down_kernel(const __grid_constant__ WeightMaps maps, const __grid_constant__ WeightMaps h_maps,
                                                                    const __grid_constant__ FewArgs a) {
   extern __shared__ uint8_t dyn[];
   __shared__ Shared<MAX> s;
-  using S = Spread<(MAX > 16 ? 2 : 1), (MAX > 32)>;
-  constexpr int MT = S::MT;
+  using S = Spread<1, false>;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   uint8_t* base = aligned_smem(dyn);
   uint4* red = reinterpret_cast<uint4*>(base);
+  float* sums = reinterpret_cast<float*>(base + kRedBytes);                // [MAX][kMaxTile] beyond 16 tokens
+  constexpr uint32_t kSumBytes = MAX > 16 ? MAX * kMaxTile * 4 : 0;
   if (tid == 0) ring_init(s.ring, a.stages, 2);
   if (warp >= kWarps) prefetch_maps(warp == kWarps ? maps : h_maps);
   pdl_trigger();
@@ -383,7 +427,7 @@ __global__ void __launch_bounds__(kThreads, 1) moe_few_down_kernel(const __grid_
   }
   DownWalk walk(a, n_used);
   DownPiece p;
-  Cursor cur(s.ring, sm100::smem_u32(base + kRedBytes), a.stages, slot_bytes(a.tile, a.box));
+  Cursor cur(s.ring, sm100::smem_u32(base + kRedBytes + kSumBytes), a.stages, slot_bytes(a.tile, a.box));
   if (warp >= kWarps) {                   // the weights do not wait for the first kernel, the rows of h do
     if (lane >= 4) return;
     if (warp == kWarps) {
@@ -406,55 +450,76 @@ __global__ void __launch_bounds__(kThreads, 1) moe_few_down_kernel(const __grid_
   while (more) {
     const int tile = p.tile, col0 = tile * a.tile, nr = min(a.tile, a.H - col0), groups = nr / 8;
     const bool starts = p.u == 0 && p.c0 == 0;
-    const int g0 = S::group0(part, groups), mine = S::my_groups(part, groups);
-    uint32_t off[S::GROUPS];
-    #pragma unroll
-    for (int n = 0; n < S::GROUPS; n++) off[n] = group_offset(nr, g0 + n, wcol);
-    float acc[MT][S::GROUPS][4];
-    clear<S>(acc);
     bool ends;
-    do {
-      // where the tokens' rows of h are in a stage of the expert: tokens that did not choose it count as zeros
-      const int box = box_rows(s.choice.rows[p.u]), e = s.choice.used[p.u];
-      int rows_at[MT][2];
-      #pragma unroll
-      for (int m = 0; m < MT; m++)
-        #pragma unroll
-        for (int h = 0; h < 2; h++) {
-          const int t = S::row(m, S::set(part), h, lane);
-          rows_at[m][h] = -1;
-          if (t < a.T)
-            for (int j = 0; j < a.top_k; j++)
-              if (s.choice.expert[t * a.top_k + j] == e) rows_at[m][h] = s.choice.at[t * a.top_k + j];
-        }
-      auto run = [&](auto tag) {
-        constexpr int G = decltype(tag)::value;
-        #pragma unroll 1
-        for (int c = p.c0; c < p.c1; c++) {
-          cur.wait_full();
-          __syncwarp();
-          Rows<S> rows;
-          rows.load(rows_at, cur.slot + (uint32_t)a.tile * kChunk, box, wcol, lane);
-          multiply<S, G>(acc, cur.slot, off, mine, rows, lane);
-          __syncwarp();
-          if (lane == 0) cur.release();
-          cur.next();
-        }
-      };
-      if (MAX == 16 && groups <= 2) run(std::integral_constant<int, 1>());
-      else if (MAX == 16 && groups <= 4) run(std::integral_constant<int, 2>());
-      else run(std::integral_constant<int, S::GROUPS>());
-      ends = p.u == n_used - 1 && p.c1 == walk.chunks;
-      more = walk.next(p);
-    } while (more && p.tile == tile);
     // a tile cut by the end of a range: the sums go to the workspace, for the last CTA to arrive
-    const bool whole = starts && ends;
     float* part_sums = a.partial + (2ll * blockIdx.x + (starts ? 1 : 0)) * a.T * a.tile;
-    add_columns<S>(acc, red, g0, mine, part, wcol, lane, [&](int t, int col, float v0, float v1) {
-      if (t >= a.T) return;
+    auto result = [&](bool whole, int t, int col, float v0, float v1) {
       if (whole) *reinterpret_cast<__nv_bfloat162*>(a.out + (long long)t * a.H + col0 + col) = __floats2bfloat162_rn(v0, v1);
       else *reinterpret_cast<float2*>(part_sums + (long long)t * a.tile + col) = make_float2(v0, v1);
-    });
+    };
+    bool whole;
+    if constexpr (MAX == 16) {
+      // all tokens at once, those that did not choose an expert as zeros: its sums stay in the accumulators
+      const int g0 = S::group0(part, groups), mine = S::my_groups(part, groups);
+      uint32_t off[S::GROUPS];
+      #pragma unroll
+      for (int n = 0; n < S::GROUPS; n++) off[n] = group_offset(nr, g0 + n, wcol);
+      float acc[S::MT][S::GROUPS][4];
+      clear<S>(acc);
+      do {
+        const int box = box_rows(s.choice.rows[p.u]), e = s.choice.used[p.u];
+        int rows_at[1][2];
+        #pragma unroll
+        for (int h = 0; h < 2; h++) {
+          const int t = S::row(0, 0, h, lane);
+          rows_at[0][h] = -1;
+          if (t < a.T)
+            for (int j = 0; j < a.top_k; j++)
+              if (s.choice.expert[t * a.top_k + j] == e) rows_at[0][h] = s.choice.at[t * a.top_k + j];
+        }
+        auto run = [&](auto tag) {
+          constexpr int G = decltype(tag)::value;
+          #pragma unroll 1
+          for (int c = p.c0; c < p.c1; c++) {
+            cur.wait_full();
+            __syncwarp();
+            Rows<S> rows;
+            rows.load(rows_at, cur.slot + (uint32_t)a.tile * kChunk, box, wcol, lane);
+            multiply<S, G>(acc, cur.slot, off, mine, rows, lane);
+            __syncwarp();
+            if (lane == 0) cur.release();
+            cur.next();
+          }
+        };
+        if (groups <= 2) run(std::integral_constant<int, 1>());
+        else if (groups <= 4) run(std::integral_constant<int, 2>());
+        else run(std::integral_constant<int, S::GROUPS>());
+        ends = p.u == n_used - 1 && p.c1 == walk.chunks;
+        more = walk.next(p);
+      } while (more && p.tile == tile);
+      whole = starts && ends;
+      add_columns<S>(acc, red, g0, mine, part, wcol, lane, [&](int t, int col, float v0, float v1) {
+        if (t < a.T) result(whole, t, col, v0, v1);
+      });
+    } else {
+      for (int i = tid; i < a.T * kMaxTile; i += kWarps * 32) sums[i] = 0.0f;
+      consumers_sync();
+      do {
+        const int rows = s.choice.rows[p.u];
+        if (rows <= 16) down_piece<Spread<1, false>>(a, s, red, sums, cur, p, groups, warp, lane);
+        else if (MAX == 32 || rows <= 32) down_piece<Spread<2, false>>(a, s, red, sums, cur, p, groups, warp, lane);
+        else down_piece<Spread<2, true>>(a, s, red, sums, cur, p, groups, warp, lane);
+        ends = p.u == n_used - 1 && p.c1 == walk.chunks;
+        more = walk.next(p);
+      } while (more && p.tile == tile);
+      whole = starts && ends;
+      for (int i = tid; i < a.T * (nr / 2); i += kWarps * 32) {
+        const int t = i / (nr / 2), col = (i - t * (nr / 2)) * 2;
+        const float2 v = *reinterpret_cast<const float2*>(sums + t * kMaxTile + col);
+        result(whole, t, col, v.x, v.y);
+      }
+      consumers_sync();                   // the sums are free for the next tile
+    }
     if (!whole) cut[starts ? 1 : 0] = tile;
   }
   // the (at most two) tiles that this CTA shares with others
@@ -521,12 +586,12 @@ bool few_plan(int T, int H, int I, int E, int top_k, FewPlan* p) {
 }
 
 template <int MAX, auto* Kernel, typename... Maps>
-cudaError_t launch_ring(FewArgs a, int tile, int box, int sms, cudaStream_t st, const Maps&... maps) {
+cudaError_t launch_ring(FewArgs a, int tile, int box, size_t sums, int sms, cudaStream_t st, const Maps&... maps) {
   a.tile = tile;
   a.box = box;
-  a.stages = ring_stages(tile, box, sizeof(Shared<MAX>));
+  a.stages = ring_stages(tile, box, sizeof(Shared<MAX>) + sums);
   const cudaError_t e = allow_smem_once<Kernel>(sizeof(Shared<MAX>));
-  return e != cudaSuccess ? e : launch_dependent(Kernel, dim3(sms), dim3(kThreads), ring_smem(tile, box, a.stages), st, maps..., a);
+  return e != cudaSuccess ? e : launch_dependent(Kernel, dim3(sms), dim3(kThreads), ring_smem(tile, box, a.stages) + sums, st, maps..., a);
 }
 
 template <int MAX>
@@ -543,8 +608,8 @@ cudaError_t few_launch(FewArgs a, const FewPlan& p, cudaStream_t st) {
   else ok = gather_map(&x, a.x, (unsigned long long)a.T, 2ull * a.H, (unsigned long long)a.ldx, bf16, 2);
   if (!ok) return cudaErrorUnknown;
   a.whole = p.whole;
-  const cudaError_t e = launch_ring<MAX, moe_few_up_kernel<MAX>>(a, p.up_tile, box_rows(a.T), p.sms, st, w13, x);
-  return e != cudaSuccess ? e : launch_ring<MAX, moe_few_down_kernel<MAX>>(a, p.down_tile, box_rows(a.T), p.sms, st, w2, h);
+  const cudaError_t e = launch_ring<MAX, moe_few_up_kernel<MAX>>(a, p.up_tile, box_rows(a.T), 0, p.sms, st, w13, x);
+  return e != cudaSuccess ? e : launch_ring<MAX, moe_few_down_kernel<MAX>>(a, p.down_tile, box_rows(a.T), MAX > 16 ? (size_t)MAX * kMaxTile * 4 : 0, p.sms, st, w2, h);
 }
 
 }  // namespace
