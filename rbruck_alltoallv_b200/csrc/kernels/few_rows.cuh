@@ -5,21 +5,22 @@
 //
 // A CTA streams pieces of W through a ring in shared memory.  One producer warp fetches, for `nr` weight rows (a multiple
 // of 8, at most 64) and a chunk of 512 bytes along K, four columns of 128 bytes with TMA, all four in one box of 64, 32, 16
-// or 8 rows (K beyond the end reads as zero).  Each of eight consumer warps takes one column, and half of the weight rows or of the
-// rows of A; the sums of the four columns are added when the K range of a piece is done.  The rows of A come through the ring
-// too, fetched by a second producer warp, in one box where they lie one behind the other and four at a time where they do not:
-// under load L2 takes longer than a stage, and registers do not reach far enough ahead.
+// or 8 rows (K beyond the end reads as zero).  Each of eight consumer warps takes a column and half of the weight rows; the
+// sums of the four columns are added when the K range of a piece is done.  The rows of A come through the ring too, fetched
+// by a second producer warp, in one box where they lie one behind the other and four at a time where they do not: under load
+// L2 takes longer than a stage, and registers do not reach far enough ahead.
 //
-// The rows of A are the M (16) of mma.sync and the weight rows its N (8): few rows waste multiplications, which are free
-// here, and not memory traffic, and a CTA's share of the weights can be cut at any multiple of 8 rows.  (tcgen05 would take
-// the weights as M, in tiles of 64 or more rows: for one token and two of 64 experts that is 44 tiles of 128 rows for 148
-// SMs.)  The order of K is free as long as A and W agree: lane t of a row has bytes 32 t to 32 t + 31 of its column, in two
+// Weight rows are the M (16) of mma.sync and rows of A its N (8).  On this GPU mma.sync is slow, a 16 x 8 x 16 product in some 32
+// cycles of a quarter of an SM: with the rows of A as M (and weights as N) up to 16 rows took as many products as 16, and 32
+// tokens of 8 experts were bound by them.  (tcgen05 is not, but its M are tiles of 64 or more weight rows: for one token and two
+// of 64 experts that is 44 tiles of 128 rows for 148 SMs.  Here a CTA's share of the weights can be cut at any multiple of 8
+// rows.)  The order of K is free as long as A and W agree: lane t of a row has bytes 32 t to 32 t + 31 of its column, in two
 // halves of 16 consecutive bytes, each of which feeds two multiplications, so every operand is one 16-byte load.  Half s of
 // all rows lies in the 16-byte units 2 t + s, which the 128-byte swizzle (unit ^ row % 8) puts into different banks for the
 // two rows that a quarter of a warp reads at a time.
 //
-// One bulk copy per weight row and chunk in place of the boxes reached a quarter of the bandwidth: 401 us against 125 for one
-// token of a layer that reads 704 MB; rows of A loaded into registers two chunks ahead, 459 us against YY for 32 tokens of it.
+// One bulk copy per weight row and chunk in place of the boxes reached a quarter of the bandwidth: 401 us against 115 for one
+// token of a layer that reads 704 MB.
 #pragma once
 #include <atomic>
 #include <cstdint>
@@ -35,7 +36,7 @@ namespace few {
 
 constexpr int kChunk = 512;               // bytes of a row per stage
 constexpr int kCols = 4;                  // columns of 128 bytes in it
-constexpr int kWarps = 8;                 // consumer warps: kCols x 2
+constexpr int kWarps = 2 * kCols;         // consumer warps
 constexpr int kThreads = (kWarps + 2) * 32;         // and two producers, one for the weights and one for the rows of A
 constexpr int kMaxRows = RBV_FEW_ROWS;    // rows of A
 constexpr int kMaxTile = 64;              // weight rows of a piece
@@ -223,114 +224,122 @@ __device__ __forceinline__ uint32_t group_offset(int rows, int g, int j) {
   return (uint32_t)(at * kChunk + j * n * 128 + (g * 8 - at) * 128);
 }
 
-// What the two warps of a column divide between them: the weight rows (at most 16 MT rows of A, in both), or the rows of A
-// (HALVES: 32 of at most 64 each; the accumulators of 64 by 64 would not fit a warp's registers).
-template <int MT_, bool HALVES_>
-struct Spread {
-  static constexpr int MT = MT_;
-  static constexpr bool HALVES = HALVES_;
-  static constexpr int SETS = HALVES ? 2 : 1;
-  static constexpr int GROUPS = HALVES ? kMaxTile / 8 : kMaxTile / 16;      // groups of 8 weight rows of a warp, at most
-  // row of A of tile m, upper or lower half h of a warp in part q
-  __device__ static __forceinline__ int row(int m, int q, int h, int lane) { return 16 * (m + q * MT) + 8 * h + (lane >> 2); }
-  __device__ static __forceinline__ int set(int part) { return HALVES ? part : 0; }
-  __device__ static __forceinline__ int group0(int part, int groups) { return HALVES ? 0 : part * ((groups + 1) / 2); }
-  __device__ static __forceinline__ int my_groups(int part, int groups) {
-    return HALVES ? groups : part ? groups - (groups + 1) / 2 : (groups + 1) / 2;
+// A warp's rows of A are NT tiles of 8, its weight rows up to two groups of 16.
+constexpr int kGroups = kMaxTile / 32;
+// The groups of 16 of `rows` weight rows that a part (0 or 1) takes.
+struct Share {
+  int first, count;                        // groups of 16
+  __device__ __forceinline__ Share(int rows, int part) {
+    const int all = (rows + 15) / 16, half = (all + 1) / 2;
+    first = part ? half : 0;
+    count = part ? all - half : half;
+  }
+};
+// Where the halves of its groups are in a stage of `rows` weight rows, column j; negative: there is none.
+struct Offsets {
+  int at[kGroups][2];
+  __device__ __forceinline__ Offsets(int rows, const Share& share, int j) {
+    #pragma unroll
+    for (int n = 0; n < kGroups; n++)
+      #pragma unroll
+      for (int h = 0; h < 2; h++) {
+        const int g = 2 * (share.first + n) + h;
+        at[n][h] = n < share.count && g * 8 < rows ? (int)group_offset(rows, g, j) : -1;
+      }
   }
 };
 
-// A lane's part of the rows of A for one chunk: 32 bytes of each of its rows, zeros for rows that do not exist.
-template <typename S>
+// A lane's part of the rows of A for one chunk: 32 bytes of row 8 i + lane / 4 of each tile i, zeros for rows that do not exist.
+template <int NT>
 struct Rows {
-  uint4 v[S::MT][2][2];                    // tile, half of the tile, half of the 32 bytes
+  uint4 v[NT][2];                          // tile, half of the 32 bytes
   // from a box of a stage; `at`: rows of it, negative for those that do not exist
-  __device__ __forceinline__ void load(const int (&at)[S::MT][2], uint32_t box, int rows, int col, int lane) {
+  __device__ __forceinline__ void load(const int (&at)[NT], uint32_t box, int rows, int col, int lane) {
     const uint32_t base = box + (uint32_t)(col * rows * 128), t = (uint32_t)lane & 3;
     #pragma unroll
-    for (int m = 0; m < S::MT; m++)
+    for (int i = 0; i < NT; i++)
       #pragma unroll
-      for (int h = 0; h < 2; h++)
-        #pragma unroll
-        for (int s = 0; s < 2; s++) {
-          v[m][h][s] = make_uint4(0u, 0u, 0u, 0u);
-          if (at[m][h] >= 0) v[m][h][s] = lds16(base + (uint32_t)at[m][h] * 128u + (((2u * t + s) ^ ((uint32_t)at[m][h] & 7u)) << 4));
-        }
+      for (int s = 0; s < 2; s++) {
+        v[i][s] = make_uint4(0u, 0u, 0u, 0u);
+        if (at[i] >= 0) v[i][s] = lds16(base + (uint32_t)at[i] * 128u + (((2u * t + s) ^ ((uint32_t)at[i] & 7u)) << 4));
+      }
   }
 };
 
-template <typename S, typename Acc>
-__device__ __forceinline__ void clear(Acc (&acc)[S::MT][S::GROUPS][4]) {
+template <typename Acc, int NT>
+__device__ __forceinline__ void clear(Acc (&acc)[kGroups][NT][4]) {
   #pragma unroll
-  for (int m = 0; m < S::MT; m++)
+  for (int n = 0; n < kGroups; n++)
     #pragma unroll
-    for (int n = 0; n < S::GROUPS; n++)
+    for (int i = 0; i < NT; i++)
       #pragma unroll
-      for (int k = 0; k < 4; k++) acc[m][n][k] = 0;
+      for (int k = 0; k < 4; k++) acc[n][i][k] = 0;
 }
 
-// One stage's part of a warp: G groups of 8 weight rows, the n-th at w + off[n].  Groups from `groups` on do not exist and are
-// multiplied as zeros: without branches all loads are on their way before the first multiplication and the chains of
-// different groups overlap.
-template <typename S, int G, typename Acc>
-__device__ __forceinline__ void multiply(Acc (&acc)[S::MT][S::GROUPS][4], uint32_t w, const uint32_t (&off)[S::GROUPS], int groups,
-                                         const Rows<S>& a, int lane) {
+// One stage's part of a warp: G of its groups, at w + off.  Halves that do not exist are multiplied as zeros: without branches
+// all loads are on their way before the first multiplication and the chains of different tiles overlap.
+template <int G, int NT, typename Acc>
+__device__ __forceinline__ void multiply(Acc (&acc)[kGroups][NT][4], uint32_t w, const Offsets& off, const Rows<NT>& a, int lane) {
   const uint32_t row = (uint32_t)lane >> 2, t = (uint32_t)lane & 3;
   const uint32_t wl = w + row * 128u;
-  constexpr int AT_ONCE = G < 4 ? G : 4;
   #pragma unroll
-  for (int q = 0; q < G; q += AT_ONCE)
+  for (int s = 0; s < 2; s++) {
+    uint4 b[G][2];
     #pragma unroll
-    for (int s = 0; s < 2; s++) {
-      uint4 b[AT_ONCE];
+    for (int n = 0; n < G; n++)
       #pragma unroll
-      for (int n = 0; n < AT_ONCE; n++) {
-        b[n] = make_uint4(0u, 0u, 0u, 0u);
-        if (q + n < groups) b[n] = lds16(wl + off[q + n] + (((2u * t + s) ^ row) << 4));
+      for (int h = 0; h < 2; h++) {
+        b[n][h] = make_uint4(0u, 0u, 0u, 0u);
+        if (off.at[n][h] >= 0) b[n][h] = lds16(wl + (uint32_t)off.at[n][h] + (((2u * t + s) ^ row) << 4));
       }
+    #pragma unroll
+    for (int half = 0; half < 2; half++)
       #pragma unroll
-      for (int half = 0; half < 2; half++)
+      for (int i = 0; i < NT; i++)
         #pragma unroll
-        for (int m = 0; m < S::MT; m++)
-          #pragma unroll
-          for (int n = 0; n < AT_ONCE; n++) {
-            const uint4 &lo = a.v[m][0][s], &hi = a.v[m][1][s];
-            if (half == 0) mma(acc[m][q + n], lo.x, hi.x, lo.y, hi.y, b[n].x, b[n].y);
-            else mma(acc[m][q + n], lo.z, hi.z, lo.w, hi.w, b[n].z, b[n].w);
-          }
-    }
+        for (int n = 0; n < G; n++) {
+          if (half == 0) mma(acc[n][i], b[n][0].x, b[n][1].x, b[n][0].y, b[n][1].y, a.v[i][s].x, a.v[i][s].y);
+          else mma(acc[n][i], b[n][0].z, b[n][1].z, b[n][0].w, b[n][1].w, a.v[i][s].z, a.v[i][s].w);
+        }
+  }
 }
 
 // Adds the sums of a part's four columns and hands them out: put(row of A, weight row of the piece, sums of that weight row and
-// the next one).  The parts do not wait for one another.
-template <typename S, typename Acc, typename Put>
-__device__ __forceinline__ void add_columns(const Acc (&acc)[S::MT][S::GROUPS][4], uint4* red, int g0, int groups, int part, int col,
-                                            int lane, Put&& put) {
+// the next one; even weight rows).  Four tiles of 16 x 8 at a time, one per warp.  The parts do not wait for one another.
+template <int NT, typename Acc, typename Put>
+__device__ __forceinline__ void add_columns(const Acc (&acc)[kGroups][NT][4], uint4* red, const Share& share, int part, int col, int lane,
+                                            Put&& put) {
   uint4* mine = red + part * (4 * kCols * 32);
+  const int g = lane >> 2, t = lane & 3;
+  const bool odd = (g & 1) != 0;
+  const int tiles = share.count * NT;
   #pragma unroll
-  for (int m = 0; m < S::MT; m++)
+  for (int first = 0; first < kGroups * NT; first += 4) {
+    if (first >= tiles) break;
     #pragma unroll
-    for (int n = 0; n < S::GROUPS; n += 4) {
-      if (n >= groups) break;
+    for (int k = 0; k < 4; k++)            // (tile first + k: group / NT, tile of rows % NT)
+      if (first + k < kGroups * NT)
+        mine[(k * kCols + col) * 32 + lane] = *reinterpret_cast<const uint4*>(acc[(first + k) / NT][(first + k) % NT]);
+    part_sync(part);
+    const int tile = first + col;
+    if (tile < tiles) {
+      Acc v[4] = {0, 0, 0, 0};             // weight rows g, g and g + 8, g + 8; rows of A 2 t, 2 t + 1 and again
       #pragma unroll
-      for (int i = 0; i < 4; i++) mine[(i * kCols + col) * 32 + lane] = *reinterpret_cast<const uint4*>(acc[m][n + i]);
-      part_sync(part);
-      if (n + col < groups) {              // warp `col` adds the columns of group n + col
-        Acc v[4] = {0, 0, 0, 0};
-        #pragma unroll
-        for (int j = 0; j < kCols; j++) {
-          const uint4 u = mine[(col * kCols + j) * 32 + lane];
-          v[0] += *reinterpret_cast<const Acc*>(&u.x);
-          v[1] += *reinterpret_cast<const Acc*>(&u.y);
-          v[2] += *reinterpret_cast<const Acc*>(&u.z);
-          v[3] += *reinterpret_cast<const Acc*>(&u.w);
-        }
-        #pragma unroll
-        for (int h = 0; h < 2; h++)
-          put(S::row(m, S::set(part), h, lane), (g0 + n + col) * 8 + (lane & 3) * 2, v[2 * h], v[2 * h + 1]);
+      for (int j = 0; j < kCols; j++) {
+        const uint4 u = mine[(col * kCols + j) * 32 + lane];
+        v[0] += *reinterpret_cast<const Acc*>(&u.x);
+        v[1] += *reinterpret_cast<const Acc*>(&u.y);
+        v[2] += *reinterpret_cast<const Acc*>(&u.z);
+        v[3] += *reinterpret_cast<const Acc*>(&u.w);
       }
-      part_sync(part);
+      #pragma unroll
+      for (int h = 0; h < 2; h++) {        // neighbouring weight rows are in lanes 4 apart: each lane gets both for one row of A
+        const Acc got = __shfl_xor_sync(0xffffffffu, odd ? v[2 * h] : v[2 * h + 1], 4);
+        put(8 * (tile % NT) + 2 * t + (odd ? 1 : 0), 16 * (share.first + tile / NT) + 8 * h + (g & ~1), odd ? got : v[2 * h], odd ? v[2 * h + 1] : got);
+      }
     }
+    part_sync(part);
+  }
 }
 
 // ---- work split along K over CTAs ------------------------------------------------------------------------------------

@@ -61,14 +61,13 @@ struct LinearWalk {
   }
 };
 
-// MAX: rows of A at most, 16, 32 or 64.
-template <int MAX>
+// NT: tiles of 8 rows of A.
+template <int NT>
 __global__ void __launch_bounds__(kThreads, 1) linear_int8_few_kernel(const __grid_constant__ WeightMaps maps, const __grid_constant__ WeightMaps q_maps,
                                                                       const __grid_constant__ LinearArgs a) {
   extern __shared__ uint8_t dyn[];
   __shared__ Ring ring;
   __shared__ int flag[2];
-  using S = Spread<(MAX > 16 ? 2 : 1), (MAX > 32)>;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(dyn) + 1023) & ~uintptr_t(1023));
   uint4* red = reinterpret_cast<uint4*>(base);
@@ -91,15 +90,10 @@ __global__ void __launch_bounds__(kThreads, 1) linear_int8_few_kernel(const __gr
     return;
   }
   pdl_wait();
-  int rows_at[S::MT][2];
+  int rows_at[NT];
   const int part = warp >> 2, col = warp & 3;
   #pragma unroll
-  for (int m = 0; m < S::MT; m++)
-    #pragma unroll
-    for (int h = 0; h < 2; h++) {
-      const int r = S::row(m, S::set(part), h, lane);
-      rows_at[m][h] = r < a.M ? r : -1;
-    }
+  for (int i = 0; i < NT; i++) rows_at[i] = 8 * i + (lane >> 2) < a.M ? 8 * i + (lane >> 2) : -1;
   auto result = [&](int r, int n, int v0, int v1) {
     const float s = __ldcg(a.row_scale + r);
     const float2 c = *reinterpret_cast<const float2*>(a.col_scale + n);
@@ -107,34 +101,31 @@ __global__ void __launch_bounds__(kThreads, 1) linear_int8_few_kernel(const __gr
   };
   int cut[2] = {-1, -1};                  // tiles shared with the CTA before and the CTA behind
   while (walk.next(p)) {
-    const int col0 = p.tile * a.tile, nr = min(a.tile, a.N - col0), groups = nr / 8;
-    const int g0 = S::group0(part, groups), mine = S::my_groups(part, groups);
-    uint32_t off[S::GROUPS];
-    #pragma unroll
-    for (int n = 0; n < S::GROUPS; n++) off[n] = group_offset(nr, g0 + n, col);
-    int acc[S::MT][S::GROUPS][4];
-    clear<S>(acc);
+    const int col0 = p.tile * a.tile, nr = min(a.tile, a.N - col0);
+    const Share share(nr, part);
+    const Offsets off(nr, share, col);
+    int acc[kGroups][NT][4];
+    clear(acc);
     auto run = [&](auto tag) {
       constexpr int G = decltype(tag)::value;
       #pragma unroll 1
       for (int c = p.c0; c < p.c1; c++) {
         cur.wait_full();
         __syncwarp();
-        Rows<S> rows;
+        Rows<NT> rows;
         rows.load(rows_at, cur.slot + (uint32_t)a.tile * kChunk, a.box, col, lane);
-        multiply<S, G>(acc, cur.slot, off, mine, rows, lane);
+        multiply<G>(acc, cur.slot, off, rows, lane);
         __syncwarp();
         if (lane == 0) cur.release();
         cur.next();
       }
     };
-    if (MAX == 16 && groups <= 2) run(std::integral_constant<int, 1>());
-    else if (MAX == 16 && groups <= 4) run(std::integral_constant<int, 2>());
-    else run(std::integral_constant<int, S::GROUPS>());
+    if (share.count <= 1) run(std::integral_constant<int, 1>());
+    else run(std::integral_constant<int, kGroups>());
     const bool starts = p.c0 == 0, whole = starts && p.c1 == walk.chunks;
     int* sums = a.partial + (2ll * blockIdx.x + (starts ? 1 : 0)) * a.M * a.tile;
-    add_columns<S>(acc, red, g0, mine, part, col, lane, [&](int r, int n, int v0, int v1) {
-      if (r >= a.M) return;
+    add_columns<NT>(acc, red, share, part, col, lane, [&](int r, int n, int v0, int v1) {
+      if (r >= a.M || n >= nr) return;
       if (whole) result(r, col0 + n, v0, v1);
       else *reinterpret_cast<int2*>(sums + r * a.tile + n) = make_int2(v0, v1);
     });
@@ -197,7 +188,7 @@ bool linear_plan(int M, int N, int K, LinearPlan* p) {
   return true;
 }
 
-template <int MAX>
+template <int NT>
 cudaError_t linear_launch(const LinearArgs& args, const int8_t* q, const void* w, const LinearPlan& p, cudaStream_t st) {
   LinearArgs a = args;
   WeightMaps maps, q_maps;
@@ -209,8 +200,8 @@ cudaError_t linear_launch(const LinearArgs& args, const int8_t* q, const void* w
   a.box = box_rows(a.M);
   a.stages = ring_stages(a.tile, a.box, sizeof(Ring) + 64);
   const size_t smem = ring_smem(a.tile, a.box, a.stages);
-  const cudaError_t e = allow_smem_once<linear_int8_few_kernel<MAX>>(sizeof(Ring) + 64);
-  return e != cudaSuccess ? e : launch_dependent(linear_int8_few_kernel<MAX>, dim3(p.sms), dim3(kThreads), smem, st, maps, q_maps, a);
+  const cudaError_t e = allow_smem_once<linear_int8_few_kernel<NT>>(sizeof(Ring) + 64);
+  return e != cudaSuccess ? e : launch_dependent(linear_int8_few_kernel<NT>, dim3(p.sms), dim3(kThreads), smem, st, maps, q_maps, a);
 }
 
 }  // namespace
@@ -243,7 +234,8 @@ extern "C" int rbv_linear_int8_few(const void* x, long long ldx, int M, const vo
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   const cudaError_t e = launch_quantize_rows_int8(x, M, nullptr, K, ldx, q, scale, a.counters, (int)(p.counter_bytes / 4), st);
   if (e != cudaSuccess) return (int)e;
-  if (M <= 16) return (int)linear_launch<16>(a, q, w, p, st);
-  if (M <= 32) return (int)linear_launch<32>(a, q, w, p, st);
-  return (int)linear_launch<64>(a, q, w, p, st);
+  if (M <= 8) return (int)linear_launch<1>(a, q, w, p, st);
+  if (M <= 16) return (int)linear_launch<2>(a, q, w, p, st);
+  if (M <= 32) return (int)linear_launch<4>(a, q, w, p, st);
+  return (int)linear_launch<8>(a, q, w, p, st);
 }

@@ -227,45 +227,57 @@ struct UpWalk {
   }
 };
 
-template <typename S, int MAX>
-__device__ __forceinline__ void up_piece(const FewArgs& a, Shared<MAX>& s, uint4* red, Cursor& cur, const UpPiece& p, int warp, int lane) {
-  const int R = s.choice.rows[p.u], groups = p.rows / 8, box = MAX == 16 ? a.box : box_rows(R), part = warp >> 2, col = warp & 3;
-  const int g0 = S::group0(part, groups), mine = S::my_groups(part, groups);
-  const int chunks = (2 * a.H + kChunk - 1) / kChunk;
-  uint32_t off[S::GROUPS];
-  #pragma unroll
-  for (int n = 0; n < S::GROUPS; n++) off[n] = group_offset(p.rows, g0 + n, col);
-  int rows_at[S::MT][2];
-  #pragma unroll
-  for (int m = 0; m < S::MT; m++)
-    #pragma unroll
-    for (int h = 0; h < 2; h++) {
-      const int r = S::row(m, S::set(part), h, lane);
-      rows_at[m][h] = r >= R ? -1 : MAX == 16 ? s.choice.list[s.choice.start[p.u] + r] / a.top_k : r;
-    }
-  float acc[S::MT][S::GROUPS][4];
-  clear<S>(acc);
+// The steps along K of a piece: NT tiles of 8 rows of A, at `rows_at` of a box of `box` rows.
+template <int NT>
+__device__ __forceinline__ void run_steps(float (&acc)[kGroups][NT][4], Cursor& cur, int steps, int tile, int box, const int (&rows_at)[NT],
+                                          const Offsets& off, const Share& share, int col, int lane) {
   auto run = [&](auto tag) {
     constexpr int G = decltype(tag)::value;
     #pragma unroll 1
-    for (int c = 0; c < chunks; c++) {
+    for (int c = 0; c < steps; c++) {
       cur.wait_full();
       __syncwarp();
-      Rows<S> rows;
-      rows.load(rows_at, cur.slot + (uint32_t)a.tile * kChunk, box, col, lane);
-      multiply<S, G>(acc, cur.slot, off, mine, rows, lane);
+      Rows<NT> rows;
+      rows.load(rows_at, cur.slot + (uint32_t)tile * kChunk, box, col, lane);
+      multiply<G>(acc, cur.slot, off, rows, lane);
       __syncwarp();
       if (lane == 0) cur.release();
       cur.next();
     }
   };
-  if (S::GROUPS == 4 && S::MT == 1 && groups <= 4) run(std::integral_constant<int, 2>());
-  else run(std::integral_constant<int, S::GROUPS>());
-  add_columns<S>(acc, red, g0, mine, part, col, lane, [&](int r, int row, float gate, float up) {
-    if (r >= R) return;
-    const int i = s.choice.start[p.u] + r;
-    const float y = s.choice.weight[s.choice.list[i]] * (gate / (1.0f + __expf(-gate)) * up);
-    a.h[(long long)i * a.I + (p.row0 + row) / 2] = __float2bfloat16_rn(y);
+  if (share.count <= 1) run(std::integral_constant<int, 1>());
+  else run(std::integral_constant<int, kGroups>());
+}
+
+// f(tag of the tiles of 8) for R rows, at most MAX.
+template <int MAX, typename F>
+__device__ __forceinline__ void by_tiles(int R, F&& f) {
+  if (R <= 8) f(std::integral_constant<int, 1>());
+  else if (MAX <= 16 || R <= 16) f(std::integral_constant<int, 2>());
+  else if (R <= 24) f(std::integral_constant<int, 3>());
+  else if (MAX <= 32 || R <= 32) f(std::integral_constant<int, 4>());
+  else f(std::integral_constant<int, 8>());
+}
+
+template <int NT, int MAX>
+__device__ __forceinline__ void up_piece(const FewArgs& a, Shared<MAX>& s, uint4* red, Cursor& cur, const UpPiece& p, int warp, int lane) {
+  const int R = s.choice.rows[p.u], box = MAX == 16 ? a.box : box_rows(R), part = warp >> 2, col = warp & 3;
+  const Share share(p.rows, part);
+  const Offsets off(p.rows, share, col);
+  const short* list = s.choice.list + s.choice.start[p.u];
+  int rows_at[NT];
+  #pragma unroll
+  for (int i = 0; i < NT; i++) {
+    const int r = 8 * i + (lane >> 2);
+    rows_at[i] = r >= R ? -1 : MAX == 16 ? list[r] / a.top_k : r;
+  }
+  float acc[kGroups][NT][4];
+  clear(acc);
+  run_steps<NT>(acc, cur, (2 * a.H + kChunk - 1) / kChunk, a.tile, box, rows_at, off, share, col, lane);
+  add_columns<NT>(acc, red, share, part, col, lane, [&](int r, int row, float gate, float up) {
+    if (r >= R || row >= p.rows) return;
+    const float y = s.choice.weight[list[r]] * (gate / (1.0f + __expf(-gate)) * up);
+    a.h[(long long)(s.choice.start[p.u] + r) * a.I + (p.row0 + row) / 2] = __float2bfloat16_rn(y);
   });
 }
 
@@ -315,12 +327,8 @@ __global__ void __launch_bounds__(kThreads, 1) moe_few_up_kernel(const __grid_co
     }
     return;
   }
-  while (walk.next(p)) {
-    const int R = s.choice.rows[p.u];
-    if (MAX == 16 || R <= 16) up_piece<Spread<1, false>>(a, s, red, cur, p, warp, lane);
-    else if (MAX == 32 || R <= 32) up_piece<Spread<2, false>>(a, s, red, cur, p, warp, lane);
-    else up_piece<Spread<2, true>>(a, s, red, cur, p, warp, lane);
-  }
+  while (walk.next(p))
+    by_tiles<MAX>(s.choice.rows[p.u], [&](auto tag) { up_piece<decltype(tag)::value>(a, s, red, cur, p, warp, lane); });
   if (!cur.ok && a.error) atomicExch(a.error, 1);
 }
 
@@ -362,45 +370,31 @@ struct DownWalk {
 
 // More than 16 tokens: an expert's rows by themselves, as in the up product; their sums over the expert's K are added to the
 // tokens' sums in shared memory, expert by expert.
-template <typename S, int MAX>
-__device__ __forceinline__ void down_piece(const FewArgs& a, Shared<MAX>& s, uint4* red, float* sums, Cursor& cur, const DownPiece& p, int groups,
+template <int NT, int MAX>
+__device__ __forceinline__ void down_piece(const FewArgs& a, Shared<MAX>& s, uint4* red, float* sums, Cursor& cur, const DownPiece& p, int nr,
                                            int warp, int lane) {
-  const int R = s.choice.rows[p.u], box = box_rows(R), part = warp >> 2, col = warp & 3;
-  const int g0 = S::group0(part, groups), mine = S::my_groups(part, groups);
-  uint32_t off[S::GROUPS];
+  const int R = s.choice.rows[p.u], part = warp >> 2, col = warp & 3;
+  const Share share(nr, part);
+  const Offsets off(nr, share, col);
+  int rows_at[NT];
   #pragma unroll
-  for (int n = 0; n < S::GROUPS; n++) off[n] = group_offset(groups * 8, g0 + n, col);
-  int rows_at[S::MT][2];
-  #pragma unroll
-  for (int m = 0; m < S::MT; m++)
-    #pragma unroll
-    for (int h = 0; h < 2; h++) {
-      const int r = S::row(m, S::set(part), h, lane);
-      rows_at[m][h] = r < R ? r : -1;
-    }
-  float acc[S::MT][S::GROUPS][4];
-  clear<S>(acc);
-  #pragma unroll 1
-  for (int c = p.c0; c < p.c1; c++) {
-    cur.wait_full();
-    __syncwarp();
-    Rows<S> rows;
-    rows.load(rows_at, cur.slot + (uint32_t)a.tile * kChunk, box, col, lane);
-    multiply<S, S::GROUPS>(acc, cur.slot, off, mine, rows, lane);
-    __syncwarp();
-    if (lane == 0) cur.release();
-    cur.next();
+  for (int i = 0; i < NT; i++) {
+    const int r = 8 * i + (lane >> 2);
+    rows_at[i] = r < R ? r : -1;
   }
+  float acc[kGroups][NT][4];
+  clear(acc);
+  run_steps<NT>(acc, cur, p.c1 - p.c0, a.tile, box_rows(R), rows_at, off, share, col, lane);
   const short* list = s.choice.list + s.choice.start[p.u];
-  add_columns<S>(acc, red, g0, mine, part, col, lane, [&](int r, int n, float v0, float v1) {
-    if (r >= R) return;
+  add_columns<NT>(acc, red, share, part, col, lane, [&](int r, int n, float v0, float v1) {
+    if (r >= R || n >= nr) return;
     float2* at = reinterpret_cast<float2*>(sums + list[r] / a.top_k * kMaxTile + n);
     float2 v = *at;
     v.x += v0;
     v.y += v1;
     *at = v;
   });
-  consumers_sync();                       // the next piece may divide rows and columns among the warps in another way
+  consumers_sync();                       // other warps may have these sums in the next piece
 }
 
 template <int MAX>
@@ -408,7 +402,6 @@ __global__ void __launch_bounds__(kThreads, 1) moe_few_down_kernel(const __grid_
                                                                    const __grid_constant__ FewArgs a) {
   extern __shared__ uint8_t dyn[];
   __shared__ Shared<MAX> s;
-  using S = Spread<1, false>;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   uint8_t* base = aligned_smem(dyn);
   uint4* red = reinterpret_cast<uint4*>(base);
@@ -448,7 +441,7 @@ __global__ void __launch_bounds__(kThreads, 1) moe_few_down_kernel(const __grid_
   const int part = warp >> 2, wcol = warp & 3;
   bool more = walk.next(p);
   while (more) {
-    const int tile = p.tile, col0 = tile * a.tile, nr = min(a.tile, a.H - col0), groups = nr / 8;
+    const int tile = p.tile, col0 = tile * a.tile, nr = min(a.tile, a.H - col0);
     const bool starts = p.u == 0 && p.c0 == 0;
     bool ends;
     // a tile cut by the end of a range: the sums go to the workspace, for the last CTA to arrive
@@ -460,55 +453,39 @@ __global__ void __launch_bounds__(kThreads, 1) moe_few_down_kernel(const __grid_
     bool whole;
     if constexpr (MAX == 16) {
       // all tokens at once, those that did not choose an expert as zeros: its sums stay in the accumulators
-      const int g0 = S::group0(part, groups), mine = S::my_groups(part, groups);
-      uint32_t off[S::GROUPS];
-      #pragma unroll
-      for (int n = 0; n < S::GROUPS; n++) off[n] = group_offset(nr, g0 + n, wcol);
-      float acc[S::MT][S::GROUPS][4];
-      clear<S>(acc);
-      do {
-        const int box = box_rows(s.choice.rows[p.u]), e = s.choice.used[p.u];
-        int rows_at[1][2];
-        #pragma unroll
-        for (int h = 0; h < 2; h++) {
-          const int t = S::row(0, 0, h, lane);
-          rows_at[0][h] = -1;
-          if (t < a.T)
-            for (int j = 0; j < a.top_k; j++)
-              if (s.choice.expert[t * a.top_k + j] == e) rows_at[0][h] = s.choice.at[t * a.top_k + j];
-        }
-        auto run = [&](auto tag) {
-          constexpr int G = decltype(tag)::value;
-          #pragma unroll 1
-          for (int c = p.c0; c < p.c1; c++) {
-            cur.wait_full();
-            __syncwarp();
-            Rows<S> rows;
-            rows.load(rows_at, cur.slot + (uint32_t)a.tile * kChunk, box, wcol, lane);
-            multiply<S, G>(acc, cur.slot, off, mine, rows, lane);
-            __syncwarp();
-            if (lane == 0) cur.release();
-            cur.next();
+      const Share share(nr, part);
+      const Offsets off(nr, share, wcol);
+      auto tokens = [&](auto tag) {
+        constexpr int NT = decltype(tag)::value;
+        float acc[kGroups][NT][4];
+        clear(acc);
+        do {
+          const int e = s.choice.used[p.u];
+          int rows_at[NT];
+          #pragma unroll
+          for (int i = 0; i < NT; i++) {
+            const int t = 8 * i + (lane >> 2);
+            rows_at[i] = -1;
+            if (t < a.T)
+              for (int j = 0; j < a.top_k; j++)
+                if (s.choice.expert[t * a.top_k + j] == e) rows_at[i] = s.choice.at[t * a.top_k + j];
           }
-        };
-        if (groups <= 2) run(std::integral_constant<int, 1>());
-        else if (groups <= 4) run(std::integral_constant<int, 2>());
-        else run(std::integral_constant<int, S::GROUPS>());
-        ends = p.u == n_used - 1 && p.c1 == walk.chunks;
-        more = walk.next(p);
-      } while (more && p.tile == tile);
-      whole = starts && ends;
-      add_columns<S>(acc, red, g0, mine, part, wcol, lane, [&](int t, int col, float v0, float v1) {
-        if (t < a.T) result(whole, t, col, v0, v1);
-      });
+          run_steps<NT>(acc, cur, p.c1 - p.c0, a.tile, box_rows(s.choice.rows[p.u]), rows_at, off, share, wcol, lane);
+          ends = p.u == n_used - 1 && p.c1 == walk.chunks;
+          more = walk.next(p);
+        } while (more && p.tile == tile);
+        whole = starts && ends;
+        add_columns<NT>(acc, red, share, part, wcol, lane, [&](int t, int col, float v0, float v1) {
+          if (t < a.T && col < nr) result(whole, t, col, v0, v1);
+        });
+      };
+      if (a.T <= 8) tokens(std::integral_constant<int, 1>());
+      else tokens(std::integral_constant<int, 2>());
     } else {
       for (int i = tid; i < a.T * kMaxTile; i += kWarps * 32) sums[i] = 0.0f;
       consumers_sync();
       do {
-        const int rows = s.choice.rows[p.u];
-        if (rows <= 16) down_piece<Spread<1, false>>(a, s, red, sums, cur, p, groups, warp, lane);
-        else if (MAX == 32 || rows <= 32) down_piece<Spread<2, false>>(a, s, red, sums, cur, p, groups, warp, lane);
-        else down_piece<Spread<2, true>>(a, s, red, sums, cur, p, groups, warp, lane);
+        by_tiles<MAX>(s.choice.rows[p.u], [&](auto tag) { down_piece<decltype(tag)::value>(a, s, red, sums, cur, p, nr, warp, lane); });
         ends = p.u == n_used - 1 && p.c1 == walk.chunks;
         more = walk.next(p);
       } while (more && p.tile == tile);
