@@ -79,6 +79,16 @@ __device__ __forceinline__ void ring_init(Ring& ring, int stages, int producers)
   sm100::mbar_fence_init();
 }
 
+// The same for all stages there may be, by the first threads of a CTA that learns later how many fit.
+__device__ __forceinline__ void ring_init_all(Ring& ring, int producers) {
+  const int s = threadIdx.x;
+  if (s >= kMaxStages) return;
+  sm100::mbar_init(&ring.full[s], producers);
+  sm100::mbar_init(&ring.empty[s], kWarps);
+  if (s == 0) ring.abort = 0;
+  sm100::mbar_fence_init();
+}
+
 // A warp's place in the ring, as addresses in shared memory: a warp that works alone pays for every instruction between two
 // loads or multiplications, a stage of a small piece with as many cycles as its bytes take.
 struct Cursor {
@@ -142,16 +152,16 @@ __device__ __forceinline__ void load_column(uint32_t dst, const CUtensorMap* m, 
 }
 
 // Fetches chunks c0 to c1 - 1 of `rows` rows (a multiple of 8) from `row0` on, one per stage, `off` bytes into it: box by box, in
-// a box column by column.  Four lanes of a warp, one for each height of a box: a lane gets a box on its way in 150 cycles or
+// a box column by column.  Four lanes of a warp (others may come along), one for each height of a box: a lane gets a box on its way in 150 cycles or
 // more whatever its size, so there is one box per height and stage (with a box per column the producer set the pace, 205 us
 // against 119 for one token of a layer that reads 704 MB).  False: a wait ran out, stop.
 template <typename E>                      // element: its size turns bytes along K into coordinates
 __device__ __forceinline__ bool feed(const WeightMaps& maps, Cursor& cur, uint32_t off, int row0, int rows, int c0, int c1) {
-  const int lane = threadIdx.x & 31, height = 8 << lane;
-  const bool mine = (rows & height) != 0;
+  const int lane = threadIdx.x & 31, size = min(lane, 3), height = 8 << size;
+  const bool mine = lane < 4 && (rows & height) != 0;
   const int before = rows & ~(2 * height - 1);           // rows in larger boxes
   const uint32_t bytes = (uint32_t)rows * kChunk, to = off + (uint32_t)before * kChunk;
-  const CUtensorMap *all = &maps.all[lane], *one = &maps.one[lane];
+  const CUtensorMap *all = &maps.all[size], *one = &maps.one[size];
   int c = c0;
   #pragma unroll 1
   for (; c < c1 && c < maps.whole; c++) {

@@ -39,8 +39,8 @@ struct FewArgs {
   int* counters;                          // one per column tile of the down product
   __nv_bfloat16* out;
   int* error;
-  int tile, box, stages, whole;                 // weight rows of a piece and rows of A in a stage, at most; ring stages;
-                                          // whole: tiles of the down product are not split
+  int tile, room, whole;                  // weight rows of a piece at most; bytes of the ring; whole: tiles of the down product are
+                                          // not split
 };
 
 // The choice, as every CTA makes it.
@@ -55,8 +55,8 @@ struct Choice {
   short index[kMoeMaxExperts];            // place of an expert in `used`
   short start[kMoeMaxExperts];            // first entry of `list` of a used expert
   short rows[kMoeMaxExperts];             // rows of a used expert
-  int warp_used[8], warp_rows[8];
-  int n_used;
+  int warp_used[8], warp_rows[8], warp_most[8];
+  int n_used, most;                       // most: rows of the expert with most
 };
 
 // Larger keys for larger logits, NaN above all, equal for both zeros; kMasked and below: -inf.
@@ -148,7 +148,8 @@ __device__ __forceinline__ void choose(Choice<TOKENS>& c, const FewArgs& a) {   
         c.at[lane] = (short)at;
         c.list[start + at] = (short)lane;
       }
-      if (lane == 0) c.n_used = __popc(firsts);
+      const int most = __reduce_max_sync(0xffffffffu, e >= 0 ? n : 0);
+      if (lane == 0) { c.n_used = __popc(firsts); c.most = most; }
     }
     __syncthreads();
     return;
@@ -168,12 +169,14 @@ __device__ __forceinline__ void choose(Choice<TOKENS>& c, const FewArgs& a) {   
       const int v = __shfl_up_sync(0xffffffffu, before, o);
       if (lane >= o) before += v;
     }
-    if (lane == 31) { c.warp_used[warp] = __popc(has); c.warp_rows[warp] = before; }
+    const int warp_most = __reduce_max_sync(0xffffffffu, n);
+    if (lane == 31) { c.warp_used[warp] = __popc(has); c.warp_rows[warp] = before; c.warp_most[warp] = warp_most; }
     consumers_sync();
-    int u = __popc(has & ((1u << lane) - 1u)), r = before - n, all_used = 0;
+    int u = __popc(has & ((1u << lane) - 1u)), r = before - n, all_used = 0, most = 0;
     for (int w = 0; w < 8; w++) {
       if (w < warp) { u += c.warp_used[w]; r += c.warp_rows[w]; }
       all_used += c.warp_used[w];
+      most = max(most, c.warp_most[w]);
     }
     if (n > 0) {
       c.used[u] = (short)tid;
@@ -181,7 +184,7 @@ __device__ __forceinline__ void choose(Choice<TOKENS>& c, const FewArgs& a) {   
       c.start[u] = (short)r;
       c.rows[u] = (short)n;
     }
-    if (tid == 0) c.n_used = all_used;
+    if (tid == 0) { c.n_used = all_used; c.most = most; }
   }
   __syncthreads();
   for (int s = tid; s < slots; s += blockDim.x)
@@ -197,6 +200,12 @@ struct Shared {
 };
 __device__ __forceinline__ uint8_t* aligned_smem(uint8_t* p) {
   return reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(p) + 1023) & ~uintptr_t(1023));
+}
+
+// The ring for stages of a.tile weight rows and `box` rows of A.
+__device__ __forceinline__ Cursor ring_cursor(Ring& ring, const FewArgs& a, uint32_t at, int box) {
+  const uint32_t slot = slot_bytes(a.tile, box);
+  return Cursor(ring, at, min(kMaxStages, (int)((uint32_t)a.room / slot)), slot);
 }
 
 // ---- up: weight rows (gate and up interleaved) of the used experts, 8 at a time, split evenly among the CTAs ------------
@@ -259,9 +268,16 @@ __device__ __forceinline__ void by_tiles(int R, F&& f) {
   else f(std::integral_constant<int, 8>());
 }
 
+// Tokens of an expert with R rows come in one box of all tokens, or gathered four rows at a time.  A box of all is an
+// instruction and up to 16 KB (32 tokens) or 32 KB (64), beside 32 KB of weights; gathering takes R instructions of some 90
+// cycles each, and a stage's weights 1260.
+template <int MAX> __device__ __forceinline__ bool in_one_box(int R) { return MAX == 16 || R > (MAX == 32 ? 4 : 8); }
+template <int MAX> __device__ __forceinline__ int token_box(int T, int R) { return box_rows(in_one_box<MAX>(R) ? T : R); }
+template <int MAX> struct XMaps { WeightMaps box; CUtensorMap rows; };
+
 template <int NT, int MAX>
 __device__ __forceinline__ void up_piece(const FewArgs& a, Shared<MAX>& s, uint4* red, Cursor& cur, const UpPiece& p, int warp, int lane) {
-  const int R = s.choice.rows[p.u], box = MAX == 16 ? a.box : box_rows(R), part = warp >> 2, col = warp & 3;
+  const int R = s.choice.rows[p.u], part = warp >> 2, col = warp & 3;
   const Share share(p.rows, part);
   const Offsets off(p.rows, share, col);
   const short* list = s.choice.list + s.choice.start[p.u];
@@ -269,11 +285,11 @@ __device__ __forceinline__ void up_piece(const FewArgs& a, Shared<MAX>& s, uint4
   #pragma unroll
   for (int i = 0; i < NT; i++) {
     const int r = 8 * i + (lane >> 2);
-    rows_at[i] = r >= R ? -1 : MAX == 16 ? list[r] / a.top_k : r;
+    rows_at[i] = r >= R ? -1 : in_one_box<MAX>(R) ? list[r] / a.top_k : r;
   }
   float acc[kGroups][NT][4];
   clear(acc);
-  run_steps<NT>(acc, cur, (2 * a.H + kChunk - 1) / kChunk, a.tile, box, rows_at, off, share, col, lane);
+  run_steps<NT>(acc, cur, (2 * a.H + kChunk - 1) / kChunk, a.tile, token_box<MAX>(a.T, R), rows_at, off, share, col, lane);
   add_columns<NT>(acc, red, share, part, col, lane, [&](int r, int row, float gate, float up) {
     if (r >= R || row >= p.rows) return;
     const float y = s.choice.weight[list[r]] * (gate / (1.0f + __expf(-gate)) * up);
@@ -281,24 +297,18 @@ __device__ __forceinline__ void up_piece(const FewArgs& a, Shared<MAX>& s, uint4
   });
 }
 
-// MAX: tokens, and with them rows of an expert, at most: 16, 32 or 64.  Up to 16 tokens all of them are fetched for every expert,
-// in one box (4 or 8 KB beside up to 32 of weights); beyond that the expert's own, gathered four at a time (one token of 64
-// experts: 14.4 us gathered, 12.6 in a box; for 32 tokens a box would be half as much as the weights).
-template <int MAX> using XMap = std::conditional_t<MAX == 16, WeightMaps, CUtensorMap>;
+// MAX: tokens, and with them rows of an expert, at most: 16, 32 or 64.
 template <int MAX>
-__global__ void __launch_bounds__(kThreads, 1) moe_few_up_kernel(const __grid_constant__ WeightMaps maps, const __grid_constant__ XMap<MAX> x_map,
+__global__ void __launch_bounds__(kThreads, 1) moe_few_up_kernel(const __grid_constant__ WeightMaps maps, const __grid_constant__ XMaps<MAX> x_maps,
                                                                  const __grid_constant__ FewArgs a) {
   extern __shared__ uint8_t dyn[];
   __shared__ Shared<MAX> s;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   uint8_t* base = aligned_smem(dyn);
   uint4* red = reinterpret_cast<uint4*>(base);
-  if (threadIdx.x == 0) ring_init(s.ring, a.stages, 2);
+  ring_init_all(s.ring, 2);
   if (warp == kWarps) prefetch_maps(maps);
-  if (warp == kWarps + 1) {
-    if constexpr (MAX == 16) prefetch_maps(x_map);
-    else if (lane == 0) sm100::tma_prefetch_desc(&x_map);
-  }
+  if (warp == kWarps + 1) prefetch_maps(x_maps.box);
   pdl_wait();
   pdl_trigger();      // after the wait: the down kernel reads the logits before it waits for this one
   if (blockIdx.x == 0)
@@ -306,7 +316,7 @@ __global__ void __launch_bounds__(kThreads, 1) moe_few_up_kernel(const __grid_co
   choose(s.choice, a);
   UpWalk walk(a, s.choice.n_used);
   UpPiece p;
-  Cursor cur(s.ring, sm100::smem_u32(base + kRedBytes), a.stages, slot_bytes(a.tile, a.box));
+  Cursor cur = ring_cursor(s.ring, a, sm100::smem_u32(base + kRedBytes), token_box<MAX>(a.T, s.choice.most));
   const int chunks = (2 * a.H + kChunk - 1) / kChunk;
   if (warp == kWarps) {
     if (lane >= 4) return;
@@ -315,15 +325,12 @@ __global__ void __launch_bounds__(kThreads, 1) moe_few_up_kernel(const __grid_co
   }
   if (warp == kWarps + 1) {
     asm volatile("fence.proxy.async;" ::: "memory");
-    if constexpr (MAX == 16) {
-      if (lane >= 4) return;
-      while (walk.next(p) && feed<__nv_bfloat16>(x_map, cur, (uint32_t)a.tile * kChunk, 0, a.box, 0, chunks)) {}
-    } else {
-      while (walk.next(p)) {
-        const short* list = s.choice.list + s.choice.start[p.u];
-        if (!feed_gathered<__nv_bfloat16>(&x_map, cur, (uint32_t)a.tile * kChunk, s.choice.rows[p.u], 0, chunks,
-                                          [&](int r) { return list[r] / a.top_k; })) break;
-      }
+    bool ok = true;
+    while (ok && walk.next(p)) {
+      const int R = s.choice.rows[p.u];
+      const short* list = s.choice.list + s.choice.start[p.u];
+      if (in_one_box<MAX>(R)) ok = feed<__nv_bfloat16>(x_maps.box, cur, (uint32_t)a.tile * kChunk, 0, box_rows(a.T), 0, chunks);
+      else ok = feed_gathered<__nv_bfloat16>(&x_maps.rows, cur, (uint32_t)a.tile * kChunk, R, 0, chunks, [&](int r) { return list[r] / a.top_k; });
     }
     return;
   }
@@ -407,7 +414,7 @@ __global__ void __launch_bounds__(kThreads, 1) moe_few_down_kernel(const __grid_
   uint4* red = reinterpret_cast<uint4*>(base);
   float* sums = reinterpret_cast<float*>(base + kRedBytes);                // [MAX][kMaxTile] beyond 16 tokens
   constexpr uint32_t kSumBytes = MAX > 16 ? MAX * kMaxTile * 4 : 0;
-  if (tid == 0) ring_init(s.ring, a.stages, 2);
+  ring_init_all(s.ring, 2);
   if (warp >= kWarps) prefetch_maps(warp == kWarps ? maps : h_maps);
   pdl_trigger();
   choose(s.choice, a);
@@ -420,7 +427,7 @@ __global__ void __launch_bounds__(kThreads, 1) moe_few_down_kernel(const __grid_
   }
   DownWalk walk(a, n_used);
   DownPiece p;
-  Cursor cur(s.ring, sm100::smem_u32(base + kRedBytes + kSumBytes), a.stages, slot_bytes(a.tile, a.box));
+  Cursor cur = ring_cursor(s.ring, a, sm100::smem_u32(base + kRedBytes + kSumBytes), box_rows(s.choice.most));
   if (warp >= kWarps) {                   // the weights do not wait for the first kernel, the rows of h do
     if (lane >= 4) return;
     if (warp == kWarps) {
@@ -563,30 +570,28 @@ bool few_plan(int T, int H, int I, int E, int top_k, FewPlan* p) {
 }
 
 template <int MAX, auto* Kernel, typename... Maps>
-cudaError_t launch_ring(FewArgs a, int tile, int box, size_t sums, int sms, cudaStream_t st, const Maps&... maps) {
+cudaError_t launch_ring(FewArgs a, int tile, size_t sums, int sms, cudaStream_t st, const Maps&... maps) {
+  const size_t smem = ring_room(sizeof(Shared<MAX>));
   a.tile = tile;
-  a.box = box;
-  a.stages = ring_stages(tile, box, sizeof(Shared<MAX>) + sums);
+  a.room = (int)(smem - 1024 /*alignment*/ - kRedBytes - sums);
   const cudaError_t e = allow_smem_once<Kernel>(sizeof(Shared<MAX>));
-  return e != cudaSuccess ? e : launch_dependent(Kernel, dim3(sms), dim3(kThreads), ring_smem(tile, box, a.stages) + sums, st, maps..., a);
+  return e != cudaSuccess ? e : launch_dependent(Kernel, dim3(sms), dim3(kThreads), smem, st, maps..., a);
 }
 
 template <int MAX>
 cudaError_t few_launch(FewArgs a, const FewPlan& p, cudaStream_t st) {
   const CUtensorMapDataType bf16 = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  const unsigned long long T = a.T, E = a.E, h_row = 2ull * a.I, x_row = 2ull * a.H, x_step = (unsigned long long)a.ldx;
   WeightMaps w13, w2, h;
-  if (!weight_maps(&w13, a.w13, 2ull * a.E * a.I, 2ull * a.H, bf16, 2, heights_up_to(p.up_tile)) ||
-      !weight_maps(&w2, a.w2, (unsigned long long)a.E * a.H, 2ull * a.I, bf16, 2, p.down_tile | a.H % p.down_tile) ||
-      !weight_maps(&h, a.h, (unsigned long long)a.T * a.top_k, 2ull * a.I, bf16, 2, heights_up_to(box_rows(a.T))))
+  XMaps<MAX> x;
+  if (!weight_maps(&w13, a.w13, 2ull * E * a.I, x_row, bf16, 2, heights_up_to(p.up_tile)) ||
+      !weight_maps(&w2, a.w2, E * a.H, h_row, bf16, 2, p.down_tile | a.H % p.down_tile) ||
+      !weight_maps(&h, a.h, T * a.top_k, h_row, bf16, 2, heights_up_to(box_rows(a.T))) ||
+      !weight_maps(&x.box, a.x, T, x_row, bf16, 2, box_rows(a.T), x_step) || (MAX > 16 && !gather_map(&x.rows, a.x, T, x_row, x_step, bf16, 2)))
     return cudaErrorUnknown;
-  XMap<MAX> x;
-  bool ok;
-  if constexpr (MAX == 16) ok = weight_maps(&x, a.x, (unsigned long long)a.T, 2ull * a.H, bf16, 2, box_rows(a.T), (unsigned long long)a.ldx);
-  else ok = gather_map(&x, a.x, (unsigned long long)a.T, 2ull * a.H, (unsigned long long)a.ldx, bf16, 2);
-  if (!ok) return cudaErrorUnknown;
   a.whole = p.whole;
-  const cudaError_t e = launch_ring<MAX, moe_few_up_kernel<MAX>>(a, p.up_tile, box_rows(a.T), 0, p.sms, st, w13, x);
-  return e != cudaSuccess ? e : launch_ring<MAX, moe_few_down_kernel<MAX>>(a, p.down_tile, box_rows(a.T), MAX > 16 ? (size_t)MAX * kMaxTile * 4 : 0, p.sms, st, w2, h);
+  const cudaError_t e = launch_ring<MAX, moe_few_up_kernel<MAX>>(a, p.up_tile, 0, p.sms, st, w13, x);
+  return e != cudaSuccess ? e : launch_ring<MAX, moe_few_down_kernel<MAX>>(a, p.down_tile, MAX > 16 ? (size_t)MAX * kMaxTile * 4 : 0, p.sms, st, w2, h);
 }
 
 }  // namespace
