@@ -38,6 +38,19 @@ Tensor packed_rows(const Tensor& x, int64_t step) {
 }
 int64_t row_step(const Tensor& x) { return x.size(0) > 1 ? x.stride(0) : x.size(1); }
 
+// A kernel's error flag, if the caller wants to know.
+int* error_flag(const Maybe& error, const Tensor& like) {
+  if (!error) return nullptr;
+  TORCH_CHECK_VALUE(error->scalar_type() == at::kInt && error->numel() >= 1 && error->device() == like.device(),
+                    "error must be an int32 tensor on the same GPU");
+  return error->data_ptr<int>();
+}
+
+// The operators without a backward pass refuse inputs that want one (rather than cut the graph without a word).
+void no_gradient(const Tensor& x, const char* what) {
+  TORCH_CHECK_VALUE(!x.requires_grad() || !at::GradMode::is_enabled(), what, " has no backward pass: call it under torch.no_grad()");
+}
+
 // ---- norms around a block ----------------------------------------------------------------------------------------------
 int norm_type(at::ScalarType t) {
   return t == at::kBFloat16 ? RBV_NORM_BF16 : t == at::kHalf ? RBV_NORM_FP16 : t == at::kFloat ? RBV_NORM_FP32 : -1;
@@ -241,6 +254,7 @@ std::tuple<Tensor, Maybe> block_norm(const Tensor& residual, const Maybe& branch
 // ---- 8-bit integers ------------------------------------------------------------------------------------------------------
 Tensor int8_rows(const Tensor& x) {
   TORCH_CHECK_VALUE(x.scalar_type() == at::kBFloat16 && x.dim() == 2, "rows must be a bf16 matrix, not ", x.sizes(), " in ", x.scalar_type());
+  no_gradient(x, "quantising rows to int8");
   const int64_t K = x.size(1);
   TORCH_CHECK_VALUE(K >= 16 && K % 16 == 0 && K <= RBV_INT8_MAX_DEPTH, "depths of 16 to ", RBV_INT8_MAX_DEPTH, " in steps of 16 are supported, not ", K);
   TORCH_CHECK_VALUE(x.is_cuda(), "the rows must be on a GPU");
@@ -285,7 +299,7 @@ Tensor grouped_gemm_int8(const Tensor& Aq, const Tensor& a_scale, const Tensor& 
     TORCH_CHECK_VALUE(t->dim() == 1 && t->size(0) == G && t->scalar_type() == at::kInt && t->is_contiguous(),
                       "group_start and group_rows must be int32 [", G, "]");
   const int64_t M = Aq.size(0), n_out = swiglu ? N / 2 : N;
-  TORCH_CHECK_VALUE(M <= 0x7fffffff, "too many rows");
+  TORCH_CHECK_VALUE(M <= RBV_INT8_MAX_ROWS, "at most ", RBV_INT8_MAX_ROWS, " rows, not ", M);
   TORCH_CHECK_VALUE(Aq.is_cuda(), "all tensors must be on one GPU");
   for (const Tensor* t : {&a_scale, &Bq, &b_scale, &group_start, &group_rows})
     TORCH_CHECK_VALUE(t->device() == Aq.device(), "all tensors must be on one GPU");
@@ -300,7 +314,7 @@ Tensor grouped_gemm_int8(const Tensor& Aq, const Tensor& a_scale, const Tensor& 
   if (M)
     launched(rbv_grouped_gemm_int8(Aq.data_ptr(), a_scale.data_ptr<float>(), M, Bq.data_ptr(), b_scale.data_ptr<float>(), out.data_ptr(),
                                    group_start.data_ptr<int>(), group_rows.data_ptr<int>(), (int)G, (int)N, (int)K, (int)row_step(out), swiglu ? 1 : 0,
-                                   error ? error->data_ptr<int>() : nullptr, (int)max_ctas, stream_of(Aq)),
+                                   error_flag(error, Aq), (int)max_ctas, stream_of(Aq)),
              "int8 grouped GEMM");
   return out;
 }
@@ -311,7 +325,7 @@ Tensor linear_int8(const Tensor& rows, const Tensor& weight, const Tensor& scale
   const int64_t M = x.size(0), K = x.size(1), N = weight.size(0);
   TORCH_CHECK_VALUE(weight.size(1) == K, "rows of ", K, " do not fit weights ", weight.sizes());
   TORCH_CHECK_VALUE(weight.device() == x.device() && scale.device() == x.device(), "all tensors must be on one GPU");
-  TORCH_CHECK_VALUE(M <= 0x7fffffff, "too many rows");
+  TORCH_CHECK_VALUE(M <= RBV_INT8_MAX_ROWS, "at most ", RBV_INT8_MAX_ROWS, " rows, not ", M);
   const c10::cuda::CUDAGuard guard(x.device());
   Tensor out = value(out_);
   if (!out.defined()) out = empty({M, N}, at::kBFloat16, x);
@@ -320,7 +334,7 @@ Tensor linear_int8(const Tensor& rows, const Tensor& weight, const Tensor& scale
                           out.is_contiguous() && !misaligned(out),
                       "out must be a contiguous, 16-byte aligned bf16 tensor [", M, ", ", N, "] on the same GPU");
   if (M == 0) return out;
-  int* err = error ? error->data_ptr<int>() : nullptr;
+  int* err = error_flag(error, x);
   if (M <= RBV_FEW_ROWS) {
     Tensor ws = empty({rbv_linear_int8_few_workspace((int)M, (int)N, (int)K)}, at::kByte, x);
     launched(rbv_linear_int8_few(x.data_ptr(), row_step(x), (int)M, weight.data_ptr(), scale.data_ptr<float>(), (int)N, (int)K, out.data_ptr(),
@@ -342,6 +356,8 @@ Tensor moe_few_tokens(const Tensor& x_, const Tensor& logits_, const Tensor& w13
                       const Maybe& error) {
   TORCH_CHECK_VALUE(x_.dim() == 2 && logits_.dim() == 2 && w13.dim() == 3 && w2.dim() == 3,
                     "x [T, H], logits [T, E], w13 [E, 2 I, H] and w2 [E, H, I] are wanted");
+  no_gradient(x_, "moe_few_tokens");
+  no_gradient(logits_, "moe_few_tokens");
   const int64_t T = x_.size(0), H = x_.size(1), E = w2.size(0), I = w2.size(2);
   TORCH_CHECK_VALUE(x_.scalar_type() == at::kBFloat16 && w13.scalar_type() == at::kBFloat16 && w2.scalar_type() == at::kBFloat16 &&
                         logits_.scalar_type() == at::kFloat,
@@ -371,7 +387,7 @@ Tensor moe_few_tokens(const Tensor& x_, const Tensor& logits_, const Tensor& w13
   TORCH_CHECK_VALUE(bytes >= 0, "a layer of ", E, " experts, hidden ", H, " and FFN width ", I, " is too large");
   Tensor ws = empty({bytes}, at::kByte, x);
   launched(rbv_moe_few_tokens(x.data_ptr(), row_step(x), logits.data_ptr<float>(), row_step(logits), (int)T, (int)H, (int)I, (int)E, (int)top_k,
-                              w13.data_ptr(), w2.data_ptr(), out.data_ptr(), ws.data_ptr(), error ? error->data_ptr<int>() : nullptr, stream_of(x)),
+                              w13.data_ptr(), w2.data_ptr(), out.data_ptr(), ws.data_ptr(), error_flag(error, x), stream_of(x)),
            "few-token MoE");
   return out;
 }

@@ -139,7 +139,8 @@ grouped_gemm_int8_kernel(const __grid_constant__ I8Maps maps, const __grid_const
   pdl_wait();
   for (int i = tid; i < p.G; i += blockDim.x) {
     s_start[i] = p.group_start ? p.group_start[i] : 0;
-    s_rows[i] = p.group_rows ? rows_inside(p.group_rows[i], s_start[i], p.a_rows, p.error) : (int)p.a_rows;
+    s_rows[i] = p.group_rows ? rows_inside(s_start[i] < 0 ? 0 : p.group_rows[i], s_start[i], p.a_rows, p.error) : (int)p.a_rows;
+    if (s_start[i] < 0 && p.error && blockIdx.x == 0) atomicCAS(p.error, 0, 6);
     atomicMax(&s_most, s_rows[i]);
   }
   tc_fence_before_sync();
@@ -297,7 +298,7 @@ extern "C" int rbv_grouped_gemm_int8(const void* A, const float* a_scale, long l
                                      void* C, const int* group_start, const int* group_rows, int G, int N, int K, int ldc,
                                      int epilogue, int* error_flag, int max_ctas, void* cuda_stream) {
   using namespace rbv;
-  if (G < 1 || G > kMoeMaxGroups || N < 8 || N % 8 || K < 16 || K % 16 || K > RBV_INT8_MAX_DEPTH || a_rows < 1 || a_rows > 0x7fffffffll ||
+  if (G < 1 || G > kMoeMaxGroups || N < 8 || N % 8 || K < 16 || K % 16 || K > RBV_INT8_MAX_DEPTH || a_rows < 1 || a_rows > RBV_INT8_MAX_ROWS ||
       ldc % 2 || (long long)G * N > 0x7fffffffll || epilogue < 0 || epilogue > 1)
     return (int)cudaErrorInvalidValue;
   if ((!group_start) != (!group_rows) || (!group_start && G != 1)) return (int)cudaErrorInvalidValue;

@@ -184,6 +184,14 @@ def test_groups_beyond_the_rows_are_left_out():
     out = grouped_gemm_int8(q, s, w, c, gs, gr, error=err)
     _check(out[30:], _want(q[30:], s[30:], w[1], c[1]))
     assert err.item() == 6
+    err.zero_()
+    out = torch.full((40, 64), 7.0, dtype=BF, device="cuda")
+    grouped_gemm_int8(q, s, w, c, torch.tensor([-5, 20], dtype=I32, device="cuda"), torch.tensor([10, 20], dtype=I32, device="cuda"),
+                      out=out, error=err)
+    assert err.item() == 6 and (out[:20] == 7).all()
+    _check(out[20:], _want(q[20:], s[20:], w[1], c[1]))
+    with pytest.raises(ValueError, match="error must be"):
+        grouped_gemm_int8(q, s, w, c, gs, gr, error=torch.zeros(1, dtype=I32))
 
 
 def test_streams_and_graphs():

@@ -23,6 +23,7 @@ def _linear(M=3, N=16, K=32):
     (dict(scale=torch.ones(16, dtype=BF)), "one fp32 scale per channel"),
     (dict(weight=torch.zeros(32, 16, dtype=I8).t()), "contiguous"),
     (dict(weight=torch.zeros(16 * 32 + 1, dtype=I8)[1:].view(16, 32)), "16-byte aligned"),
+    (dict(x=torch.zeros(3, 32, dtype=BF, requires_grad=True)), "no backward pass"),
     (dict(), "on a GPU"),
 ])
 def test_linear_refusals(change, words):

@@ -88,6 +88,20 @@ def test_masked_experts_and_empty_rows():
     assert (got == 0).all()
 
 
+def test_infinite_logits_and_results_in_place():
+    from rbruck_alltoallv_b200.ops.moe import moe_few_tokens
+    x, logits, w13, w2 = _make(18, 64, 40, 6)
+    want = moe_few_tokens(x, logits, w13, w2)
+    logits[4, 2] = math.inf
+    got = moe_few_tokens(x, logits, w13, w2)
+    others = [t for t in range(18) if t != 4]
+    assert got[4].isnan().all() and torch.equal(got[others], want[others])
+    y = x.clone()
+    assert moe_few_tokens(y, logits, w13, w2, out=y) is not None and torch.equal(y[others], want[others])
+    with pytest.raises(ValueError, match="error must be"):
+        moe_few_tokens(x, logits, w13, w2, error=torch.zeros(1, dtype=torch.int32))
+
+
 def test_a_bad_token_stays_alone():
     from rbruck_alltoallv_b200.ops.moe import moe_few_tokens
     x, logits, w13, w2 = _make(24, 256, 128, 4)

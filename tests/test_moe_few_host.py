@@ -28,6 +28,8 @@ def _args(T=3, H=16, I=24, E=4):
     ({**_args(E=16), "top_k": 9}, "top_k"),
     (dict(w2=torch.zeros(4, 24, 16, dtype=BF).transpose(1, 2)), "contiguous"),
     (dict(w13=torch.zeros(4 * 48 * 16 + 1, dtype=BF)[1:].view(4, 48, 16)), "16-byte aligned"),
+    (dict(x=torch.zeros(3, 16, dtype=BF, requires_grad=True)), "no backward pass"),
+    (dict(logits=torch.zeros(3, 4, requires_grad=True)), "no backward pass"),
     (dict(), "on one GPU"),
 ])
 def test_refusals(change, words):
