@@ -22,6 +22,7 @@
 // One bulk copy per weight row and chunk in place of the boxes reached a quarter of the bandwidth: 401 us against 115 for one
 // token of a layer that reads 704 MB.
 #pragma once
+#include <algorithm>
 #include <atomic>
 #include <cstdint>
 #include <cuda.h>
@@ -370,20 +371,31 @@ inline int tile_rows(long long groups, int parts) {
   return (int)(n < 1 ? 8 : n > kMaxTile / 8 ? kMaxTile : n * 8);
 }
 
-// How `n` weight rows (or columns of the result) of row_bytes each, `experts` times, are cut: rows of a piece, and whether pieces
-// stay whole.  To put together a tile that several CTAs share takes as long as about 110 KB of weights per SM (2.5 us): where
-// whole tiles, some width of them, leave no CTA more than that above an even share, they are not split.  Otherwise the widest,
-// in one box, that leave a CTA eight steps to share the work out evenly.  False: too much for 32-bit step numbers.
-inline bool split_plan(long long n, long long row_bytes, long long experts, int sms, int* tile, int* whole) {
-  const long long steps = experts * ((row_bytes + kChunk - 1) / kChunk), row = experts * row_bytes;
-  long long best = n * row / sms + (110 << 10);
-  *whole = 0;
+// How `n` weight rows (or columns of the result) of row_bytes each, `experts` times, are cut for `rows` rows of A: rows of a
+// piece, and whether pieces stay whole, by the nanoseconds that the CTA with most of the work takes.  Measured: a step of t
+// weight rows takes as long as its 512 t bytes at an SM's share of the memory's rate (twice that where half the SMs have
+// nothing to do), as its multiplications (2.8 ns per weight row and tile of 8 rows of A) or as its waits (0.25 us); the end
+// of a piece 1.1 us, once per expert where every expert's sums are put away (`each`); putting a tile together that several
+// CTAs share 3.2 us, and 0.2 us for every 512 sums of every one of them.  8-bit weights of 4096 columns, 3 rows of A, a call:
+// 28672 weight rows in whole tiles of 64 / 32 / 8 26.5 / 29.6 / 62.5 us; 4096 in whole tiles of 64 / 32 / 8 8.1 / 7.9 / 13.4
+// us, split among the SMs in 64 11.8 us.  A layer of 12 experts, 1024 / 2816: whole 50 us, split 36.5 us.
+// False: too much for 32-bit step numbers.
+inline bool split_plan(long long n, long long row_bytes, long long experts, int sms, int rows, int row_tiles, bool each, int* tile, int* whole) {
+  const long long chunks = (row_bytes + kChunk - 1) / kChunk, steps = experts * chunks;
+  double best = 1e300;
   for (int t = kMaxTile; t >= 8; t /= 2) {
-    const long long tiles = (n + t - 1) / t, most = (tiles + sms - 1) / sms * t * row;
-    if (most < best) { best = most; *whole = 1; *tile = t; }
+    const long long tiles = (n + t - 1) / t, total = tiles * steps;
+    for (int w = 1; w >= 0; w--) {
+      const long long parts = w ? tiles : total, busy = parts < sms ? parts : sms;
+      const long long most = w ? (tiles + sms - 1) / sms * steps : (total + busy - 1) / busy;       // steps of a CTA
+      const double share = busy * 2 > sms ? (double)busy / sms : 0.5;
+      const double step = std::max({11.6 * t * share, 2.8 * t * row_tiles, 209.0 + 35.0 * row_tiles});
+      const double ends = each ? (double)most / chunks + 1 - w : (double)most / steps + 1 - w;
+      const double join = w ? 0.0 : 3200.0 + 205.0 * ((steps + most - 1) / most + 1) * ((rows * t + 511) / 512);
+      const double ns = most * step + ends * (1000.0 + 125.0 * row_tiles) + join;
+      if (ns < best) { best = ns; *tile = t; *whole = w; }
+    }
   }
-  if (!*whole)
-    for (*tile = kMaxTile; *tile > 8 && (n + *tile - 1) / *tile * steps < 8ll * sms;) *tile /= 2;
   return (n + *tile - 1) / *tile * steps * sms <= 0xffffffffll;
 }
 

@@ -179,7 +179,7 @@ bool linear_plan(int M, int N, int K, LinearPlan* p) {
   if (M < 1 || M > kMaxRows || N < 8 || K < 16 || N % 8 || K % 16 || K > RBV_INT8_MAX_DEPTH) return false;
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&p->sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return false;
-  if (!split_plan(N, K, 1, p->sms, &p->tile, &p->whole)) return false;
+  if (!split_plan(N, K, 1, p->sms, M, box_rows(M) / 8, false, &p->tile, &p->whole)) return false;
   auto up = [](size_t v) { return (v + 255) / 256 * 256; };
   p->q_bytes = up((size_t)M * K);
   p->scale_bytes = up((size_t)M * 4);

@@ -562,7 +562,9 @@ bool few_plan(int T, int H, int I, int E, int top_k, FewPlan* p) {
   if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&p->sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return false;
   const int used = E < T * top_k ? E : T * top_k;   // experts in use, at most
   p->up_tile = tile_rows((long long)used * (2 * I / 8), p->sms);
-  if (!split_plan(H, 2ll * I, used, p->sms, &p->down_tile, &p->whole) || (long long)used * (2 * I / 8) * p->sms > 0xffffffffll) return false;
+  const bool each = T > 16;                         // the down product goes expert by expert
+  const int row_tiles = each ? (T * top_k + 8 * used - 1) / (8 * used) : (T + 7) / 8;
+  if (!split_plan(H, 2ll * I, used, p->sms, T, row_tiles, each, &p->down_tile, &p->whole) || (long long)used * (2 * I / 8) * p->sms > 0xffffffffll) return false;
   p->h_bytes = round_up((size_t)T * top_k * I * 2, 256);
   p->partial_bytes = round_up((size_t)2 * p->sms * T * p->down_tile * 4, 256);
   p->counter_bytes = round_up((size_t)(H / 8) * 4, 256);
