@@ -37,24 +37,32 @@ __device__ __forceinline__ __nv_bfloat162 vec_max(uint4 v, __nv_bfloat162 m) {
 __device__ __forceinline__ float no_nan(float m) { return m == m ? m : INFINITY; }
 
 __device__ __forceinline__ unsigned quantize_slowly(float x, float s) {
-  return (unsigned)max(-127, min(127, __float2int_rn(__fdiv_rn(x, s)))) & 0xffu;
+  return (unsigned)max(-127, min(127, __float2int_rn(__fdiv_rn(x, s))));
+}
+
+// Two 32-bit numbers in one register pair: a * b + c of both with one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(reinterpret_cast<unsigned long long&>(d))
+      : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)), "l"(reinterpret_cast<unsigned long long&>(c)));
+  return d;
 }
 
 // t = x * inv is within 2^-22 of x / s, relatively, and |t| <= 127.01: where t is further than 2^-14 from a half both round alike.
-// Adding 1.5 * 2^23 rounds t to an integer, which then stands in the low byte.
+// Adding 1.5 * 2^23 (to the exact product, in one fused step) rounds t to an integer, which then stands in the low byte.
 __device__ __forceinline__ uint2 quantize_vec(uint4 v, float s, float inv) {
   const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&v);
   constexpr float kMagic = 12582912.0f;
+  const float2 magic = make_float2(kMagic, kMagic), inv2 = make_float2(inv, inv), minus = make_float2(-1.0f, -1.0f);
   unsigned u[8];
   float far = 0.0f;                        // largest distance from the integer next to it
   #pragma unroll
   for (int j = 0; j < 4; j++) {
-    const float2 f = __bfloat1622float2(h[j]);
-    const float a = __fmul_rn(f.x, inv), b = __fmul_rn(f.y, inv), ua = __fadd_rn(a, kMagic), ub = __fadd_rn(b, kMagic);
-    far = fmaxf(far, fabsf(__fsub_rn(a, __fsub_rn(ua, kMagic))));
-    far = fmaxf(far, fabsf(__fsub_rn(b, __fsub_rn(ub, kMagic))));
-    u[2 * j] = __float_as_uint(ua);
-    u[2 * j + 1] = __float_as_uint(ub);
+    const float2 f = __bfloat1622float2(h[j]), up = fma2(f, inv2, magic), d = fma2(f, inv2, fma2(up, minus, magic));
+    far = fmaxf(far, fmaxf(fabsf(d.x), fabsf(d.y)));
+    u[2 * j] = __float_as_uint(up.x);
+    u[2 * j + 1] = __float_as_uint(up.y);
   }
   if (far > 0.5f - 6.2e-5f) {              // one in a thousand
     #pragma unroll
@@ -68,9 +76,12 @@ __device__ __forceinline__ uint2 quantize_vec(uint4 v, float s, float inv) {
                     __byte_perm(__byte_perm(u[4], u[5], 0x0040), __byte_perm(u[6], u[7], 0x0040), 0x5410));
 }
 
-// A row per blockDim.x threads (a warp, or the CTA); NV vectors per thread in registers, 0: read the row twice.
-template <int NV>
-__global__ void __launch_bounds__(512) quantize_rows_int8_kernel(const __grid_constant__ QuantArgs a) {
+// A row per blockDim.x threads (a warp, or the CTA); NV vectors per thread in registers, 0: read the row twice.  CTAS: of 512
+// threads per SM.  Three leave 40 registers and spill a few, which pays only where CTAs are so large that with 57 registers no
+// more than two fit (4096 rows of 11136: 43.7 us with two, 35.4 with three; 16384 rows of 4096: 47.6 and 48.3; 2000 of 2048: 4.8
+// and 6.6).
+template <int NV, int CTAS>
+__global__ void __launch_bounds__(512, CTAS) quantize_rows_int8_kernel(const __grid_constant__ QuantArgs a) {
   __shared__ float red[2][16];
   pdl_wait();
   pdl_trigger();      // after the wait: the kernel behind may read its weights before it waits for this one
@@ -139,16 +150,19 @@ cudaError_t launch_quantize_rows_int8(const void* x, long long rows, const int* 
   const QuantArgs a{static_cast<const __nv_bfloat16*>(x), rows, ldx, used, K, static_cast<int8_t*>(q), scale, zero, zeros};
   const int nvec = K / 8;
   // Few rows: as many threads per row as it has vectors, for latency.  More rows than SMs: four vectors per thread, so that an SM
-  // has some eight rows on the way (with 512 threads per row of 4096 it had three: 16384 rows took 95 us, now XXQ).
+  // has some eight rows on the way (with 512 threads per row of 4096 it had three: 16384 rows took 95 us, now 48).
   const int want_nv = rows > sms ? 4 : 1, lanes = (nvec + want_nv - 1) / want_nv;
   const int threads = lanes <= 32 ? 32 : lanes <= 512 ? (lanes + 31) / 32 * 32 : 512, per_cta = threads == 32 ? 4 : 1;
   const int nv = (nvec + threads - 1) / threads;
-  const long long want = (rows + per_cta - 1) / per_cta, most = (long long)sms * (2048 / (threads * per_cta));
-  const dim3 grid((unsigned)(want < most ? want : most)), block(threads, per_cta);
-  if (nv <= 1) return launch_dependent(quantize_rows_int8_kernel<1>, grid, block, 0, st, a);
-  if (nv <= 2) return launch_dependent(quantize_rows_int8_kernel<2>, grid, block, 0, st, a);
-  if (nv <= 4) return launch_dependent(quantize_rows_int8_kernel<4>, grid, block, 0, st, a);
-  return launch_dependent(quantize_rows_int8_kernel<0>, grid, block, 0, st, a);
+  auto launch = [&](auto* two, auto* three) {
+    const bool large = threads > 256;
+    const long long want = (rows + per_cta - 1) / per_cta, most = (long long)sms * ((large ? 1536 : 1024) / (threads * per_cta));
+    return launch_dependent(large ? three : two, dim3((unsigned)(want < most ? want : most)), dim3(threads, per_cta), 0, st, a);
+  };
+  if (nv <= 1) return launch(quantize_rows_int8_kernel<1, 2>, quantize_rows_int8_kernel<1, 3>);
+  if (nv <= 2) return launch(quantize_rows_int8_kernel<2, 2>, quantize_rows_int8_kernel<2, 3>);
+  if (nv <= 4) return launch(quantize_rows_int8_kernel<4, 2>, quantize_rows_int8_kernel<4, 3>);
+  return launch(quantize_rows_int8_kernel<0, 2>, quantize_rows_int8_kernel<0, 3>);
 }
 
 }  // namespace rbv

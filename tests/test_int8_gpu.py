@@ -115,6 +115,17 @@ def test_linear(M, N, K):
     _check(got, _want(*_plain_rows(x), w, c))
 
 
+@pytest.mark.parametrize("M,N,K", [(65, 1016, 11136), (96, 256, 8208), (160, 4096, 14336), (200, 264, 5120), (520, 520, 4096), (1300, 2048, 4096),
+                                   (4700, 4096, 1024), (3, 28672, 4096), (40, 9608, 3600), (64, 14336, 1040)])
+def test_linear_more_sizes(M, N, K):
+    """Tiles that do not fill the SMs, or just more than fill them; twice, for what a call leaves behind."""
+    from rbruck_alltoallv_b200.ops.moe import linear_int8
+    x, (w, c) = _rows(M, K, seed=M), _weight((N, K), seed=N)
+    want = _want(*_plain_rows(x), w, c)
+    for _ in range(2):
+        _check(linear_int8(x, w, c), want)
+
+
 def test_linear_extremes_are_exact():
     """The largest sum of the largest depth, 131072 * 127 * 127, and its negative."""
     from rbruck_alltoallv_b200.ops.moe import linear_int8
