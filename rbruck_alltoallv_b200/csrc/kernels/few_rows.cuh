@@ -402,9 +402,9 @@ inline bool split_plan(long long n, long long row_bytes, long long experts, int 
 // Dynamic shared memory that a CTA can have beside `fixed` bytes of static variables (which the compiler may round up).
 inline size_t ring_room(size_t fixed) { return 227 * 1024 - (fixed + 511) / 256 * 256; }
 
-// Stages that fit.
-inline int ring_stages(int tile, int rows, size_t fixed) {
-  const size_t room = ring_room(fixed) - 1024 /*alignment*/ - kRedBytes, n = room / slot_bytes(tile, rows);
+// Stages that fit beside `other` bytes of dynamic shared memory.
+inline int ring_stages(int tile, int rows, size_t fixed, size_t other) {
+  const size_t room = ring_room(fixed) - 1024 /*alignment*/ - kRedBytes - other, n = room / slot_bytes(tile, rows);
   return n > (size_t)kMaxStages ? kMaxStages : (int)n;
 }
 // Once per kernel and device: as much dynamic shared memory as there is beside `fixed` bytes.  (A call on one token takes less

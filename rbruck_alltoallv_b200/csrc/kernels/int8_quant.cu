@@ -10,11 +10,14 @@
 
 #include <cstdint>
 
+#include "kernels/int8_quant.cuh"
 #include "kernels/pdl.cuh"
 #include "rbv/moe.h"
 
 namespace rbv {
 namespace {
+
+using namespace quant;
 
 struct QuantArgs {
   const __nv_bfloat16* x;
@@ -26,55 +29,6 @@ struct QuantArgs {
   int* zero;                  // optional: `zeros` words to set to zero (counters of the kernel behind this one)
   int zeros;
 };
-
-// Largest magnitudes of the even and the odd ones of eight values; a NaN stays.
-__device__ __forceinline__ __nv_bfloat162 vec_max(uint4 v, __nv_bfloat162 m) {
-  const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&v);
-  #pragma unroll
-  for (int j = 0; j < 4; j++) m = __hmax2_nan(m, __habs2(h[j]));
-  return m;
-}
-__device__ __forceinline__ float no_nan(float m) { return m == m ? m : INFINITY; }
-
-__device__ __forceinline__ unsigned quantize_slowly(float x, float s) {
-  return (unsigned)max(-127, min(127, __float2int_rn(__fdiv_rn(x, s))));
-}
-
-// Two 32-bit numbers in one register pair: a * b + c of both with one instruction.
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-  float2 d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;"
-      : "=l"(reinterpret_cast<unsigned long long&>(d))
-      : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)), "l"(reinterpret_cast<unsigned long long&>(c)));
-  return d;
-}
-
-// t = x * inv is within 2^-22 of x / s, relatively, and |t| <= 127.01: where t is further than 2^-14 from a half both round alike.
-// Adding 1.5 * 2^23 (to the exact product, in one fused step) rounds t to an integer, which then stands in the low byte.
-__device__ __forceinline__ uint2 quantize_vec(uint4 v, float s, float inv) {
-  const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&v);
-  constexpr float kMagic = 12582912.0f;
-  const float2 magic = make_float2(kMagic, kMagic), inv2 = make_float2(inv, inv), minus = make_float2(-1.0f, -1.0f);
-  unsigned u[8];
-  float far = 0.0f;                        // largest distance from the integer next to it
-  #pragma unroll
-  for (int j = 0; j < 4; j++) {
-    const float2 f = __bfloat1622float2(h[j]), up = fma2(f, inv2, magic), d = fma2(f, inv2, fma2(up, minus, magic));
-    far = fmaxf(far, fmaxf(fabsf(d.x), fabsf(d.y)));
-    u[2 * j] = __float_as_uint(up.x);
-    u[2 * j + 1] = __float_as_uint(up.y);
-  }
-  if (far > 0.5f - 6.2e-5f) {              // one in a thousand
-    #pragma unroll
-    for (int j = 0; j < 4; j++) {
-      const float2 f = __bfloat1622float2(h[j]);
-      u[2 * j] = quantize_slowly(f.x, s);
-      u[2 * j + 1] = quantize_slowly(f.y, s);
-    }
-  }
-  return make_uint2(__byte_perm(__byte_perm(u[0], u[1], 0x0040), __byte_perm(u[2], u[3], 0x0040), 0x5410),
-                    __byte_perm(__byte_perm(u[4], u[5], 0x0040), __byte_perm(u[6], u[7], 0x0040), 0x5410));
-}
 
 // A row per blockDim.x threads (a warp, or the CTA); NV vectors per thread in registers, 0: read the row twice.  CTAS: of 512
 // threads per SM.  Three leave 40 registers and spill a few, which pays only where CTAs are so large that with 57 registers no
@@ -119,20 +73,19 @@ __global__ void __launch_bounds__(512, CTAS) quantize_rows_int8_kernel(const __g
       for (int o = 8; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
       m = __shfl_sync(0xffffffffu, m, 0);
     }
-    const bool tiny = m < 0x1p-100f, bad = m == INFINITY;
-    const float s = tiny || bad ? 1.0f : __fdiv_rn(m, 127.0f), inv = tiny || bad ? 0.0f : __frcp_rn(s);
-    if (threadIdx.x == 0) a.scale[r] = bad ? __int_as_float(0x7fffffff) : s;
+    const RowScale row(m);
+    if (threadIdx.x == 0) a.scale[r] = row.scale;
     uint2* q = reinterpret_cast<uint2*>(a.q + r * a.K);
-    if (tiny || bad) {
+    if (row.zero) {
       for (int at = threadIdx.x; at < nvec; at += blockDim.x) q[at] = make_uint2(0u, 0u);
     } else if (NV) {
       #pragma unroll
       for (int i = 0; i < NV; i++) {
         const int at = i * (int)blockDim.x + (int)threadIdx.x;
-        if (at < nvec) q[at] = quantize_vec(v[i], s, inv);
+        if (at < nvec) q[at] = quantize_vec(v[i], row);
       }
     } else {
-      for (int at = threadIdx.x; at < nvec; at += blockDim.x) q[at] = quantize_vec(__ldg(x + at), s, inv);
+      for (int at = threadIdx.x; at < nvec; at += blockDim.x) q[at] = quantize_vec(__ldg(x + at), row);
     }
   }
 }

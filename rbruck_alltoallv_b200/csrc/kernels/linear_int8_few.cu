@@ -4,6 +4,11 @@
 // reads the weights once.  The second kernel starts while the first one runs and has its first weights on the way by then;
 // only the quantised rows have to be waited for.  Work is column tiles x chunks of K, cut evenly among the SMs; integer sums of
 // a tile that several CTAs share are exact in any order.
+//
+// Up to 4096 elements of A in at most 8 rows, and tiles that are not split: one kernel, in which every CTA quantises the rows for
+// itself (they come out of L2) while its first weights are on their way.  4096 x 4096, one row: 7.9 us with two kernels, 6.2 with
+// one, from Python 7.3 and 5.9.  Four times the elements, eight vectors per thread, cost more than the second kernel (4 rows: 11.4
+// us, 7.9 with two).
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
@@ -11,6 +16,7 @@
 #include <type_traits>
 
 #include "kernels/few_rows.cuh"
+#include "kernels/int8_quant.cuh"
 #include "kernels/pdl.cuh"
 #include "rbv/moe.h"
 
@@ -31,7 +37,60 @@ struct LinearArgs {
   __nv_bfloat16* out;
   int* error;
   int tile, box, stages, whole;
+  const __nv_bfloat16* x;                 // rows that are quantised here, ldx elements apart
+  long long ldx;
+  uint32_t row_bytes;                     // room for them, a multiple of 1024
 };
+
+constexpr int kOwnElems = 4096, kOwnRows = 8;      // of A at most, where every CTA quantises it for itself
+
+// The rows in shared memory as Rows<1>::load reads them: chunk by chunk, column by column, M rows of 128 bytes with the 16-byte
+// units swizzled.  All consumer warps; scales[r] of row r, `largest` zero before.
+__device__ __forceinline__ void quantize_own(const LinearArgs& a, uint8_t* rows, unsigned* largest, float* scales) {
+  using namespace quant;
+  constexpr int kVecs = kOwnElems / 8 / (kWarps * 32);
+  const int tid = threadIdx.x, nvec = a.K / 8, total = a.M * nvec;
+  uint4 v[kVecs];
+  int row[kVecs];
+  #pragma unroll
+  for (int i = 0; i < kVecs; i++) {
+    const int f = i * kWarps * 32 + tid;
+    row[i] = f / nvec;
+    v[i] = make_uint4(0u, 0u, 0u, 0u);
+    if (f < total) v[i] = __ldg(reinterpret_cast<const uint4*>(a.x + row[i] * a.ldx) + f - row[i] * nvec);
+  }
+  #pragma unroll
+  for (int i = 0; i < kVecs; i++) {
+    if (i * kWarps * 32 >= total) break;
+    const __nv_bfloat162 both = vec_max(v[i], __float2bfloat162_rn(0.0f));
+    const unsigned m = __float_as_uint(fmaxf(no_nan(__low2float(both)), no_nan(__high2float(both))));
+    const int first = __shfl_sync(0xffffffffu, row[i], 0);
+    if (__all_sync(0xffffffffu, row[i] == first)) {        // (magnitudes are in order as unsigned numbers)
+      const unsigned most = __reduce_max_sync(0xffffffffu, m);
+      if ((tid & 31) == 0 && first < a.M) atomicMax(largest + first, most);
+    } else if (row[i] < a.M) {
+      atomicMax(largest + row[i], m);
+    }
+  }
+  consumers_sync();
+  const int chunk_bytes = a.M * kChunk;
+  auto place = [&](int r, int k) {
+    const int chunk = k / kChunk, col = k / 128 % kCols, unit = k / 16 % 8;
+    return reinterpret_cast<uint2*>(rows + chunk * chunk_bytes + (col * a.M + r) * 128 + ((unit ^ (r & 7)) << 4) + k % 16);
+  };
+  #pragma unroll
+  for (int i = 0; i < kVecs; i++) {
+    const int f = i * kWarps * 32 + tid;
+    if (f >= total) break;
+    const RowScale scale(__uint_as_float(largest[row[i]]));
+    const int at = f - row[i] * nvec;
+    if (at == 0) scales[row[i]] = scale.scale;
+    *place(row[i], at * 8) = scale.zero ? make_uint2(0u, 0u) : quantize_vec(v[i], scale);
+  }
+  const int behind = (kChunk - a.K % kChunk) % kChunk / 8;       // from the end of a row to the end of its last chunk
+  for (int f = tid; f < a.M * behind; f += kWarps * 32) *place(f / behind, a.K + f % behind * 8) = make_uint2(0u, 0u);
+  consumers_sync();
+}
 
 struct LinearPiece { int tile, c0, c1; };
 
@@ -61,26 +120,32 @@ struct LinearWalk {
   }
 };
 
-// NT: tiles of 8 rows of A.
-template <int NT>
+// NT: tiles of 8 rows of A.  OWN: the rows are quantised here.
+template <int NT, bool OWN>
 __global__ void __launch_bounds__(kThreads, 1) linear_int8_few_kernel(const __grid_constant__ WeightMaps maps, const __grid_constant__ WeightMaps q_maps,
                                                                       const __grid_constant__ LinearArgs a) {
   extern __shared__ uint8_t dyn[];
   __shared__ Ring ring;
   __shared__ int flag[2];
+  __shared__ unsigned largest[kOwnRows];
+  __shared__ float scales[kOwnRows];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(dyn) + 1023) & ~uintptr_t(1023));
   uint4* red = reinterpret_cast<uint4*>(base);
-  if (tid == 0) ring_init(ring, a.stages, 2);
-  if (warp >= kWarps) prefetch_maps(warp == kWarps ? maps : q_maps);
+  if (tid == 0) ring_init(ring, a.stages, OWN ? 1 : 2);
+  if (OWN && tid < kOwnRows) largest[tid] = 0u;
+  if (warp == kWarps) prefetch_maps(maps);
+  if (!OWN && warp == kWarps + 1) prefetch_maps(q_maps);
   pdl_trigger();
   __syncthreads();
   LinearWalk walk(a);
   LinearPiece p;
-  Cursor cur(ring, sm100::smem_u32(base + kRedBytes), a.stages, slot_bytes(a.tile, a.box));
+  uint8_t* own_rows = base + kRedBytes;
+  Cursor cur(ring, sm100::smem_u32(own_rows + (OWN ? a.row_bytes : 0u)), a.stages, slot_bytes(a.tile, OWN ? 0 : a.box));
   if (warp >= kWarps) {
-    if (lane >= 4) return;
+    if (lane >= 4 || (OWN && warp > kWarps)) return;
     if (warp == kWarps) {
+      if (OWN) pdl_wait();                // (the kernel before may be one that makes the weights; with two it is the quantiser)
       while (walk.next(p) && feed<int8_t>(maps, cur, 0, p.tile * a.tile, min(a.tile, a.N - p.tile * a.tile), p.c0, p.c1)) {}
     } else {
       pdl_wait();
@@ -90,12 +155,13 @@ __global__ void __launch_bounds__(kThreads, 1) linear_int8_few_kernel(const __gr
     return;
   }
   pdl_wait();
+  if (OWN) quantize_own(a, own_rows, largest, scales);
   int rows_at[NT];
   const int part = warp >> 2, col = warp & 3;
   #pragma unroll
   for (int i = 0; i < NT; i++) rows_at[i] = 8 * i + (lane >> 2) < a.M ? 8 * i + (lane >> 2) : -1;
   auto result = [&](int r, int n, int v0, int v1) {
-    const float s = __ldcg(a.row_scale + r);
+    const float s = OWN ? scales[r] : __ldcg(a.row_scale + r);
     const float2 c = *reinterpret_cast<const float2*>(a.col_scale + n);
     *reinterpret_cast<__nv_bfloat162*>(a.out + (long long)r * a.N + n) = __floats2bfloat162_rn((float)v0 * s * c.x, (float)v1 * s * c.y);
   };
@@ -113,7 +179,8 @@ __global__ void __launch_bounds__(kThreads, 1) linear_int8_few_kernel(const __gr
         cur.wait_full();
         __syncwarp();
         Rows<NT> rows;
-        rows.load(rows_at, cur.slot + (uint32_t)a.tile * kChunk, a.box, col, lane);
+        if (OWN) rows.load(rows_at, sm100::smem_u32(own_rows) + (uint32_t)(c * a.M * kChunk), a.M, col, lane);
+        else rows.load(rows_at, cur.slot + (uint32_t)a.tile * kChunk, a.box, col, lane);
         multiply<G>(acc, cur.slot, off, rows, lane);
         __syncwarp();
         if (lane == 0) cur.release();
@@ -173,7 +240,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_int8_few_kernel(const __gr
   if (!cur.ok && a.error) atomicExch(a.error, 1);
 }
 
-struct LinearPlan { int sms, tile, whole; size_t q_bytes, scale_bytes, partial_bytes, counter_bytes; };
+struct LinearPlan { int sms, tile, whole, own; size_t q_bytes, scale_bytes, partial_bytes, counter_bytes; };
 
 bool linear_plan(int M, int N, int K, LinearPlan* p) {
   if (M < 1 || M > kMaxRows || N < 8 || K < 16 || N % 8 || K % 16 || K > RBV_INT8_MAX_DEPTH) return false;
@@ -181,6 +248,12 @@ bool linear_plan(int M, int N, int K, LinearPlan* p) {
   if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&p->sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return false;
   if (!split_plan(N, K, 1, p->sms, M, box_rows(M) / 8, false, &p->tile, &p->whole)) return false;
   auto up = [](size_t v) { return (v + 255) / 256 * 256; };
+  p->own = p->whole && M <= kOwnRows && (long long)M * K <= kOwnElems;
+  if (p->own) {                           // nothing is left for another kernel
+    p->q_bytes = p->scale_bytes = p->counter_bytes = 0;
+    p->partial_bytes = 256;
+    return true;
+  }
   p->q_bytes = up((size_t)M * K);
   p->scale_bytes = up((size_t)M * 4);
   p->partial_bytes = up((size_t)2 * p->sms * M * p->tile * 4);
@@ -188,20 +261,22 @@ bool linear_plan(int M, int N, int K, LinearPlan* p) {
   return true;
 }
 
-template <int NT>
+template <int NT, bool OWN = false>
 cudaError_t linear_launch(const LinearArgs& args, const int8_t* q, const void* w, const LinearPlan& p, cudaStream_t st) {
   LinearArgs a = args;
   WeightMaps maps, q_maps;
   if (!weight_maps(&maps, w, (unsigned long long)a.N, (unsigned long long)a.K, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p.tile | a.N % p.tile) ||
-      !weight_maps(&q_maps, q, (unsigned long long)a.M, (unsigned long long)a.K, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, box_rows(a.M)))
+      (!OWN && !weight_maps(&q_maps, q, (unsigned long long)a.M, (unsigned long long)a.K, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, box_rows(a.M))))
     return cudaErrorUnknown;
   a.tile = p.tile;
   a.whole = p.whole;
-  a.box = box_rows(a.M);
-  a.stages = ring_stages(a.tile, a.box, sizeof(Ring) + 64);
-  const size_t smem = ring_smem(a.tile, a.box, a.stages);
-  const cudaError_t e = allow_smem_once<linear_int8_few_kernel<NT>>(sizeof(Ring) + 64);
-  return e != cudaSuccess ? e : launch_dependent(linear_int8_few_kernel<NT>, dim3(p.sms), dim3(kThreads), smem, st, maps, q_maps, a);
+  a.box = OWN ? 0 : box_rows(a.M);
+  a.row_bytes = OWN ? ((uint32_t)a.M * (uint32_t)((a.K + kChunk - 1) / kChunk * kChunk) + 1023) / 1024 * 1024 : 0u;
+  constexpr size_t kFixed = sizeof(Ring) + 128;
+  a.stages = ring_stages(a.tile, a.box, kFixed, a.row_bytes);
+  const size_t smem = ring_smem(a.tile, a.box, a.stages) + a.row_bytes;
+  const cudaError_t e = allow_smem_once<linear_int8_few_kernel<NT, OWN>>(kFixed);
+  return e != cudaSuccess ? e : launch_dependent(linear_int8_few_kernel<NT, OWN>, dim3(p.sms), dim3(kThreads), smem, st, maps, q_maps, a);
 }
 
 }  // namespace
@@ -232,6 +307,12 @@ extern "C" int rbv_linear_int8_few(const void* x, long long ldx, int M, const vo
   a.out = static_cast<__nv_bfloat16*>(out);
   a.error = error_flag;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (p.own) {
+    if (reinterpret_cast<uintptr_t>(x) & 15 || ldx % 8) return (int)cudaErrorMisalignedAddress;
+    a.x = static_cast<const __nv_bfloat16*>(x);
+    a.ldx = ldx;
+    return (int)linear_launch<1, true>(a, nullptr, w, p, st);
+  }
   const cudaError_t e = launch_quantize_rows_int8(x, M, nullptr, K, ldx, q, scale, a.counters, (int)(p.counter_bytes / 4), st);
   if (e != cudaSuccess) return (int)e;
   if (M <= 8) return (int)linear_launch<1>(a, q, w, p, st);

@@ -115,6 +115,30 @@ def test_linear(M, N, K):
     _check(got, _want(*_plain_rows(x), w, c))
 
 
+@pytest.mark.parametrize("M,K", [(1, 4096), (1, 16), (2, 2048), (3, 1360), (4, 1024), (5, 816), (8, 512), (8, 528), (7, 400), (1, 4112)])
+def test_linear_rows_quantised_by_every_cta(M, K):
+    from rbruck_alltoallv_b200.ops.moe import linear_int8
+    wide = torch.zeros(M, K + 24, dtype=BF, device="cuda")
+    x, (w, c) = wide[:, 8:8 + K], _weight((264, K), seed=K)
+    x.copy_(_rows(M, K, seed=M))
+    q, s = _plain_rows(x)
+    _check(linear_int8(x, w, c), _want(q, s, w, c))
+    x[0] = 0
+    x[M - 1, K // 2] = float("nan") if M % 2 else float("inf")
+    got = linear_int8(x, w, c)
+    assert got[M - 1].isnan().all() and (M == 1 or (got[0] == 0).all())
+    _check(got[1:M - 1], _want(q[1:M - 1], s[1:M - 1], w, c)) if M > 2 else None
+
+
+def test_linear_right_behind_the_kernel_that_makes_its_weights():
+    from rbruck_alltoallv_b200.ops.moe import linear_int8, quantize_rows_int8
+    x, one, two = _rows(1, 4096, seed=1), _rows(4096, 4096, seed=2), _rows(4096, 4096, seed=3)
+    wants = [linear_int8(x, *quantize_rows_int8(v)) for v in (one, two)]
+    torch.cuda.synchronize()
+    for v, want in [(one, wants[0]), (two, wants[1])] * 10:
+        assert torch.equal(linear_int8(x, *quantize_rows_int8(v)), want)
+
+
 @pytest.mark.parametrize("M,N,K", [(65, 1016, 11136), (96, 256, 8208), (160, 4096, 14336), (200, 264, 5120), (520, 520, 4096), (1300, 2048, 4096),
                                    (4700, 4096, 1024), (3, 28672, 4096), (40, 9608, 3600), (64, 14336, 1040)])
 def test_linear_more_sizes(M, N, K):
