@@ -236,6 +236,12 @@ grouped_gemm_int8_kernel(const __grid_constant__ I8Maps maps, const __grid_const
       const int b = i & 1;
       const int nw = tl.n0 + (int)rank * IH + q * 32;   // first of this warp's 32 channels
       const float cs = nw + lane < p.N ? __ldg(p.col_scale + (size_t)tl.g * p.N + nw + lane) : 0.0f;
+      float rs[IT / (2 * IU)];                          // scales of this warp's tokens, on their way while the tile is multiplied
+      #pragma unroll
+      for (int j = 0; j < IT / (2 * IU); j++) {
+        const int c = first + j * 2 * IU + lane;
+        rs[j] = c < tl.ntok ? __ldg(p.row_scale + tl.tok0 + c) : 0.0f;
+      }
       if (!mbar_wait(&tfull_bar[b], ((uint32_t)i >> 1) & 1u, abort_flag)) { ok = false; break; }
       tc_fence_after_sync();
       const uint32_t taddr = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)b * IT;
@@ -244,11 +250,12 @@ grouped_gemm_int8_kernel(const __grid_constant__ I8Maps maps, const __grid_const
       for (int c = first; c < tl.nt; c += 2 * IU) {
         uint32_t r[32];
         tmem_ld32(taddr + c, r);
-        const float rs = c + lane < tl.ntok ? __ldg(p.row_scale + tl.tok0 + c + lane) : 0.0f;
         tmem_ld_wait();
         #pragma unroll
         for (int k = 0; k < 32; k++)
-          r[k] = __float_as_uint((float)(int)r[k] * cs * __shfl_sync(0xffffffffu, rs, k));
+          r[k] = __float_as_uint((float)(int)r[k] * cs * __shfl_sync(0xffffffffu, rs[0], k));
+        #pragma unroll
+        for (int j = 0; j + 1 < IT / (2 * IU); j++) rs[j] = rs[j + 1];
         __nv_bfloat16* rows = p.C + (size_t)(tl.tok0 + c) * p.ldc;
         // (all lanes take part in the exchanges; tokens or channels that do not exist are not stored)
         if (p.swiglu) tokepi::store_swiglu(r, rows, p.ldc, nw / 2, (lane >> 2) * 4 < live_cols ? tl.ntok - c : 0, lane);
