@@ -30,5 +30,7 @@ def block_norm(residual: torch.Tensor, branch: Optional[torch.Tensor] = None, po
     None.  The weights ``[hidden]`` and the gate are in the branch's type or fp32.  ``gate`` is one value per channel
     ``[hidden]``, per token ``[..., 1]`` or per element; any other shape that broadcasts to the residual's is expanded first.
     ``normed`` has the branch's type and is made from the sum before that is rounded to the residual's type.  Rows may be
-    strided (elements of a row packed).  Launched on the current stream of the tensors' device."""
+    strided (elements of a row packed).  Launched on the current stream of the tensors' device; both passes can be captured into a
+    graph, the backward pass while no graph of an earlier, eager pass through the same leaves is alive (torch would accumulate into
+    them on that pass's stream, which a capture does not survive)."""
     return _native.torch_ops().block_norm(residual, branch, post_weight, gate, scale, pre_weight, eps)

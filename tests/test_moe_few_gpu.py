@@ -112,6 +112,19 @@ def test_a_bad_token_stays_alone():
     assert torch.equal(got[others], clean[others]) and got[5].isnan().all()
 
 
+@pytest.mark.parametrize("T", [2, 9, 16, 30, 64])
+def test_bad_tokens_stay_alone_in_every_size_of_batch(T):
+    from rbruck_alltoallv_b200.ops.moe import moe_few_tokens
+    x, logits, w13, w2 = _make(T, 264, 136, 5)
+    logits[T - 1] = logits[0]                            # on the same experts
+    logits[T // 2] = -math.inf                           # a padded slot with anything in it
+    clean = moe_few_tokens(x, logits, w13, w2)
+    x[0, 3], x[T // 2] = math.inf, math.nan
+    got = moe_few_tokens(x, logits, w13, w2)
+    assert not got[0].isfinite().all()
+    assert torch.equal(got[1:], clean[1:]) and (got[T // 2] == 0).all()
+
+
 def test_strides_out_and_no_tokens():
     from rbruck_alltoallv_b200.ops.moe import moe_few_tokens
     x, logits, w13, w2 = _make(10, 128, 64, 8)
