@@ -133,8 +133,8 @@ struct Cursor {
   }
 };
 
-// Shared memory of a CTA: the buffer in which warps add their sums, then the stages, 1024-byte aligned.
-constexpr uint32_t kRedBytes = 2 * 4 * kCols * 32 * 16;       // four groups of weight rows at a time per part
+// Shared memory of a CTA: the buffer, or two, in which warps add their sums, then the stages, 1024-byte aligned.
+constexpr uint32_t kRedBytes = 2 * 4 * kCols * 32 * 16;       // four tiles at a time per part
 // A stage: `tile` weight rows and `rows` of A.
 __host__ __device__ inline uint32_t slot_bytes(int tile, int rows) { return (uint32_t)(tile + rows) * kChunk; }
 // Rows of the box that holds r rows of A.
@@ -316,17 +316,21 @@ __device__ __forceinline__ void multiply(Acc (&acc)[kGroups][NT][4], uint32_t w,
 }
 
 // Adds the sums of a part's four columns and hands them out: put(row of A, weight row of the piece, sums of that weight row and
-// the next one; even weight rows).  Four tiles of 16 x 8 at a time, one per warp.  The parts do not wait for one another.
+// the next one; even weight rows).  Four tiles of 16 x 8 at a time, one per warp.  The parts do not wait for one another.  With two
+// buffers in turn, from call to call too, one barrier is enough: who writes into one has passed the barrier behind which everybody
+// has left it.
+struct Red { uint4* at; bool two; int turn = 0; };
 template <int NT, typename Acc, typename Put>
-__device__ __forceinline__ void add_columns(const Acc (&acc)[kGroups][NT][4], uint4* red, const Share& share, int part, int col, int lane,
+__device__ __forceinline__ void add_columns(const Acc (&acc)[kGroups][NT][4], Red& red, const Share& share, int part, int col, int lane,
                                             Put&& put) {
-  uint4* mine = red + part * (4 * kCols * 32);
   const int g = lane >> 2, t = lane & 3;
   const bool odd = (g & 1) != 0;
   const int tiles = share.count * NT;
   #pragma unroll
   for (int first = 0; first < kGroups * NT; first += 4) {
     if (first >= tiles) break;
+    uint4* mine = red.at + (2 * red.turn + part) * (4 * kCols * 32);
+    if (red.two) red.turn ^= 1;
     #pragma unroll
     for (int k = 0; k < 4; k++)            // (tile first + k: group / NT, tile of rows % NT)
       if (first + k < kGroups * NT)
@@ -349,7 +353,7 @@ __device__ __forceinline__ void add_columns(const Acc (&acc)[kGroups][NT][4], ui
         put(8 * (tile % NT) + 2 * t + (odd ? 1 : 0), 16 * (share.first + tile / NT) + 8 * h + (g & ~1), odd ? got : v[2 * h], odd ? v[2 * h + 1] : got);
       }
     }
-    part_sync(part);
+    if (!red.two) part_sync(part);
   }
 }
 
@@ -404,7 +408,7 @@ inline size_t ring_room(size_t fixed) { return 227 * 1024 - (fixed + 511) / 256 
 
 // Stages that fit beside `other` bytes of dynamic shared memory.
 inline int ring_stages(int tile, int rows, size_t fixed, size_t other) {
-  const size_t room = ring_room(fixed) - 1024 /*alignment*/ - kRedBytes - other, n = room / slot_bytes(tile, rows);
+  const size_t room = ring_room(fixed) - 1024 /*alignment*/ - other, n = room / slot_bytes(tile, rows);
   return n > (size_t)kMaxStages ? kMaxStages : (int)n;
 }
 // Once per kernel and device: as much dynamic shared memory as there is beside `fixed` bytes.  (A call on one token takes less
@@ -419,7 +423,7 @@ inline cudaError_t allow_smem_once(size_t fixed) {
   if (e == cudaSuccess && dev < 64) done.fetch_or(1ull << dev, std::memory_order_relaxed);
   return e;
 }
-inline size_t ring_smem(int tile, int rows, int stages) { return 1024 + kRedBytes + (size_t)slot_bytes(tile, rows) * stages; }
+inline size_t ring_smem(int tile, int rows, int stages) { return 1024 + (size_t)slot_bytes(tile, rows) * stages; }
 
 typedef CUresult (*TensorMapEncoder)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
                                      const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion,

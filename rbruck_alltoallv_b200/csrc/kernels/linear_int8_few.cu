@@ -131,7 +131,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_int8_few_kernel(const __gr
   __shared__ float scales[kOwnRows];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(dyn) + 1023) & ~uintptr_t(1023));
-  uint4* red = reinterpret_cast<uint4*>(base);
+  Red red{reinterpret_cast<uint4*>(base), true};
   if (tid == 0) ring_init(ring, a.stages, OWN ? 1 : 2);
   if (OWN && tid < kOwnRows) largest[tid] = 0u;
   if (warp == kWarps) prefetch_maps(maps);
@@ -140,7 +140,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_int8_few_kernel(const __gr
   __syncthreads();
   LinearWalk walk(a);
   LinearPiece p;
-  uint8_t* own_rows = base + kRedBytes;
+  uint8_t* own_rows = base + 2 * kRedBytes;
   Cursor cur(ring, sm100::smem_u32(own_rows + (OWN ? a.row_bytes : 0u)), a.stages, slot_bytes(a.tile, OWN ? 0 : a.box));
   if (warp >= kWarps) {
     if (lane >= 4 || (OWN && warp > kWarps)) return;
@@ -273,8 +273,8 @@ cudaError_t linear_launch(const LinearArgs& args, const int8_t* q, const void* w
   a.box = OWN ? 0 : box_rows(a.M);
   a.row_bytes = OWN ? ((uint32_t)a.M * (uint32_t)((a.K + kChunk - 1) / kChunk * kChunk) + 1023) / 1024 * 1024 : 0u;
   constexpr size_t kFixed = sizeof(Ring) + 128;
-  a.stages = ring_stages(a.tile, a.box, kFixed, a.row_bytes);
-  const size_t smem = ring_smem(a.tile, a.box, a.stages) + a.row_bytes;
+  a.stages = ring_stages(a.tile, a.box, kFixed, 2 * kRedBytes + a.row_bytes);
+  const size_t smem = ring_smem(a.tile, a.box, a.stages) + 2 * kRedBytes + a.row_bytes;
   const cudaError_t e = allow_smem_once<linear_int8_few_kernel<NT, OWN>>(kFixed);
   return e != cudaSuccess ? e : launch_dependent(linear_int8_few_kernel<NT, OWN>, dim3(p.sms), dim3(kThreads), smem, st, maps, q_maps, a);
 }

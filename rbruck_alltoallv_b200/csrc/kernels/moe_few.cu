@@ -41,6 +41,7 @@ struct FewArgs {
   int* error;
   int tile, room, whole;                  // weight rows of a piece at most; bytes of the ring; whole: tiles of the down product are
                                           // not split
+  uint32_t red;                           // bytes in which warps add their sums
 };
 
 // The choice, as every CTA makes it.
@@ -276,7 +277,7 @@ template <int MAX> __device__ __forceinline__ int token_box(int T, int R) { retu
 template <int MAX> struct XMaps { WeightMaps box; CUtensorMap rows; };
 
 template <int NT, int MAX>
-__device__ __forceinline__ void up_piece(const FewArgs& a, Shared<MAX>& s, uint4* red, Cursor& cur, const UpPiece& p, int warp, int lane) {
+__device__ __forceinline__ void up_piece(const FewArgs& a, Shared<MAX>& s, Red& red, Cursor& cur, const UpPiece& p, int warp, int lane) {
   const int R = s.choice.rows[p.u], part = warp >> 2, col = warp & 3;
   const Share share(p.rows, part);
   const Offsets off(p.rows, share, col);
@@ -305,7 +306,7 @@ __global__ void __launch_bounds__(kThreads, 1) moe_few_up_kernel(const __grid_co
   __shared__ Shared<MAX> s;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   uint8_t* base = aligned_smem(dyn);
-  uint4* red = reinterpret_cast<uint4*>(base);
+  Red red{reinterpret_cast<uint4*>(base), a.red > kRedBytes};
   ring_init_all(s.ring, 2);
   if (warp == kWarps) prefetch_maps(maps);
   if (warp == kWarps + 1) prefetch_maps(x_maps.box);
@@ -316,7 +317,7 @@ __global__ void __launch_bounds__(kThreads, 1) moe_few_up_kernel(const __grid_co
   choose(s.choice, a);
   UpWalk walk(a, s.choice.n_used);
   UpPiece p;
-  Cursor cur = ring_cursor(s.ring, a, sm100::smem_u32(base + kRedBytes), token_box<MAX>(a.T, s.choice.most));
+  Cursor cur = ring_cursor(s.ring, a, sm100::smem_u32(base + a.red), token_box<MAX>(a.T, s.choice.most));
   const int chunks = (2 * a.H + kChunk - 1) / kChunk;
   if (warp == kWarps) {
     if (lane >= 4) return;
@@ -378,7 +379,7 @@ struct DownWalk {
 // More than 16 tokens: an expert's rows by themselves, as in the up product; their sums over the expert's K are added to the
 // tokens' sums in shared memory, expert by expert.
 template <int NT, int MAX>
-__device__ __forceinline__ void down_piece(const FewArgs& a, Shared<MAX>& s, uint4* red, float* sums, Cursor& cur, const DownPiece& p, int nr,
+__device__ __forceinline__ void down_piece(const FewArgs& a, Shared<MAX>& s, Red& red, float* sums, Cursor& cur, const DownPiece& p, int nr,
                                            int warp, int lane) {
   const int R = s.choice.rows[p.u], part = warp >> 2, col = warp & 3;
   const Share share(nr, part);
@@ -411,8 +412,8 @@ __global__ void __launch_bounds__(kThreads, 1) moe_few_down_kernel(const __grid_
   __shared__ Shared<MAX> s;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   uint8_t* base = aligned_smem(dyn);
-  uint4* red = reinterpret_cast<uint4*>(base);
-  float* sums = reinterpret_cast<float*>(base + kRedBytes);                // [MAX][kMaxTile] beyond 16 tokens
+  Red red{reinterpret_cast<uint4*>(base), a.red > kRedBytes};
+  float* sums = reinterpret_cast<float*>(base + a.red);                // [MAX][kMaxTile] beyond 16 tokens
   constexpr uint32_t kSumBytes = MAX > 16 ? MAX * kMaxTile * 4 : 0;
   ring_init_all(s.ring, 2);
   if (warp >= kWarps) prefetch_maps(warp == kWarps ? maps : h_maps);
@@ -427,7 +428,7 @@ __global__ void __launch_bounds__(kThreads, 1) moe_few_down_kernel(const __grid_
   }
   DownWalk walk(a, n_used);
   DownPiece p;
-  Cursor cur = ring_cursor(s.ring, a, sm100::smem_u32(base + kRedBytes + kSumBytes), box_rows(s.choice.most));
+  Cursor cur = ring_cursor(s.ring, a, sm100::smem_u32(base + a.red + kSumBytes), box_rows(s.choice.most));
   if (warp >= kWarps) {                   // the weights do not wait for the first kernel, the rows of h do
     if (lane >= 4) return;
     if (warp == kWarps) {
@@ -572,10 +573,14 @@ bool few_plan(int T, int H, int I, int E, int top_k, FewPlan* p) {
 }
 
 template <int MAX, auto* Kernel, typename... Maps>
-cudaError_t launch_ring(FewArgs a, int tile, size_t sums, int sms, cudaStream_t st, const Maps&... maps) {
+cudaError_t launch_ring(FewArgs a, int tile, size_t row_bytes, size_t sums, int sms, cudaStream_t st, const Maps&... maps) {
   const size_t smem = ring_room(sizeof(Shared<MAX>));
   a.tile = tile;
-  a.room = (int)(smem - 1024 /*alignment*/ - kRedBytes - sums);
+  // A second buffer for the sums saves a barrier at the end of every piece and costs half a stage.  Up to 16 tokens and pieces of at
+  // most 8 steps gain (31 tokens of 128 experts, 512 / 1024: 98.5 -> 91.5 us; 16 tokens of 8, 4096 / 14336: 421 -> 413), long pieces
+  // with more tokens lose (64 tokens: 468 -> 512).
+  a.red = MAX == 16 || row_bytes <= 8 * kChunk ? 2 * kRedBytes : kRedBytes;
+  a.room = (int)(smem - 1024 /*alignment*/ - a.red - sums);
   const cudaError_t e = allow_smem_once<Kernel>(sizeof(Shared<MAX>));
   return e != cudaSuccess ? e : launch_dependent(Kernel, dim3(sms), dim3(kThreads), smem, st, maps..., a);
 }
@@ -592,8 +597,8 @@ cudaError_t few_launch(FewArgs a, const FewPlan& p, cudaStream_t st) {
       !weight_maps(&x.box, a.x, T, x_row, bf16, 2, box_rows(a.T), x_step) || (MAX > 16 && !gather_map(&x.rows, a.x, T, x_row, x_step, bf16, 2)))
     return cudaErrorUnknown;
   a.whole = p.whole;
-  const cudaError_t e = launch_ring<MAX, moe_few_up_kernel<MAX>>(a, p.up_tile, 0, p.sms, st, w13, x);
-  return e != cudaSuccess ? e : launch_ring<MAX, moe_few_down_kernel<MAX>>(a, p.down_tile, MAX > 16 ? (size_t)MAX * kMaxTile * 4 : 0, p.sms, st, w2, h);
+  const cudaError_t e = launch_ring<MAX, moe_few_up_kernel<MAX>>(a, p.up_tile, x_row, 0, p.sms, st, w13, x);
+  return e != cudaSuccess ? e : launch_ring<MAX, moe_few_down_kernel<MAX>>(a, p.down_tile, h_row, MAX > 16 ? (size_t)MAX * kMaxTile * 4 : 0, p.sms, st, w2, h);
 }
 
 }  // namespace
