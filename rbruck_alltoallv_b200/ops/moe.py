@@ -540,9 +540,9 @@ class MoEExpertParallel:
     def decode(self, x: torch.Tensor, logits: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """The layer for a batch of decoded tokens: any number of them up to :data:`FEW_TOKENS`, whatever ``tokens`` the layer
         was made for, in two kernels (:func:`moe_few_tokens`).  bf16 experts on one rank.  Up to 16 tokens it takes less time than
-        :meth:`forward` (8 experts, 4096 / 14336: 1 token 115 against 141 us, 16 tokens 415 against 433; 64 experts, 2048 / 1408:
-        1 token 15 against 47 us, 16 tokens 77 against 88), for 32 about the same (420 against 437, 120 against 119), for 64 a
-        tenth more (483 against 438, 178 against 163)."""
+        :meth:`forward` (8 experts, 4096 / 14336: 1 token 115 against 141 us, 16 tokens 406 against 434; 64 experts, 2048 / 1408:
+        1 token 14 against 45 us, 16 tokens 83 against 90), for 32 about the same (420 against 440, 133 against 132), for 64 a
+        tenth more (475 against 434, 184 against 166)."""
         if self.P != 1 or self.fp8:
             raise ValueError("decode() is for bf16 experts on one rank")
         return moe_few_tokens(x, logits, self.w13, self.w2, 2, out, self.error[1:2])
