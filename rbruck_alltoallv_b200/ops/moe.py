@@ -279,12 +279,17 @@ def quantize_rows_int8(x: torch.Tensor, used: Optional[torch.Tensor] = None):
 
 
 def quantize_weight_int8(w: torch.Tensor):
-    """bf16 / fp32 [..., N, K] -> (int8 [..., N, K], fp32 scales [..., N]), one scale per output channel."""
+    """bf16 / fp32 [..., N, K] -> (int8 [..., N, K], fp32 scales [..., N]), one scale per output channel.  As in
+    :func:`quantize_rows_int8` a channel with an infinity or a NaN gets zeros and the scale NaN, so that what is made of it is
+    NaN; one whose values are all so small (below 2^-119) that its scale would not be a normal number becomes zeros with the
+    scale 1."""
     f = w.float()
     amax = f.abs().amax(dim=-1)
-    scale = torch.where(amax > 0, amax / 127.0, torch.ones_like(amax))
-    q = torch.round(f / scale[..., None]).clamp_(-127, 127).to(torch.int8)
-    return q.contiguous(), scale.contiguous()
+    finite = amax.isfinite()
+    live = finite & (amax / 127.0 >= torch.finfo(torch.float32).smallest_normal)
+    scale = torch.where(live, amax / 127.0, torch.ones_like(amax))
+    q = torch.round(f / scale[..., None]).clamp_(-127, 127).masked_fill_(~live[..., None], 0).to(torch.int8)
+    return q.contiguous(), scale.masked_fill(~finite, float("nan")).contiguous()
 
 
 def dequantize_int8(q: torch.Tensor, scale: torch.Tensor) -> torch.Tensor:

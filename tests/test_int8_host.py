@@ -70,3 +70,23 @@ def test_weight_quantiser():
     assert ((dequantize_int8(q, s) - w.float()).abs() <= s[..., None] * (0.5 + 127 * 2 ** -22)).all()
     top = q.abs().amax(-1)
     assert (top[s != 1] == 127).all()
+
+
+@pytest.mark.parametrize("kind", [torch.float32, BF])
+def test_weight_quantiser_of_bad_and_tiny_channels(kind):
+    """As for rows: a channel with a NaN or an infinity gets the scale NaN, so that whatever is made of it is NaN, and one whose
+    values are all below 2^-100 zeros and the scale 1; its neighbours are what they were."""
+    w = torch.randn(2, 9, 32, generator=torch.Generator().manual_seed(2)).to(kind)
+    want, ws = quantize_weight_int8(w)
+    w[0, 1, 3], w[0, 2, 31], w[1, 3, 0] = float("nan"), float("inf"), -float("inf")
+    w[1, 4], w[1, 5], w[1, 6] = 2.0 ** -120, 0.0, 2.0 ** -119
+    q, s = quantize_weight_int8(w)
+    for at in ((0, 1), (0, 2), (1, 3)):
+        assert s[at].isnan() and (q[at] == 0).all() and dequantize_int8(q, s)[at].isnan().all()
+    for at in ((1, 4), (1, 5)):
+        assert s[at] == 1 and (q[at] == 0).all()
+    assert (q[1, 6] == 127).all() and s[1, 6] == w[1, 6, 0].float() / 127.0
+    rest = torch.ones(2, 9, dtype=torch.bool)
+    for at in ((0, 1), (0, 2), (1, 3), (1, 4), (1, 5), (1, 6)):
+        rest[at] = False
+    assert torch.equal(q[rest], want[rest]) and torch.equal(s[rest], ws[rest])
