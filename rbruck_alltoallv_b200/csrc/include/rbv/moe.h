@@ -72,7 +72,7 @@ int rbv_grouped_gemm_int8(const void* A, const float* a_scale, long long a_rows,
 int rbv_quantize_rows_int8(const void* x_bf16, long long rows, const int* used, int K, long long ldx, void* out_int8,
                            float* scale, void* cuda_stream);
 /* Linear of a few rows (1 <= M <= 64), quantised within the call: x [M, K] bf16, W [N, K] int8 with w_scale [N], out [M, N]
- * bf16.  workspace: rbv_linear_int8_few_workspace(...) bytes of this call alone (-1 for sizes that are not taken). */
+ * bf16, which may share memory with x.  workspace: rbv_linear_int8_few_workspace(...) bytes of this call alone (-1 for sizes that are not taken). */
 long long rbv_linear_int8_few_workspace(int M, int N, int K);
 int rbv_linear_int8_few(const void* x, long long ldx, int M, const void* W, const float* w_scale, int N, int K, void* out,
                         void* workspace, int* error_flag, void* cuda_stream);

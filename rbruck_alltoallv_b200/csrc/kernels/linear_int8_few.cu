@@ -8,7 +8,7 @@
 // Up to 4096 elements of A in at most 8 rows, and tiles that are not split: one kernel, in which every CTA quantises the rows for
 // itself (they come out of L2) while its first weights are on their way.  4096 x 4096, one row: 7.9 us with two kernels, 6.2 with
 // one, from Python 7.3 and 5.9.  Four times the elements, eight vectors per thread, cost more than the second kernel (4 rows: 11.4
-// us, 7.9 with two).
+// us, 7.9 with two).  Results that are written over the rows take two kernels.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
@@ -249,13 +249,12 @@ bool linear_plan(int M, int N, int K, LinearPlan* p) {
   if (!split_plan(N, K, 1, p->sms, M, box_rows(M) / 8, false, &p->tile, &p->whole)) return false;
   auto up = [](size_t v) { return (v + 255) / 256 * 256; };
   p->own = p->whole && M <= kOwnRows && (long long)M * K <= kOwnElems;
-  if (p->own) {                           // nothing is left for another kernel
-    p->q_bytes = p->scale_bytes = p->counter_bytes = 0;
-    p->partial_bytes = 256;
-    return true;
-  }
   p->q_bytes = up((size_t)M * K);
   p->scale_bytes = up((size_t)M * 4);
+  if (p->own) {                           // one kernel, or two (results over the rows); tiles are whole
+    p->partial_bytes = p->counter_bytes = 0;
+    return true;
+  }
   p->partial_bytes = up((size_t)2 * p->sms * M * p->tile * 4);
   p->counter_bytes = up((size_t)((N + p->tile - 1) / p->tile) * 4);
   return true;
@@ -296,6 +295,9 @@ extern "C" int rbv_linear_int8_few(const void* x, long long ldx, int M, const vo
   if ((reinterpret_cast<uintptr_t>(w) | reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(workspace) |
        reinterpret_cast<uintptr_t>(w_scale)) & 15)
     return (int)cudaErrorMisalignedAddress;
+  // With one kernel a CTA may read the rows when another one has already stored its results: never over the rows themselves.
+  const uintptr_t x_at = reinterpret_cast<uintptr_t>(x), out_at = reinterpret_cast<uintptr_t>(out);
+  if (x_at < out_at + 2ull * M * N && out_at < x_at + 2ull * ((M - 1) * ldx + K)) p.own = 0;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   int8_t* q = reinterpret_cast<int8_t*>(ws);
   float* scale = reinterpret_cast<float*>(ws + p.q_bytes);

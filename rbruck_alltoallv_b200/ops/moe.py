@@ -317,8 +317,8 @@ def linear_int8(x: torch.Tensor, weight: torch.Tensor, scale: torch.Tensor, out:
 
     ``x`` [rows, K] bf16, ``weight`` [N, K] int8 and ``scale`` [N] fp32 (:func:`quantize_weight_int8`), ``out`` [rows, N] bf16; N a
     multiple of 8, K of 16.  Up to 64 rows the weights are streamed past the rows, split evenly among the SMs
-    (``csrc/kernels/linear_int8_few.cu``); more rows go through the grouped GEMM as one group.  A
-    row that holds an infinity or a NaN becomes NaN.  No backward pass (rows that require a gradient are refused)."""
+    (``csrc/kernels/linear_int8_few.cu``); more rows go through the grouped GEMM as one group.  ``out``
+    may be ``x`` itself, or share memory with it.  A row that holds an infinity or a NaN becomes NaN.  No backward pass (rows that require a gradient are refused)."""
     return _native.torch_ops().linear_int8(x, weight, scale, out, error)
 
 

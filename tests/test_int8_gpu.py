@@ -299,3 +299,24 @@ def test_layer_with_int8_experts(T, H, I, E):
         assert (got.double() - want).norm() <= 0.02 * want.norm()
     finally:
         comm.close()
+
+
+@pytest.mark.parametrize("M,K", [(1, 4096), (2, 2048), (8, 512), (7, 528), (1, 4112), (40, 4096), (64, 1024), (80, 2048)])
+def test_linear_in_place(M, K):
+    """Results over the rows they are made of, wholly and in part, while another stream keeps SMs busy, so that CTAs start one after
+    the other: nobody may read a row that somebody has written over."""
+    from rbruck_alltoallv_b200.ops.moe import linear_int8
+    w, c = _weight((K, K), seed=K)
+    x = _rows(M, K, seed=M)
+    want = linear_int8(x, w, c)
+    big, side = torch.randn(4096, 4096, device="cuda"), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for i in range(10):
+        both = torch.zeros(M * K + 8 * K, dtype=BF, device="cuda")
+        at = i % 2 * 8 * (K // 16)
+        y, out = both[:M * K].view(M, K), both[at:at + M * K].view(M, K)
+        y.copy_(x)
+        with torch.cuda.stream(side):
+            big @ big
+        assert torch.equal(linear_int8(y, w, c, out=out), want)
+    side.synchronize()
