@@ -232,7 +232,9 @@ std::tuple<Tensor, Maybe> block_norm(const Tensor& residual, const Maybe& branch
       gate_kind = RBV_GATE_TOKEN;
     } else {
       gate_kind = RBV_GATE_FULL;
-      if (gate->sizes() != residual.sizes()) g = gate->expand(residual.sizes());
+      // The gradient of an expanded gate is written element by element and then summed: in 32 bits, so that it is rounded once.
+      if (gate->sizes() != residual.sizes())
+        g = (gate->requires_grad() && at::GradMode::is_enabled() ? gate->to(at::kFloat) : *gate).expand(residual.sizes());
     }
   }
   TORCH_CHECK_VALUE(eps >= 0.0, "eps must not be negative");

@@ -251,3 +251,14 @@ def test_several_rows_per_cta(T, H, kind, res, gate):
     if H > 8192 and T > 160:
         T = 160
     _check(*_make(T, H, kind, res, F32, gate, seed=T + H))
+
+
+@pytest.mark.parametrize("kind", [BF, HF])
+@pytest.mark.parametrize("shape", [(2, 1, 72), (1, 300, 1), (300, 1), (1,), (2, 300, 1)])
+def test_gradient_of_a_broadcast_gate_is_rounded_once(kind, shape):
+    """A gate in 16 bits that is shared by many elements: its gradient is a sum of up to 43200 terms and rounded like any other, not
+    term by term.  The sum over 600 or 72 x 600 terms is torch's, a tree of 32-bit additions: within 2^-17 of the magnitudes too."""
+    v, dr2, du = _make(600, 72, kind, F32, F32, "none", seed=6)
+    three = {n: (t.view(2, 300, 72) if t is not None and t.dim() == 2 else t) for n, t in v.items()}
+    three["gate"] = torch.randn(shape, device="cuda", generator=torch.Generator(device="cuda").manual_seed(8)).to(kind)
+    _check(three, dr2.view(2, 300, 72), du.view(2, 300, 72))
