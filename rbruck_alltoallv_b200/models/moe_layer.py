@@ -41,7 +41,8 @@ class MoEBlock:
     front of the next block where ``next_weight`` is given.
 
     ``pre_weight``, ``post_weight``, ``next_weight`` [H] and ``gate`` (per channel, token or element; optional) as
-    :func:`~rbruck_alltoallv_b200.ops.norm.block_norm` takes them; the residual is bf16 or fp32."""
+    :func:`~rbruck_alltoallv_b200.ops.norm.block_norm` takes them; the residual is bf16 or fp32.  The experts and their router
+    have no backward pass: a call that would need one (the normed input, the router or the experts' weights require a gradient) is refused."""
 
     def __init__(self, layer: MoELayer, pre_weight, post_weight, gate=None, scale=1.0, next_weight=None, eps=1e-6):
         if layer.router_weight is None:
@@ -54,6 +55,10 @@ class MoEBlock:
         ``decode``: any number of tokens up to 64, through the layer's :meth:`~MoELayer.decode`."""
         if normed is None:
             _, normed = block_norm(residual, pre_weight=self.pre_weight, eps=self.eps)
+        ep = self.layer.ep
+        if torch.is_grad_enabled() and any(t.requires_grad for t in (normed, self.layer.router_weight, ep.w13, ep.w2)):
+            raise ValueError("the experts have no backward pass: call the block under torch.no_grad(), or with an input norm, a router "
+                             "and experts that want no gradient")
         normed = normed.to(torch.bfloat16)
         out = self.layer.decode(normed) if decode else self.layer(normed)
         return block_norm(residual, out, self.post_weight, self.gate, self.scale, self.next_weight, self.eps)

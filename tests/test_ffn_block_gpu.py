@@ -120,3 +120,23 @@ def test_training_step(kind, res):
     limit = 2.0 ** -16 if kind == F32 else 0.04
     for k in params:
         assert (leaves[k].grad.double() - exact[k].grad).norm() <= limit * exact[k].grad.norm(), k
+
+
+@pytest.mark.parametrize("decode", [False, True])
+def test_a_block_that_would_lose_a_gradient_is_refused(comm, decode):
+    from rbruck_alltoallv_b200.models.moe_layer import MoEBlock, MoELayer
+    w_in, w_post, w_next, gate, router = _weights()
+    layer = MoELayer(comm, E, H, I, T, router_weight=router)
+    x = torch.randn(T, H, device="cuda")
+    for leaf in (w_in, x):
+        leaf.requires_grad_()
+        with pytest.raises(ValueError, match="no backward pass"):
+            MoEBlock(layer, w_in, w_post, gate, 0.5, w_next)(x, decode=decode)
+        with torch.no_grad():
+            assert not MoEBlock(layer, w_in, w_post, gate, 0.5, w_next)(x, decode=decode)[0].requires_grad
+        leaf.requires_grad_(False)
+    w_post.requires_grad_()                              # behind the experts
+    r, u = MoEBlock(layer, w_in, w_post, gate, 0.5, w_next)(x, decode=decode)
+    (r.sum() + u.sum()).backward()
+    layer.ep.check()
+    assert w_post.grad.isfinite().all() and (w_post.grad != 0).any()
