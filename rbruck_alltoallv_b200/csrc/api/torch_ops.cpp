@@ -273,6 +273,7 @@ void int8_weight(const Tensor& w, const Tensor& scale, int64_t dim) {
                     RBV_INT8_MAX_DEPTH, " in steps of 16 are supported, not ", N, " x ", K);
   TORCH_CHECK_VALUE(w.is_contiguous() && scale.is_contiguous() && !misaligned(w) && !misaligned(scale),
                     "weights and scales must be contiguous and 16-byte aligned");
+  no_gradient(scale, "an int8 product");
 }
 
 std::tuple<Tensor, Tensor> quantize_rows_int8(const Tensor& rows, const Maybe& used) {
@@ -296,6 +297,7 @@ Tensor grouped_gemm_int8(const Tensor& Aq, const Tensor& a_scale, const Tensor& 
                         a_scale.scalar_type() == at::kFloat,
                     "rows must be int8 [M, ", K, "] with fp32 scales [M], not ", Aq.sizes(), " in ", Aq.scalar_type(), " with ", a_scale.sizes());
   TORCH_CHECK_VALUE(Aq.is_contiguous() && a_scale.is_contiguous() && !misaligned(Aq), "rows and scales must be contiguous and 16-byte aligned");
+  no_gradient(a_scale, "grouped_gemm_int8");
   TORCH_CHECK_VALUE(G >= 1 && G <= 64, "at most 64 groups, not ", G);
   for (const Tensor* t : {&group_start, &group_rows})
     TORCH_CHECK_VALUE(t->dim() == 1 && t->size(0) == G && t->scalar_type() == at::kInt && t->is_contiguous(),
@@ -358,8 +360,7 @@ Tensor moe_few_tokens(const Tensor& x_, const Tensor& logits_, const Tensor& w13
                       const Maybe& error) {
   TORCH_CHECK_VALUE(x_.dim() == 2 && logits_.dim() == 2 && w13.dim() == 3 && w2.dim() == 3,
                     "x [T, H], logits [T, E], w13 [E, 2 I, H] and w2 [E, H, I] are wanted");
-  no_gradient(x_, "moe_few_tokens");
-  no_gradient(logits_, "moe_few_tokens");
+  for (const Tensor* t : {&x_, &logits_, &w13, &w2}) no_gradient(*t, "moe_few_tokens");
   const int64_t T = x_.size(0), H = x_.size(1), E = w2.size(0), I = w2.size(2);
   TORCH_CHECK_VALUE(x_.scalar_type() == at::kBFloat16 && w13.scalar_type() == at::kBFloat16 && w2.scalar_type() == at::kBFloat16 &&
                         logits_.scalar_type() == at::kFloat,

@@ -282,8 +282,8 @@ def quantize_weight_int8(w: torch.Tensor):
     """bf16 / fp32 [..., N, K] -> (int8 [..., N, K], fp32 scales [..., N]), one scale per output channel.  As in
     :func:`quantize_rows_int8` a channel with an infinity or a NaN gets zeros and the scale NaN, so that what is made of it is
     NaN; one whose values are all so small (below 2^-119) that its scale would not be a normal number becomes zeros with the
-    scale 1."""
-    f = w.float()
+    scale 1.  What comes out has no gradient."""
+    f = w.detach().float()
     amax = f.abs().amax(dim=-1)
     finite = amax.isfinite()
     live = finite & (amax / 127.0 >= torch.finfo(torch.float32).smallest_normal)
@@ -318,7 +318,7 @@ def linear_int8(x: torch.Tensor, weight: torch.Tensor, scale: torch.Tensor, out:
     ``x`` [rows, K] bf16, ``weight`` [N, K] int8 and ``scale`` [N] fp32 (:func:`quantize_weight_int8`), ``out`` [rows, N] bf16; N a
     multiple of 8, K of 16.  Up to 64 rows the weights are streamed past the rows, split evenly among the SMs
     (``csrc/kernels/linear_int8_few.cu``); more rows go through the grouped GEMM as one group.  ``out``
-    may be ``x`` itself, or share memory with it.  A row that holds an infinity or a NaN becomes NaN.  No backward pass (rows that require a gradient are refused)."""
+    may be ``x`` itself, or share memory with it.  A row that holds an infinity or a NaN becomes NaN.  No backward pass (rows and scales that require a gradient are refused)."""
     return _native.torch_ops().linear_int8(x, weight, scale, out, error)
 
 
@@ -344,7 +344,8 @@ def moe_few_tokens(x: torch.Tensor, logits: torch.Tensor, w13: torch.Tensor, w2:
     ``top_k`` is spread over those, and one without any other gets a row of zeros (a padded slot of a batch).  A NaN or +inf among
     a token's logits makes its row NaN.  The number of tokens may change from call to call; weights are read for the experts that
     some token chooses, once each.  The weights are taken to be finite: one that is
-    not spoils the row of every token of a call that reads it.  No backward pass (inputs that require a gradient are refused).
+    not spoils the row of every token of a call that reads it.  No backward pass (inputs and weights that require a gradient are
+    refused, but under ``torch.no_grad()``).
     ``error`` (int32 CUDA tensor): set to non-zero if a bounded wait ran out."""
     return _native.torch_ops().moe_few_tokens(x, logits, w13, w2, top_k, out, error)
 

@@ -90,3 +90,17 @@ def test_weight_quantiser_of_bad_and_tiny_channels(kind):
     for at in ((0, 1), (0, 2), (1, 3), (1, 4), (1, 5), (1, 6)):
         rest[at] = False
     assert torch.equal(q[rest], want[rest]) and torch.equal(s[rest], ws[rest])
+
+
+def test_scales_that_want_a_gradient_are_refused():
+    with pytest.raises(ValueError, match="no backward pass"):
+        linear_int8(**{**_linear(), "scale": torch.ones(16, requires_grad=True)})
+    for name, shape in (("a_scale", (5,)), ("b_scale", (2, 16))):
+        with pytest.raises(ValueError, match="no backward pass"):
+            grouped_gemm_int8(**{**_grouped(), name: torch.ones(shape, requires_grad=True)})
+    with torch.no_grad(), pytest.raises(ValueError, match="on a GPU"):
+        linear_int8(**{**_linear(), "scale": torch.ones(16, requires_grad=True)})
+    q, s = quantize_weight_int8(torch.randn(16, 32, requires_grad=True))      # a trained weight, quantised for serving
+    assert not s.requires_grad
+    with pytest.raises(ValueError, match="on a GPU"):
+        linear_int8(torch.zeros(3, 32, dtype=BF), q, s)

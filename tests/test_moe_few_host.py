@@ -35,3 +35,13 @@ def _args(T=3, H=16, I=24, E=4):
 def test_refusals(change, words):
     with pytest.raises(ValueError, match=words):
         moe_few_tokens(**{**_args(), **change})
+
+
+@pytest.mark.parametrize("name", ["w13", "w2"])
+def test_weights_that_want_a_gradient_are_refused(name):
+    args = _args()
+    args[name].requires_grad_()
+    with pytest.raises(ValueError, match="no backward pass"):
+        moe_few_tokens(**args)
+    with torch.no_grad(), pytest.raises(ValueError, match="on one GPU"):
+        moe_few_tokens(**args)
