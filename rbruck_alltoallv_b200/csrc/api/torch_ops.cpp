@@ -5,6 +5,7 @@
 // the interpreter lock between two threads).  Every kernel is launched on the current stream of its tensors' device, and
 // workspaces belong to one call.
 #include <ATen/ATen.h>
+#include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -46,9 +47,16 @@ int* error_flag(const Maybe& error, const Tensor& like) {
   return error->data_ptr<int>();
 }
 
+// Nothing here has a forward-mode derivative: a tangent is refused rather than dropped.
+void no_tangent(const Tensor& t, const char* what) {
+  TORCH_CHECK_VALUE(!c10::AutogradState::get_tls_state().get_fw_grad_mode() || !t._fw_grad(/*level=*/0).defined(), what,
+                    " has no forward-mode derivative");
+}
+
 // The operators without a backward pass refuse inputs that want one (rather than cut the graph without a word).
 void no_gradient(const Tensor& x, const char* what) {
   TORCH_CHECK_VALUE(!x.requires_grad() || !at::GradMode::is_enabled(), what, " has no backward pass: call it under torch.no_grad()");
+  no_tangent(x, what);
 }
 
 // ---- norms around a block ----------------------------------------------------------------------------------------------
@@ -238,6 +246,9 @@ std::tuple<Tensor, Maybe> block_norm(const Tensor& residual, const Maybe& branch
     }
   }
   TORCH_CHECK_VALUE(eps >= 0.0, "eps must not be negative");
+  no_tangent(residual, "block_norm");
+  for (const Maybe* t : {&branch, &post_weight, &gate, &pre_weight})
+    if (*t) no_tangent(**t, "block_norm");
   TORCH_CHECK_VALUE(residual.is_cuda(), "block_norm runs on a GPU: the tensors are on the host");
   bool graph = residual.requires_grad();
   for (const Maybe* t : {&branch, &post_weight, &gate, &pre_weight}) graph = graph || (*t && (*t)->requires_grad());

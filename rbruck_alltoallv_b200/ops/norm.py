@@ -23,7 +23,7 @@ def block_norm(residual: torch.Tensor, branch: Optional[torch.Tensor] = None, po
                eps: float = 1e-6) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
     """``(residual_out, normed)`` with ``residual_out = residual + scale * gate * rms_norm(branch) * post_weight`` and
     ``normed = rms_norm(residual_out) * pre_weight``, where ``rms_norm(v) = v / sqrt(mean(v ** 2) + eps)`` over the last
-    dimension; one kernel, differentiable (once) in all five tensors.
+    dimension; one kernel, differentiable (once, in reverse mode) in all five tensors.
 
     ``branch`` (the block's output) and ``residual`` are ``[..., hidden]``, in bf16, fp16 or fp32; the residual may be fp32
     next to a 16-bit branch.  Without a branch ``residual_out`` is the residual itself; without ``pre_weight`` ``normed`` is

@@ -104,3 +104,17 @@ def test_scales_that_want_a_gradient_are_refused():
     assert not s.requires_grad
     with pytest.raises(ValueError, match="on a GPU"):
         linear_int8(torch.zeros(3, 32, dtype=BF), q, s)
+
+
+@pytest.mark.parametrize("name", ["x", "scale"])
+def test_tangents_are_refused(name):
+    """There is no forward-mode derivative: a dual number's tangent must not be dropped."""
+    import torch.autograd.forward_ad as fwd
+    args = _linear()
+    with fwd.dual_level():
+        args[name] = fwd.make_dual(args[name], torch.ones_like(args[name]))
+        with pytest.raises(ValueError, match="forward-mode"):
+            linear_int8(**args)
+        args[name] = fwd.unpack_dual(args[name]).primal
+        with pytest.raises(ValueError, match="on a GPU"):
+            linear_int8(**args)

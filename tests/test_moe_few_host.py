@@ -45,3 +45,17 @@ def test_weights_that_want_a_gradient_are_refused(name):
         moe_few_tokens(**args)
     with torch.no_grad(), pytest.raises(ValueError, match="on one GPU"):
         moe_few_tokens(**args)
+
+
+@pytest.mark.parametrize("name", ["x", "logits", "w13", "w2"])
+def test_tangents_are_refused(name):
+    """There is no forward-mode derivative: a dual number's tangent must not be dropped."""
+    import torch.autograd.forward_ad as fwd
+    args = _args()
+    with fwd.dual_level():
+        args[name] = fwd.make_dual(args[name], torch.ones_like(args[name]))
+        with pytest.raises(ValueError, match="forward-mode"):
+            moe_few_tokens(**args)
+        args[name] = fwd.unpack_dual(args[name]).primal
+        with pytest.raises(ValueError, match="on one GPU"):
+            moe_few_tokens(**args)

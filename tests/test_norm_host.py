@@ -62,3 +62,17 @@ def test_oracle_gradients_against_differences(gate):
                 moved[i] += sign * 1e-5
                 at[sign] = loss({**v, name: moved.view_as(t)})
             assert abs((at[1] - at[-1]) / 2e-5 - got[name][0].view(-1)[i].item()) < 1e-6, name
+
+
+@pytest.mark.parametrize("name", ["residual", "branch", "post_weight", "gate", "pre_weight"])
+def test_tangents_are_refused(name):
+    """There is no forward-mode derivative: a dual number's tangent must not be dropped."""
+    import torch.autograd.forward_ad as fwd
+    args = {**_args(), "gate": torch.ones(16)}
+    with fwd.dual_level():
+        args[name] = fwd.make_dual(args[name], torch.ones_like(args[name]))
+        with pytest.raises(ValueError, match="forward-mode"):
+            block_norm(**args)
+        args[name] = fwd.unpack_dual(args[name]).primal
+        with pytest.raises(ValueError, match="on the host"):
+            block_norm(**args)
