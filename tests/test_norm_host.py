@@ -76,3 +76,13 @@ def test_tangents_are_refused(name):
         args[name] = fwd.unpack_dual(args[name]).primal
         with pytest.raises(ValueError, match="on the host"):
             block_norm(**args)
+
+
+def test_a_learnable_scale_is_refused():
+    """``scale`` is a number: a tensor that wants a gradient must not become one without a word (it can be a gate of one element)."""
+    scale = torch.tensor(0.5, requires_grad=True)
+    with pytest.raises(ValueError, match="scale is a number"):
+        block_norm(**{**_args(), "scale": scale})
+    for number in (1, 0.5, scale.detach()):
+        with pytest.raises(ValueError, match="on the host"):
+            block_norm(**{**_args(), "scale": number})
