@@ -13,10 +13,11 @@
 //
 // Two pairs of kernels.  Where there are more rows than SMs, of 2 KB or more, one persistent CTA per SM works on several rows
 // at a time, each by a group of warps of its own (block_norm_rows_*): a row passes through four dependent steps, wait, sum,
-// sum, store, so what keeps HBM busy is rows in work, up to eight forward and two backward (there a thread also holds the
-// sums over the tokens of its columns).  A group's leader fetches its next row into shared memory with one bulk copy per
-// tensor; the weights are in shared memory too.  With one row per CTA of 512 threads and the weights in registers 8192 x 4096
-// in bf16 took 59 us forward, and 4096 x 4096 with the residual in fp32 75 us backward; now 47 and 63.
+// sum, store, so what keeps HBM busy is rows in work: four forward and two backward for 4096 elements (there a thread also holds
+// the sums over the tokens of its columns), up to eight for shorter rows, 32 and 16 for the shortest, of one warp each.  A group's
+// leader fetches its next row into shared memory with one bulk copy per tensor; the weights are in shared memory too.  With one
+// row per CTA of 512 threads and the weights in registers 8192 x 4096 in bf16 took 59 us forward, and 4096 x 4096 with the
+// residual in fp32 75 us backward; now 47 and 63.
 // Short rows, unaligned ones, and few tokens go straight to the registers of one group of threads per row.
 //
 // Sums over the tokens: every thread keeps those of its own columns in registers for all rows of its CTA, and the CTAs' sums
@@ -379,7 +380,7 @@ constexpr int kNormSlots = 64;
 
 struct NormShared {
   uint64_t full[kNormSlots];
-  float red[2][32][16];                     // a sum's parts by turn, group and warp
+  float red[2][32 * 16];                    // a sum's parts by turn, group and warp: 16 warps a group, or one group of up to 32
   int abort;
 };
 
@@ -435,7 +436,7 @@ struct RowGroup {
     #pragma unroll
     for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     if (blockDim.x == 32) return v;
-    float* r = sh.red[turn][group];
+    float* r = sh.red[turn] + group * 16;
     turn ^= 1;
     if ((threadIdx.x & 31) == 0) r[threadIdx.x >> 5] = v;
     sync();

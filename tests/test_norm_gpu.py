@@ -262,3 +262,17 @@ def test_gradient_of_a_broadcast_gate_is_rounded_once(kind, shape):
     three = {n: (t.view(2, 300, 72) if t is not None and t.dim() == 2 else t) for n, t in v.items()}
     three["gate"] = torch.randn(shape, device="cuda", generator=torch.Generator(device="cuda").manual_seed(8)).to(kind)
     _check(three, dr2.view(2, 300, 72), du.view(2, 300, 72))
+
+
+@pytest.mark.parametrize("T", [149, 300, 4800, 9500])
+@pytest.mark.parametrize("gate", ["none", "channel", "token", "full"])
+def test_rows_of_one_warp(T, gate):
+    """512 elements in 32 bits are the shortest rows that go several to a CTA: a group is one warp, up to 32 of them.  9500 rows are
+    65 in the CTA with most, 5 a group: the chains of additions stay below 64."""
+    _check(*_make(T, 512, F32, F32, F32, gate, seed=T))
+
+
+@pytest.mark.parametrize("H", [8200, 12288, 16384])
+@pytest.mark.parametrize("gate", ["none", "full"])
+def test_rows_of_more_than_sixteen_warps(H, gate):
+    _check(*_make(310, H, BF, BF, BF, gate, seed=H))
