@@ -49,7 +49,7 @@ int* error_flag(const Maybe& error, const Tensor& like) {
 
 // Nothing here has a forward-mode derivative: a tangent is refused rather than dropped.
 void no_tangent(const Tensor& t, const char* what) {
-  TORCH_CHECK_VALUE(!c10::AutogradState::get_tls_state().get_fw_grad_mode() || !t._fw_grad(/*level=*/0).defined(), what,
+  TORCH_CHECK_VALUE(!t._fw_grad(/*level=*/0).defined() || !c10::AutogradState::get_tls_state().get_fw_grad_mode(), what,
                     " has no forward-mode derivative");
 }
 

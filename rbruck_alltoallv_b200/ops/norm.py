@@ -33,6 +33,6 @@ def block_norm(residual: torch.Tensor, branch: Optional[torch.Tensor] = None, po
     strided (elements of a row packed).  Launched on the current stream of the tensors' device; both passes can be captured into a
     graph, the backward pass while no graph of an earlier, eager pass through the same leaves is alive (torch would accumulate into
     them on that pass's stream, which a capture does not survive)."""
-    if isinstance(scale, torch.Tensor) and scale.requires_grad and torch.is_grad_enabled():
+    if type(scale) is not float and isinstance(scale, torch.Tensor) and scale.requires_grad and torch.is_grad_enabled():
         raise ValueError("scale is a number: one that is learned goes into the gate")
     return _native.torch_ops().block_norm(residual, branch, post_weight, gate, scale, pre_weight, eps)
