@@ -380,7 +380,7 @@ constexpr int kNormSlots = 64;
 
 struct NormShared {
   uint64_t full[kNormSlots];
-  float red[2][32 * 16];                    // a sum's parts by turn, group and warp: 16 warps a group, or one group of up to 32
+  float red[2][16][32];                     // a sum's parts by turn, group (of several warps: 8 at most) and warp (32 at most)
   int abort;
 };
 
@@ -436,7 +436,7 @@ struct RowGroup {
     #pragma unroll
     for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     if (blockDim.x == 32) return v;
-    float* r = sh.red[turn] + group * 16;
+    float* r = sh.red[turn][group];
     turn ^= 1;
     if ((threadIdx.x & 31) == 0) r[threadIdx.x >> 5] = v;
     sync();
