@@ -973,7 +973,9 @@ Shape choose_shape(const rbv_norm_t& a, bool backward, int sms) {
   bool ok = a.H % vec == 0 && aligned(a.z, a.z_ld, vec, zs) && aligned(a.r, a.r_ld, vec, rs) && aligned(a.w1, 0, vec, zs) &&
             aligned(a.w2, 0, vec, zs) && (a.gate_kind != RBV_GATE_CHANNEL || aligned(a.gate, 0, vec, zs)) &&
             (a.gate_kind != RBV_GATE_FULL || aligned(a.gate, a.gate_ld, vec, zs));
-  if (backward) ok = ok && aligned(a.dr2, a.dr2_ld, vec, rs) && aligned(a.du, a.du_ld, vec, zs) && aligned(a.dz, a.H, vec, zs) && aligned(a.dr, a.H, vec, rs);
+  if (backward)
+    ok = ok && aligned(a.dr2, a.dr2_ld, vec, rs) && aligned(a.du, a.du_ld, vec, zs) && aligned(a.dz, a.H, vec, zs) && aligned(a.dr, a.H, vec, rs) &&
+         (a.gate_kind != RBV_GATE_FULL || aligned(a.dgate, a.H, vec, zs)) && aligned(a.partial, 0, vec, zs);
   else ok = ok && aligned(a.r2, a.H, vec, rs) && aligned(a.u, a.H, vec, zs);
   const size_t bytes = row_bytes(a, backward);
   if (ok && (size_t)a.H * zs >= 2048 && a.T > sms && bytes > 0) {
