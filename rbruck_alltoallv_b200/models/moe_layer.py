@@ -53,8 +53,9 @@ class MoEBlock:
     def forward(self, residual, normed=None, decode=False):
         """``(residual, normed)`` behind the block from those in front of it; ``normed`` may be left out for the first block.
         ``decode``: any number of tokens up to 64, through the layer's :meth:`~MoELayer.decode`."""
-        if normed is None:
-            _, normed = block_norm(residual, pre_weight=self.pre_weight, eps=self.eps)
+        if normed is None:                     # (with no block's output in 16 bits the weight has the residual's type or is fp32)
+            weight = self.pre_weight.float() if residual.dtype == torch.float32 else self.pre_weight
+            _, normed = block_norm(residual, pre_weight=weight, eps=self.eps)
         ep = self.layer.ep
         if torch.is_grad_enabled() and any(t.requires_grad for t in (normed, self.layer.router_weight, ep.w13, ep.w2)):
             raise ValueError("the experts have no backward pass: call the block under torch.no_grad(), or with an input norm, a router "

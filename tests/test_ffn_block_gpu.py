@@ -140,3 +140,18 @@ def test_a_block_that_would_lose_a_gradient_is_refused(comm, decode):
     (r.sum() + u.sum()).backward()
     layer.ep.check()
     assert w_post.grad.isfinite().all() and (w_post.grad != 0).any()
+
+
+@pytest.mark.parametrize("decode", [False, True])
+def test_weights_in_16_bits_next_to_a_residual_in_32(comm, decode):
+    """Bit for bit the block with the same weights in 32 bits."""
+    from rbruck_alltoallv_b200.models.moe_layer import MoEBlock, MoELayer
+    *weights, router = [w.to(BF) for w in _weights()]
+    layer = MoELayer(comm, E, H, I, T, router_weight=router)
+    x = torch.randn(T, H, device="cuda")
+    w_in, w_post, w_next, gate = weights
+    got = MoEBlock(layer, w_in, w_post, gate, 0.5, w_next)(x, decode=decode)
+    w_in, w_post, w_next, gate = [w.float() for w in weights]
+    want = MoEBlock(layer, w_in, w_post, gate, 0.5, w_next)(x, decode=decode)
+    layer.ep.check()
+    assert all(torch.equal(a, b) for a, b in zip(got, want)) and got[0].dtype == F32 and got[1].dtype == BF

@@ -50,3 +50,12 @@ def test_gradients_around_the_experts_are_not_refused():
     block = MoEBlock(Layer(), _ones(), _ones(trainable=True), gate=_ones(trainable=True), next_weight=_ones(trainable=True))
     with pytest.raises(LookupError):
         block(torch.zeros(3, H, requires_grad=True), _normed())
+
+
+@pytest.mark.parametrize("weight", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("residual", [torch.bfloat16, torch.float32])
+def test_the_first_norm_takes_weights_of_either_type(weight, residual):
+    """(refused for the host's tensors, not for their types)"""
+    block = MoEBlock(Layer(), _ones().to(weight), _ones().to(weight))
+    with pytest.raises(ValueError, match="on the host"):
+        block(torch.zeros(3, H, dtype=residual))
