@@ -282,6 +282,7 @@ void int8_weight(const Tensor& w, const Tensor& scale, int64_t dim) {
   const int64_t N = w.size(-2), K = w.size(-1);
   TORCH_CHECK_VALUE(N >= 8 && N % 8 == 0 && K >= 16 && K % 16 == 0 && K <= RBV_INT8_MAX_DEPTH, "channels in steps of 8 and depths of 16 to ",
                     RBV_INT8_MAX_DEPTH, " in steps of 16 are supported, not ", N, " x ", K);
+  TORCH_CHECK_VALUE(w.numel() / K <= RBV_INT8_MAX_CHANNELS, "at most ", RBV_INT8_MAX_CHANNELS, " channels in all groups, not ", w.numel() / K);
   TORCH_CHECK_VALUE(w.is_contiguous() && scale.is_contiguous() && !misaligned(w) && !misaligned(scale),
                     "weights and scales must be contiguous and 16-byte aligned");
   no_gradient(scale, "an int8 product");
@@ -351,7 +352,9 @@ Tensor linear_int8(const Tensor& rows, const Tensor& weight, const Tensor& scale
   if (M == 0) return out;
   int* err = error_flag(error, x);
   if (M <= RBV_FEW_ROWS) {
-    Tensor ws = empty({rbv_linear_int8_few_workspace((int)M, (int)N, (int)K)}, at::kByte, x);
+    const long long bytes = rbv_linear_int8_few_workspace((int)M, (int)N, (int)K);
+    TORCH_CHECK_VALUE(bytes >= 0, "weights of ", N, " x ", K, " are too large for a few rows");
+    Tensor ws = empty({bytes}, at::kByte, x);
     launched(rbv_linear_int8_few(x.data_ptr(), row_step(x), (int)M, weight.data_ptr(), scale.data_ptr<float>(), (int)N, (int)K, out.data_ptr(),
                                  ws.data_ptr(), err, stream_of(x)),
              "int8 linear");

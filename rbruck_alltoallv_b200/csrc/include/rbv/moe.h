@@ -63,6 +63,7 @@ int rbv_grouped_gemm_fp8_tok(const void* A, const float* a_scale_t, long long a_
  * group_start and group_rows null with G = 1: one group of all rows.  error_flag may be null. */
 #define RBV_INT8_MAX_DEPTH 131072
 #define RBV_INT8_MAX_ROWS 0x7fffff00     /* rows of an int8 GEMM at most (row numbers and a tile beyond them fit an int) */
+#define RBV_INT8_MAX_CHANNELS 0x7fffff00 /* and channels of all groups together */
 int rbv_grouped_gemm_int8(const void* A, const float* a_scale, long long a_rows, const void* B, const float* b_scale,
                           void* C, const int* group_start, const int* group_rows, int G, int N, int K, int ldc,
                           int epilogue, int* error_flag, int max_ctas, void* cuda_stream);

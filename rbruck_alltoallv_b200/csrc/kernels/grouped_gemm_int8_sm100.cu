@@ -306,7 +306,7 @@ extern "C" int rbv_grouped_gemm_int8(const void* A, const float* a_scale, long l
                                      int epilogue, int* error_flag, int max_ctas, void* cuda_stream) {
   using namespace rbv;
   if (G < 1 || G > kMoeMaxGroups || N < 8 || N % 8 || K < 16 || K % 16 || K > RBV_INT8_MAX_DEPTH || a_rows < 1 || a_rows > RBV_INT8_MAX_ROWS ||
-      ldc % 2 || (long long)G * N > 0x7fffffffll || epilogue < 0 || epilogue > 1)
+      ldc % 2 || (long long)G * N > RBV_INT8_MAX_CHANNELS || epilogue < 0 || epilogue > 1)
     return (int)cudaErrorInvalidValue;
   if ((!group_start) != (!group_rows) || (!group_start && G != 1)) return (int)cudaErrorInvalidValue;
   if (((reinterpret_cast<uintptr_t>(A) | reinterpret_cast<uintptr_t>(B)) & 15) || (reinterpret_cast<uintptr_t>(C) & 3))

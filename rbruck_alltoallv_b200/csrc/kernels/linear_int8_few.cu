@@ -243,7 +243,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_int8_few_kernel(const __gr
 struct LinearPlan { int sms, tile, whole, own; size_t q_bytes, scale_bytes, partial_bytes, counter_bytes; };
 
 bool linear_plan(int M, int N, int K, LinearPlan* p) {
-  if (M < 1 || M > kMaxRows || N < 8 || K < 16 || N % 8 || K % 16 || K > RBV_INT8_MAX_DEPTH) return false;
+  if (M < 1 || M > kMaxRows || N < 8 || K < 16 || N % 8 || K % 16 || K > RBV_INT8_MAX_DEPTH || N > RBV_INT8_MAX_CHANNELS) return false;
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&p->sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return false;
   if (!split_plan(N, K, 1, p->sms, M, box_rows(M) / 8, false, &p->tile, &p->whole)) return false;

@@ -118,3 +118,15 @@ def test_tangents_are_refused(name):
         args[name] = fwd.unpack_dual(args[name]).primal
         with pytest.raises(ValueError, match="on a GPU"):
             linear_int8(**args)
+
+
+@pytest.mark.parametrize("channels", [2 ** 32 + 8, 2 ** 31 - 8])
+def test_channels_beyond_an_int_are_refused(channels):
+    """Channel numbers, and a tile beyond them, are 32-bit integers in the kernels: 2^32 + 8 channels must not become 8."""
+    weight, scale = torch.zeros(1, 16, dtype=I8).expand(channels, 16), torch.ones(1).expand(channels)
+    with pytest.raises(ValueError, match="at most 2147483392 channels"):
+        linear_int8(torch.zeros(3, 16, dtype=BF), weight, scale)
+    per_group = channels // 64 * 8
+    with pytest.raises(ValueError, match="at most 2147483392 channels"):
+        grouped_gemm_int8(**{**_grouped(G=8, K=16), "Bq": weight[:per_group].expand(8, per_group, 16),
+                             "b_scale": scale[:per_group].expand(8, per_group)})
