@@ -12,6 +12,7 @@
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
 
+#include <initializer_list>
 #include <optional>
 #include <tuple>
 #include <vector>
@@ -38,6 +39,22 @@ Tensor packed_rows(const Tensor& x, int64_t step) {
   return x;
 }
 int64_t row_step(const Tensor& x) { return x.size(0) > 1 ? x.stride(0) : x.size(1); }
+
+// Results over an operand that other CTAs still read would be a race.
+void apart(const Tensor& out, std::initializer_list<const Tensor*> operands, const char* what) {
+  auto span = [](const Tensor& t) {
+    int64_t last = 0;
+    for (int64_t i = 0; i < t.dim(); i++) last += (t.size(i) - 1) * t.stride(i);
+    const auto at = reinterpret_cast<uintptr_t>(t.data_ptr());
+    return std::pair<uintptr_t, uintptr_t>(at, at + (last + 1) * t.element_size());
+  };
+  const auto [begin, end] = span(out);
+  for (const Tensor* t : operands) {
+    if (t->numel() == 0) continue;
+    const auto [from, to] = span(*t);
+    TORCH_CHECK_VALUE(to <= begin || end <= from, "out must not share memory with ", what);
+  }
+}
 
 // A kernel's error flag, if the caller wants to know.
 int* error_flag(const Maybe& error, const Tensor& like) {
@@ -327,6 +344,7 @@ Tensor grouped_gemm_int8(const Tensor& Aq, const Tensor& a_scale, const Tensor& 
                           out.device() == Aq.device() && out.stride(1) == 1 && !misaligned(out, 4) &&
                           (M <= 1 || (out.stride(0) % 2 == 0 && out.stride(0) >= n_out && out.stride(0) <= 0x7fffffff)),
                       "out must be a bf16 tensor [", M, ", ", n_out, "] with packed, 4-byte aligned rows on the same GPU");
+  if (out_ && M) apart(out, {&Aq, &a_scale, &Bq, &b_scale, &group_start, &group_rows}, "an operand");
   if (M)
     launched(rbv_grouped_gemm_int8(Aq.data_ptr(), a_scale.data_ptr<float>(), M, Bq.data_ptr(), b_scale.data_ptr<float>(), out.data_ptr(),
                                    group_start.data_ptr<int>(), group_rows.data_ptr<int>(), (int)G, (int)N, (int)K, (int)row_step(out), swiglu ? 1 : 0,
@@ -350,6 +368,7 @@ Tensor linear_int8(const Tensor& rows, const Tensor& weight, const Tensor& scale
                           out.is_contiguous() && !misaligned(out),
                       "out must be a contiguous, 16-byte aligned bf16 tensor [", M, ", ", N, "] on the same GPU");
   if (M == 0) return out;
+  if (out_) apart(out, {&weight, &scale}, "the weights or their scales");
   int* err = error_flag(error, x);
   if (M <= RBV_FEW_ROWS) {
     const long long bytes = rbv_linear_int8_few_workspace((int)M, (int)N, (int)K);
@@ -397,6 +416,7 @@ Tensor moe_few_tokens(const Tensor& x_, const Tensor& logits_, const Tensor& w13
                           out.is_contiguous() && !misaligned(out),
                       "out must be a contiguous, 16-byte aligned bf16 tensor [T, H] on the same GPU");
   if (T == 0) return out;
+  if (out_) apart(out, {&logits_, &w13, &w2}, "the logits or the weights");      // (the tokens are read before)
   const Tensor x = packed_rows(x_, 8);
   Tensor logits = logits_;
   if ((E > 1 && logits.stride(1) != 1) || (T > 1 && logits.stride(0) < E)) logits = logits.contiguous();

@@ -306,7 +306,8 @@ def grouped_gemm_int8(Aq: torch.Tensor, a_scale: torch.Tensor, Bq: torch.Tensor,
     ``Aq`` [M, K] int8 with ``a_scale`` [M], ``Bq`` [G, N, K] int8 with ``b_scale`` [G, N], ``group_start`` / ``group_rows`` int32
     CUDA tensors [G], G <= 64; N a multiple of 8, K of 16.  With ``swiglu`` the rows of ``Bq[g]`` interleave gate and up projections
     and ``out`` is [M, N // 2].  Rows of ``out`` outside the groups are left as they are; rows of a group beyond the end of ``Aq``, and
-    a group that starts before it, are left out and recorded as error 6 in ``error`` (int32 CUDA tensor, optional)."""
+    a group that starts before it, are left out and recorded as error 6 in ``error`` (int32 CUDA tensor, optional).  ``out`` shares no
+    memory with an operand."""
     return _native.torch_ops().grouped_gemm_int8(Aq, a_scale, Bq, b_scale, group_start, group_rows, out, swiglu, error, max_ctas)
 
 
@@ -318,7 +319,7 @@ def linear_int8(x: torch.Tensor, weight: torch.Tensor, scale: torch.Tensor, out:
     ``x`` [rows, K] bf16, ``weight`` [N, K] int8 and ``scale`` [N] fp32 (:func:`quantize_weight_int8`), ``out`` [rows, N] bf16; N a
     multiple of 8, K of 16.  Up to 64 rows the weights are streamed past the rows, split evenly among the SMs
     (``csrc/kernels/linear_int8_few.cu``); more rows go through the grouped GEMM as one group.  ``out``
-    may be ``x`` itself, or share memory with it.  A row that holds an infinity or a NaN becomes NaN.  No backward pass (rows and scales that require a gradient are refused)."""
+    may be ``x`` itself, or share memory with it (but not with the weights).  A row that holds an infinity or a NaN becomes NaN.  No backward pass (rows and scales that require a gradient are refused)."""
     return _native.torch_ops().linear_int8(x, weight, scale, out, error)
 
 
@@ -346,7 +347,8 @@ def moe_few_tokens(x: torch.Tensor, logits: torch.Tensor, w13: torch.Tensor, w2:
     some token chooses, once each.  The weights are taken to be finite: one that is
     not spoils the row of every token of a call that reads it.  No backward pass (inputs and weights that require a gradient are
     refused, but under ``torch.no_grad()``).
-    ``error`` (int32 CUDA tensor): set to non-zero if a bounded wait ran out."""
+    ``out`` may be ``x`` itself, but shares no memory with the logits or the weights.  ``error`` (int32 CUDA tensor): set to non-zero
+    if a bounded wait ran out."""
     return _native.torch_ops().moe_few_tokens(x, logits, w13, w2, top_k, out, error)
 
 

@@ -320,3 +320,26 @@ def test_linear_in_place(M, K):
             big @ big
         assert torch.equal(linear_int8(y, w, c, out=out), want)
     side.synchronize()
+
+
+def test_results_over_operands_are_refused():
+    from rbruck_alltoallv_b200.ops.moe import grouped_gemm_int8, linear_int8
+    raw = torch.zeros(1 << 16, dtype=torch.uint8, device="cuda")
+    as_bf = lambda at, *shape: raw[at:].view(BF)[:math.prod(shape)].view(shape)
+    w, c = raw[:64 * 64].view(I8).view(64, 64), raw[4096:4096 + 256].view(torch.float32)
+    for M in (4, 70):
+        x = _rows(M, 64)
+        for at in (0, 2048, 4096, 4096 + 240):
+            with pytest.raises(ValueError, match="must not share memory"):
+                linear_int8(x, w, c, out=as_bf(at, M, 64))
+        linear_int8(x, w, c, out=as_bf(4096 + 256, M, 64))              # right behind them
+    q, s = raw[8192:8192 + 70 * 64].view(I8).view(70, 64), torch.ones(70, device="cuda")
+    gs, gr = torch.zeros(1, dtype=I32, device="cuda"), torch.full((1,), 70, dtype=I32, device="cuda")
+    for at in (0, 4096, 8192, 8192 + 70 * 64 - 16):
+        with pytest.raises(ValueError, match="must not share memory"):
+            grouped_gemm_int8(q, s, w[None], c[None], gs, gr, out=as_bf(at, 70, 64))
+    for at in (0, 16):
+        with pytest.raises(ValueError, match="must not share memory"):
+            grouped_gemm_int8(_plain_rows(_rows(70, 64))[0], raw[16384:16384 + 280].view(torch.float32), w[None].clone(), c[None].clone(), gs, gr,
+                              out=as_bf(16384 + at, 70, 64))
+    grouped_gemm_int8(q, s, w[None], c[None], gs, gr, out=as_bf(16384, 70, 64))

@@ -208,3 +208,14 @@ def test_layer_decode():
             fp8.decode(x[:4], torch.zeros(4, E, device="cuda"))
     finally:
         comm.close()
+
+
+def test_results_over_operands_are_refused():
+    from rbruck_alltoallv_b200.ops.moe import moe_few_tokens
+    x, logits, w13, w2 = _make(5, 64, 40, 8)
+    shared = torch.zeros(5 * 64, dtype=BF, device="cuda")
+    over = shared[:80].view(torch.float32).view(5, 8)
+    over.copy_(logits)
+    for scores, out in ((over, shared), (logits, w2.view(-1)[64:64 + 5 * 64]), (logits, w13.view(-1)[:5 * 64])):
+        with pytest.raises(ValueError, match="must not share memory"):
+            moe_few_tokens(x, scores, w13, w2, out=out.view(5, 64))
