@@ -76,6 +76,12 @@ void no_gradient(const Tensor& x, const char* what) {
   no_tangent(x, what);
 }
 
+// A result's tensor that the caller gave: not one that wants a gradient, and autograd learns that it was written.
+void written(const Tensor& out, const char* what) {
+  no_gradient(out, what);
+  if (!out.is_inference()) out.unsafeGetTensorImpl()->bump_version();
+}
+
 // ---- norms around a block ----------------------------------------------------------------------------------------------
 int norm_type(at::ScalarType t) {
   return t == at::kBFloat16 ? RBV_NORM_BF16 : t == at::kHalf ? RBV_NORM_FP16 : t == at::kFloat ? RBV_NORM_FP32 : -1;
@@ -344,7 +350,10 @@ Tensor grouped_gemm_int8(const Tensor& Aq, const Tensor& a_scale, const Tensor& 
                           out.device() == Aq.device() && out.stride(1) == 1 && !misaligned(out, 4) &&
                           (M <= 1 || (out.stride(0) % 2 == 0 && out.stride(0) >= n_out && out.stride(0) <= 0x7fffffff)),
                       "out must be a bf16 tensor [", M, ", ", n_out, "] with packed, 4-byte aligned rows on the same GPU");
-  if (out_ && M) apart(out, {&Aq, &a_scale, &Bq, &b_scale, &group_start, &group_rows}, "an operand");
+  if (out_ && M) {
+    apart(out, {&Aq, &a_scale, &Bq, &b_scale, &group_start, &group_rows}, "an operand");
+    written(out, "grouped_gemm_int8");
+  }
   if (M)
     launched(rbv_grouped_gemm_int8(Aq.data_ptr(), a_scale.data_ptr<float>(), M, Bq.data_ptr(), b_scale.data_ptr<float>(), out.data_ptr(),
                                    group_start.data_ptr<int>(), group_rows.data_ptr<int>(), (int)G, (int)N, (int)K, (int)row_step(out), swiglu ? 1 : 0,
@@ -368,7 +377,10 @@ Tensor linear_int8(const Tensor& rows, const Tensor& weight, const Tensor& scale
                           out.is_contiguous() && !misaligned(out),
                       "out must be a contiguous, 16-byte aligned bf16 tensor [", M, ", ", N, "] on the same GPU");
   if (M == 0) return out;
-  if (out_) apart(out, {&weight, &scale}, "the weights or their scales");
+  if (out_) {
+    apart(out, {&weight, &scale}, "the weights or their scales");
+    written(out, "linear_int8");
+  }
   int* err = error_flag(error, x);
   if (M <= RBV_FEW_ROWS) {
     const long long bytes = rbv_linear_int8_few_workspace((int)M, (int)N, (int)K);
@@ -416,7 +428,10 @@ Tensor moe_few_tokens(const Tensor& x_, const Tensor& logits_, const Tensor& w13
                           out.is_contiguous() && !misaligned(out),
                       "out must be a contiguous, 16-byte aligned bf16 tensor [T, H] on the same GPU");
   if (T == 0) return out;
-  if (out_) apart(out, {&logits_, &w13, &w2}, "the logits or the weights");      // (the tokens are read before)
+  if (out_) {
+    apart(out, {&logits_, &w13, &w2}, "the logits or the weights");              // (the tokens are read before)
+    written(out, "moe_few_tokens");
+  }
   const Tensor x = packed_rows(x_, 8);
   Tensor logits = logits_;
   if ((E > 1 && logits.stride(1) != 1) || (T > 1 && logits.stride(0) < E)) logits = logits.contiguous();

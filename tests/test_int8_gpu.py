@@ -343,3 +343,29 @@ def test_results_over_operands_are_refused():
             grouped_gemm_int8(_plain_rows(_rows(70, 64))[0], raw[16384:16384 + 280].view(torch.float32), w[None].clone(), c[None].clone(), gs, gr,
                               out=as_bf(16384 + at, 70, 64))
     grouped_gemm_int8(q, s, w[None], c[None], gs, gr, out=as_bf(16384, 70, 64))
+
+
+@pytest.mark.parametrize("M", [3, 70])
+@pytest.mark.parametrize("which", ["linear", "grouped", "moe"])
+def test_results_written_over_what_a_graph_has_saved(M, which):
+    """Autograd has to learn that ``out`` was written: a gradient made from the new values would be wrong without a word."""
+    from rbruck_alltoallv_b200.ops.moe import grouped_gemm_int8, linear_int8, moe_few_tokens
+    from rbruck_alltoallv_b200.ops.norm import block_norm
+    if which == "moe":
+        M = min(M, 64)
+    (w, c), x = _weight((64, 64)), _rows(M, 64)
+    q, s = _plain_rows(x)
+    gs, gr = torch.zeros(1, dtype=I32, device="cuda"), torch.full((1,), M, dtype=I32, device="cuda")
+    w13, w2, logits = _rows(2 * 2 * 40, 64).view(2, 80, 64), _rows(2 * 64, 40).view(2, 64, 40), torch.zeros(M, 2, device="cuda")
+    call = {"linear": lambda out: linear_int8(x, w, c, out=out), "grouped": lambda out: grouped_gemm_int8(q, s, w[None], c[None], gs, gr, out=out),
+            "moe": lambda out: moe_few_tokens(x, logits, w13, w2, out=out)}[which]
+    out, weight = torch.empty(M, 64, dtype=BF, device="cuda"), torch.ones(64, device="cuda", requires_grad=True)
+    call(out)
+    r, _ = block_norm(torch.zeros(M, 64, dtype=BF, device="cuda"), out, weight)
+    call(out)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        r.float().sum().backward()
+    with pytest.raises(ValueError, match="no backward pass"):
+        call(torch.empty(M, 64, dtype=BF, device="cuda", requires_grad=True))
+    with torch.inference_mode():
+        call(torch.empty(M, 64, dtype=BF, device="cuda"))
