@@ -899,8 +899,8 @@ cudaError_t launch_shape(const rbv_norm_t& a, const Shape& s, cudaStream_t st) {
   else kernel = full ? block_norm_kernel<TZ, TR, VEC, NV, MAXT, true> : block_norm_kernel<TZ, TR, VEC, NV, MAXT, false>;
   int grid = s.grid;
   if (!BACKWARD && grid > s.sms) {          // more rows than CTAs that fit at once: as many persistent CTAs as do
-    static std::atomic<int> fits[33];       // CTAs per SM by warps per CTA, 0: not asked yet
-    std::atomic<int>& known = fits[s.threads * s.rows / 32];
+    static std::atomic<int> fits[2][33];    // CTAs per SM by kernel and warps per CTA, 0: not asked yet
+    std::atomic<int>& known = fits[full][s.threads * s.rows / 32];
     int n = known.load(std::memory_order_relaxed);
     if (n == 0) {
       const cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, s.threads * s.rows, 0);
