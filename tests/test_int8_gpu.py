@@ -369,3 +369,32 @@ def test_results_written_over_what_a_graph_has_saved(M, which):
         call(torch.empty(M, 64, dtype=BF, device="cuda", requires_grad=True))
     with torch.inference_mode():
         call(torch.empty(M, 64, dtype=BF, device="cuda"))
+
+
+def test_offsets_beyond_32_bits():
+    """Rows, weights and results of more than 2^31 elements each: their last parts, from 64 bits."""
+    from rbruck_alltoallv_b200.ops.moe import grouped_gemm_int8, linear_int8, quantize_rows_int8
+    K = 16384
+    M = 2 ** 31 // K + 5
+    x = torch.zeros(M, K, dtype=BF, device="cuda")
+    x[-5:] = _rows(5, K)
+    q, s = quantize_rows_int8(x)
+    want, ws = _plain_rows(x[-5:])
+    assert torch.equal(q[-5:], want) and torch.equal(s[-5:], ws) and (q[:-5] == 0).all()
+    del x
+    N = 2 ** 31 // K + 8                                     # the rows' integers as weights of as many channels
+    w, c = torch.zeros(N, K, dtype=I8, device="cuda"), torch.ones(N, device="cuda")
+    w[-16:], c[-16:] = _weight((16, K))
+    for rows in (3, 70):
+        y = _rows(rows, K, seed=rows)
+        got = linear_int8(y, w, c)
+        _check(got[:, -16:], _want(*_plain_rows(y), w[-16:], c[-16:]))
+        assert (got[:, :-16] == 0).all()
+    del w, q
+    rows, N = 2 ** 31 // 32768 + 70, 32768                   # results
+    (w, c), y = _weight((N, 16)), _rows(rows, 16)
+    q, s = _plain_rows(y)
+    gs, gr = torch.tensor([0, rows - 70], dtype=I32, device="cuda"), torch.tensor([rows - 70, 70], dtype=I32, device="cuda")
+    got = grouped_gemm_int8(q, s, torch.stack([w, w]), torch.stack([c, c]), gs, gr)
+    for at in (0, rows - 200, rows - 100):
+        _check(got[at:at + 100], _want(q[at:at + 100], s[at:at + 100], w, c))

@@ -219,3 +219,27 @@ def test_results_over_operands_are_refused():
     for scores, out in ((over, shared), (logits, w2.view(-1)[64:64 + 5 * 64]), (logits, w13.view(-1)[:5 * 64])):
         with pytest.raises(ValueError, match="must not share memory"):
             moe_few_tokens(x, scores, w13, w2, out=out.view(5, 64))
+
+
+def test_a_token_alone_and_in_a_batch():
+    """The cut of the work depends on the batch, and with it the order of sums: a token agrees with itself within both bounds."""
+    from rbruck_alltoallv_b200.ops.moe import moe_few_tokens
+    x, logits, w13, w2 = _make(64, 512, 704, 16, seed=4)
+    want, bound = moe_few_oracle.layer(x, logits, w13, w2, 2)
+    limit = (want.abs() + bound) * 2.0 ** -8 + bound
+    whole = moe_few_tokens(x, logits, w13, w2).double()
+    for n in (1, 2, 9, 17, 33):
+        part = moe_few_tokens(x[:n], logits[:n], w13, w2).double()
+        assert ((part - whole[:n]).abs() <= 2 * limit[:n]).all()
+
+
+def test_weights_beyond_32_bits():
+    E, H, I = 24, 4096, 14336                                # 2.8e9 elements of w13
+    w13, w2 = torch.zeros(E, 2 * I, H, dtype=BF, device="cuda"), torch.zeros(E, H, I, dtype=BF, device="cuda")
+    x, logits, a, b = _make(5, H, I, 2)
+    w13[22:], w2[22:] = a, b
+    scores = torch.full((5, E), -1e4, device="cuda")
+    scores[:, 22:] = logits
+    for T in (1, 5):
+        got = _check(x[:T], scores[:T], w13, w2, 2)
+        assert (got != 0).any()

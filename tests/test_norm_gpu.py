@@ -276,3 +276,36 @@ def test_rows_of_one_warp(T, gate):
 @pytest.mark.parametrize("gate", ["none", "full"])
 def test_rows_of_more_than_sixteen_warps(H, gate):
     _check(*_make(310, H, BF, BF, BF, gate, seed=H))
+
+
+@pytest.mark.parametrize("T", [300, 1189])
+@pytest.mark.parametrize("H", [131, 1001, 4097, 8191])
+@pytest.mark.parametrize("gate", ["none", "channel", "token", "full"])
+@pytest.mark.parametrize("kind,res", [(F32, F32), (BF, F32), (HF, HF)])
+def test_widths_that_are_not_whole_vectors_over_many_rows(T, H, gate, kind, res):
+    """More rows than CTAs fit at once: a CTA of single elements goes on to its next row, and sums over several."""
+    _check(*_make(T, H, kind, res, F32, gate, seed=T + H))
+
+
+def test_offsets_beyond_32_bits():
+    """More than 2^31 elements: the last rows are those of a call on them alone, in both passes and with a gate per element.  (Both
+    calls have more rows than SMs, so that they take the same kernels; the sums over the tokens are left out.)"""
+    from rbruck_alltoallv_b200.ops.norm import block_norm
+    H, tail = 4096, 300
+    T = 2 ** 31 // H + tail
+    v, dr2, du = _make(tail, H, BF, BF, F32, "full")
+    rows = {n: t for n, t in v.items() if t.dim() == 2} | {"dr2": dr2, "du": du}
+    big = {}
+    for n, t in rows.items():
+        big[n] = torch.zeros(T, H, dtype=BF, device="cuda")
+        big[n][-tail:] = t
+    for s in (rows, big):
+        for n in ("residual", "branch", "gate"):
+            s[n].requires_grad_()
+    results = []
+    for s in (rows, big):
+        out = block_norm(s["residual"], s["branch"], v["post_weight"], s["gate"], 0.5, v["pre_weight"])
+        grads = torch.autograd.grad(out, [s["residual"], s["branch"], s["gate"]], (s["dr2"], s["du"]))
+        results.append([t.detach()[-tail:] for t in (*out, *grads)])
+    for a, b in zip(*results):
+        assert torch.equal(a, b)
