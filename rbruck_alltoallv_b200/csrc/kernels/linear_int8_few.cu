@@ -6,9 +6,11 @@
 // a tile that several CTAs share are exact in any order.
 //
 // Up to 4096 elements of A in at most 8 rows, and tiles that are not split: one kernel, in which every CTA quantises the rows for
-// itself (they come out of L2) while its first weights are on their way.  4096 x 4096, one row: 7.9 us with two kernels, 6.2 with
-// one, from Python 7.3 and 5.9.  Four times the elements, eight vectors per thread, cost more than the second kernel (4 rows: 11.4
-// us, 7.9 with two).  Results that are written over the rows take two kernels.
+// itself (they come out of L2) while its first weights are on their way.  4096 x 4096, one row: 7.9 us with two kernels, 6.0 with
+// one.  4096 is what two vectors per thread hold, not where the times cross.  Both forms (one kernel with four vectors per thread
+// up to 8192 elements, with eight up to 16384), 4096 channels, graph replays: one row of 5120 9.0 us with two kernels, 6.7 with one
+// of four vectors, 7.6 of eight; of 8192 11.1, 8.8, 9.9; of 14336 14.9, -, 15.3; four rows of 2048 5.9, 6.6, 7.3; of 4096 7.9, -,
+// 11.1; and one row of 4096 itself 5.9, 5.9, 6.7.  Results that are written over the rows take two kernels.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 

@@ -11,7 +11,10 @@
 // weights are split among the SMs at multiples of 8 rows (up) or 256 columns of K (down; few_rows.cuh).  The second kernel
 // starts as SMs become free and has its first weights on the way before the first one has finished: only h has to be waited
 // for.  The gate weight is applied to h, before its rounding, so that the down product can add a token's experts in its
-// accumulators: the rounding is relative, and the same as without it.
+// accumulators: the rounding is relative, and the same as without it.  h is rounded because the tensor cores take 16 bits: a second
+// bf16 term for the rest would double h and the multiplications of the down product, which 32 and 64 tokens are near to being
+// bound by.  It costs as much as the rounding of the result: 0.0024 of a result's size (root mean square) against 64 bits, where the
+// last rounding alone leaves 0.0017, as in the layer's general path.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
@@ -577,7 +580,7 @@ cudaError_t launch_ring(FewArgs a, int tile, size_t row_bytes, size_t sums, int 
   const size_t smem = ring_room(sizeof(Shared<MAX>));
   a.tile = tile;
   // A second buffer for the sums saves a barrier at the end of every piece and costs half a stage.  Up to 16 tokens and pieces of at
-  // most 8 steps gain (31 tokens of 128 experts, 512 / 1024: 98.5 -> 91.5 us; 16 tokens of 8, 4096 / 14336: 421 -> 413), long pieces
+  // most 8 steps gain (31 tokens of 128 experts, 512 / 1024: 98.5 -> 91.5 us; 16 tokens of 8, 4096 / 14336: 421 -> 411), long pieces
   // with more tokens lose (64 tokens: 468 -> 512).
   a.red = MAX == 16 || row_bytes <= 8 * kChunk ? 2 * kRedBytes : kRedBytes;
   a.room = (int)(smem - 1024 /*alignment*/ - a.red - sums);

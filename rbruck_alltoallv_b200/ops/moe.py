@@ -306,8 +306,8 @@ def grouped_gemm_int8(Aq: torch.Tensor, a_scale: torch.Tensor, Bq: torch.Tensor,
     ``Aq`` [M, K] int8 with ``a_scale`` [M], ``Bq`` [G, N, K] int8 with ``b_scale`` [G, N], ``group_start`` / ``group_rows`` int32
     CUDA tensors [G], G <= 64; N a multiple of 8, K of 16.  With ``swiglu`` the rows of ``Bq[g]`` interleave gate and up projections
     and ``out`` is [M, N // 2].  Rows of ``out`` outside the groups are left as they are; rows of a group beyond the end of ``Aq``, and
-    a group that starts before it, are left out and recorded as error 6 in ``error`` (int32 CUDA tensor, optional).  ``out`` shares no
-    memory with an operand."""
+    a group that starts before it, are left out and recorded as error 6 in ``error`` (int32 CUDA tensor, optional; 1 to 3: a bounded
+    wait ran out and rows are missing; nothing else tells).  ``out`` shares no memory with an operand."""
     return _native.torch_ops().grouped_gemm_int8(Aq, a_scale, Bq, b_scale, group_start, group_rows, out, swiglu, error, max_ctas)
 
 
@@ -319,7 +319,8 @@ def linear_int8(x: torch.Tensor, weight: torch.Tensor, scale: torch.Tensor, out:
     ``x`` [rows, K] bf16, ``weight`` [N, K] int8 and ``scale`` [N] fp32 (:func:`quantize_weight_int8`), ``out`` [rows, N] bf16; N a
     multiple of 8, K of 16.  Up to 64 rows the weights are streamed past the rows, split evenly among the SMs
     (``csrc/kernels/linear_int8_few.cu``); more rows go through the grouped GEMM as one group.  ``out``
-    may be ``x`` itself, or share memory with it (but not with the weights).  A row that holds an infinity or a NaN becomes NaN.  No backward pass (rows and scales that require a gradient are refused)."""
+    may be ``x`` itself, or share memory with it (but not with the weights).  A row that holds an infinity or a NaN becomes NaN.  No backward pass (rows and scales that require a gradient are refused).  ``error`` as in
+    :func:`grouped_gemm_int8`."""
     return _native.torch_ops().linear_int8(x, weight, scale, out, error)
 
 
@@ -345,10 +346,11 @@ def moe_few_tokens(x: torch.Tensor, logits: torch.Tensor, w13: torch.Tensor, w2:
     ``top_k`` is spread over those, and one without any other gets a row of zeros (a padded slot of a batch).  A NaN or +inf among
     a token's logits makes its row NaN.  The number of tokens may change from call to call; weights are read for the experts that
     some token chooses, once each.  The weights are taken to be finite: one that is
-    not spoils the row of every token of a call that reads it.  No backward pass (inputs and weights that require a gradient are
+    not spoils the row of every token of a call that reads it.  The FFN's intermediate is rounded to bf16 (as in
+    :meth:`MoEExpertParallel.forward`), sums and weights are held in 32 bits.  No backward pass (inputs and weights that require a gradient are
     refused, but under ``torch.no_grad()``).
     ``out`` may be ``x`` itself, but shares no memory with the logits or the weights.  ``error`` (int32 CUDA tensor): set to non-zero
-    if a bounded wait ran out."""
+    if a bounded wait ran out, which makes the results garbage; nothing else tells."""
     return _native.torch_ops().moe_few_tokens(x, logits, w13, w2, top_k, out, error)
 
 
@@ -548,9 +550,9 @@ class MoEExpertParallel:
     def decode(self, x: torch.Tensor, logits: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """The layer for a batch of decoded tokens: any number of them up to :data:`FEW_TOKENS`, whatever ``tokens`` the layer
         was made for, in two kernels (:func:`moe_few_tokens`).  bf16 experts on one rank.  Up to 16 tokens it takes less time than
-        :meth:`forward` (8 experts, 4096 / 14336: 1 token 115 against 141 us, 16 tokens 406 against 434; 64 experts, 2048 / 1408:
-        1 token 14 against 45 us, 16 tokens 83 against 90), for 32 about the same (420 against 440, 133 against 132), for 64 a
-        tenth more (475 against 434, 184 against 166)."""
+        :meth:`forward` (8 experts, 4096 / 14336: 1 token 112 against 138 us, 16 tokens 414 against 438; 64 experts, 2048 / 1408:
+        1 token 14 against 40 us, 16 tokens 82 against 91), for 32 about the same (433 against 440, 128 against 127), for 64 more
+        (506 against 440, 182 against 165)."""
         if self.P != 1 or self.fp8:
             raise ValueError("decode() is for bf16 experts on one rank")
         return moe_few_tokens(x, logits, self.w13, self.w2, 2, out, self.error[1:2])
