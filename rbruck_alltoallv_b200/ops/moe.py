@@ -318,9 +318,9 @@ def linear_int8(x: torch.Tensor, weight: torch.Tensor, scale: torch.Tensor, out:
 
     ``x`` [rows, K] bf16, ``weight`` [N, K] int8 and ``scale`` [N] fp32 (:func:`quantize_weight_int8`), ``out`` [rows, N] bf16; N a
     multiple of 8, K of 16.  Up to 64 rows the weights are streamed past the rows, split evenly among the SMs
-    (``csrc/kernels/linear_int8_few.cu``); more rows go through the grouped GEMM as one group.  ``out``
-    may be ``x`` itself, or share memory with it (but not with the weights).  A row that holds an infinity or a NaN becomes NaN.  No backward pass (rows and scales that require a gradient are refused).  ``error`` as in
-    :func:`grouped_gemm_int8`."""
+    (``csrc/kernels/linear_int8_few.cu``); more rows go through the grouped GEMM as one group.  ``out`` may be ``x`` itself, or share
+    memory with it (but not with the weights).  A row that holds an infinity or a NaN becomes NaN.  No backward pass (rows and
+    scales that require a gradient are refused).  ``error`` as in :func:`grouped_gemm_int8`."""
     return _native.torch_ops().linear_int8(x, weight, scale, out, error)
 
 
@@ -347,9 +347,8 @@ def moe_few_tokens(x: torch.Tensor, logits: torch.Tensor, w13: torch.Tensor, w2:
     a token's logits makes its row NaN.  The number of tokens may change from call to call; weights are read for the experts that
     some token chooses, once each.  The weights are taken to be finite: one that is
     not spoils the row of every token of a call that reads it.  The FFN's intermediate is rounded to bf16 (as in
-    :meth:`MoEExpertParallel.forward`), sums and weights are held in 32 bits.  No backward pass (inputs and weights that require a gradient are
-    refused, but under ``torch.no_grad()``).
-    ``out`` may be ``x`` itself, but shares no memory with the logits or the weights.  ``error`` (int32 CUDA tensor): set to non-zero
+    :meth:`MoEExpertParallel.forward`), sums and softmax are held in 32 bits.  No backward pass (inputs and weights that require a
+    gradient are refused, but under ``torch.no_grad()``).  ``out`` may be ``x`` itself, but shares no memory with the logits or the weights.  ``error`` (int32 CUDA tensor): set to non-zero
     if a bounded wait ran out, which makes the results garbage; nothing else tells."""
     return _native.torch_ops().moe_few_tokens(x, logits, w13, w2, top_k, out, error)
 
