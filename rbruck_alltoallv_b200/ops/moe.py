@@ -354,7 +354,8 @@ def moe_few_tokens(x: torch.Tensor, logits: torch.Tensor, w13: torch.Tensor, w2:
 
 
 class MoEExpertParallel:
-    """One MoE FFN layer sharded by experts over the ranks of a communicator (one rank per GPU)."""
+    """One MoE FFN layer sharded by experts over the ranks of a communicator (one rank per GPU).  For inference: there is no backward
+    pass, and the result of :meth:`forward` has no graph, whatever its inputs require."""
 
     def __init__(self, comm, num_experts: int, hidden: int, inter: int, tokens: int, capacity_factor: float = 2.0,
                  seed: int = 0, init_std: float = 0.02, fp8: bool = False, overlap: Optional[bool] = None,
